@@ -64,7 +64,7 @@ PS_API const char* ps_last_error(void);
 PS_API uint64_t ps_launch_count(void);
 /* Reads (and with clear != 0, clears) the current device's status word after
  * synchronising `stream`. *code receives 0 or a device error code
- * (1 block id, 2 slot, 3 token id, 4 wait timeout, 5 metadata). */
+ * (1 block id, 2 slot, 3 token id, 4 wait timeout, 5 metadata, 6 free blocks). */
 PS_API int ps_device_status(int* code, int clear, ps_stream_t stream);
 
 /* ------------------------------------------------------- (a1) KV writes */
@@ -252,6 +252,83 @@ PS_API int ps_topk(float* vals_dev, int32_t* idx_dev, const void* logits_dev, in
  * exceeds u * sum(p)], u = uniforms_dev[row] in [0, 1). temperature > 0. */
 PS_API int ps_sample_topk(int32_t* out_dev, const float* vals_dev, const int32_t* idx_dev, const float* uniforms_dev,
                           int M, int k, float temperature, ps_stream_t stream);
+
+/* ----------------------------------------- (g) trees of drafted tokens
+ *
+ * Several drafted continuations of a sequence, verified in one step. The
+ * step's new tokens of request b are rows [cu_q[b], cu_q[b+1]); row i of a
+ * request is stored at cache position seq + i and is a node of a tree: its
+ * parent is an earlier row of the same request (-1: none; row 0, the last
+ * confirmed token, is the root). Mask rows are words = ceil(max_q_len / 64)
+ * int64 words; bit j % 64 of word j / 64 says that node j is an ancestor of
+ * the node, or the node itself. At most 256 nodes per request. No counterpart
+ * in the reference, which feeds one token per sequence and step
+ * (engine/runner.py:65-79). */
+
+/* Block tables, positions, slots and masks of a step, from lengths on the
+ * device. For request b with seq_lens[b] tokens cached, q_lens[b] new ones and
+ * held[b] blocks in its row of tables_in:
+ *   need = ceil((seq + q) / block_size), take = max(0, need - held), the
+ *   requests take from free_blocks in their order;
+ *   tables[b] = the held entries, the taken blocks, -1 behind (tables may be
+ *   tables_in itself); held_out[b] = the entries the row now has;
+ *   cu_q int32 [num_seqs + 1]; for its rows positions = seq + i (with parents:
+ *   seq + the node's depth), slots = table[(seq + i) / bs] * bs + (seq + i) % bs.
+ *   parents int32 [total_tokens] or NULL (an ordinary chunk: no masks);
+ *   tree_mask int64 [total_tokens][words].
+ * Rows of [cu_q[num_seqs], total_tokens) get position 0, slot -1, mask 0.
+ * *free_used = the blocks that the step wants; above num_free the entries and
+ * slots that got none are -1, held_out counts the blocks that were given, and
+ * error 6 is recorded. Lengths below 0, rows past total_tokens, contexts past
+ * the table and parents outside [-1, i) are recorded as error 5 and handled as
+ * 0, cut off, slot -1 and -1. held_out must not alias held, seq_lens, q_lens. */
+PS_API int ps_build_step_tables(int32_t* tables_dev, int32_t* held_out_dev, int32_t* cu_q_dev, int32_t* positions_dev,
+                                int32_t* slots_dev, int64_t* tree_mask_dev, int32_t* free_used_dev,
+                                const int32_t* tables_in_dev, const int32_t* held_dev, const int32_t* seq_lens_dev,
+                                const int32_t* q_lens_dev, const int32_t* free_blocks_dev, const int32_t* parents_dev,
+                                int num_seqs, int total_tokens, int max_q_len, int max_blocks_per_seq, int num_free,
+                                int num_blocks, int block_size, ps_stream_t stream);
+
+/* Scratch bytes ps_tree_attention needs (any contents; one buffer per stream);
+ * 0 for arguments that it rejects. */
+PS_API size_t ps_tree_attention_workspace_size(int num_seqs, int max_q_len, int max_ctx, int num_q_heads,
+                                               int num_kv_heads, int head_dim);
+
+/* ps_paged_attention with the tree's rule in place of the causal one: node i
+ * of request b sees the cached keys [0, start_pos[b]) and the nodes of its mask
+ * row; its output is 0 when that is nothing. What a node does not see does not
+ * reach it, whatever the cache holds there. The K/V of the new tokens are in
+ * the cache already. Rows behind cu_q[num_seqs] are left as they were.
+ * max_q_len <= 256 and max_ctx are host bounds; a request beyond them is
+ * skipped and recorded (error 5). head_dim 64 or 128, PS_BF16 or PS_F16, any
+ * block size; q, out and the caches 16-byte aligned. */
+PS_API int ps_tree_attention(void* out_dev, const void* q_dev, const void* k_cache_dev, const void* v_cache_dev,
+                             const int32_t* block_tables_dev, int max_blocks_per_seq, const int32_t* cu_q_dev,
+                             const int32_t* start_pos_dev, const int64_t* tree_mask_dev, int num_seqs, int total_q,
+                             int max_q_len, int max_ctx, int num_blocks, int block_size, int num_q_heads,
+                             int num_kv_heads, int head_dim, int dtype, void* workspace_dev, size_t workspace_bytes,
+                             ps_stream_t stream);
+
+/* The longest path of each tree that the model agrees with, and the move of its
+ * K/V. tokens int64 [total_tokens]: the rows' token ids; targets int32
+ * [total_tokens]: the model's next token after each row (ps_argmax). Node 0 is
+ * accepted; node i > 0 is if its parent (the highest node below i in its mask
+ * row) and all of its mask row are, and tokens[i] == targets[parent]. The path
+ * is the mask row of the accepted node with most ancestors (the lowest such
+ * node), ascending:
+ *   num[b] = its length (0 for a request without rows), nodes[b] = the path,
+ *   out_tokens[b] = targets along it (the tokens the step yields), both int32
+ *   [num_seqs][max_q_len] padded with -1, start_out[b] = start_pos[b] + num[b];
+ *   in both caches ([num_layers][num_blocks][block_size][num_kv_heads][head_dim],
+ *   dtype PS_BF16 / PS_F16 / PS_F32; both NULL: no move) the rows at positions
+ *   start + path[k] move to start + k. Rows behind start_out are left over.
+ * num and start_out must not alias start_pos or cu_q. max_q_len <= 256. */
+PS_API int ps_accept_trees(int32_t* num_dev, int32_t* nodes_dev, int32_t* out_tokens_dev, int32_t* start_out_dev,
+                           const int64_t* tokens_dev, const int32_t* targets_dev, const int64_t* tree_mask_dev,
+                           const int32_t* cu_q_dev, const int32_t* start_pos_dev, int num_seqs, int total_tokens,
+                           int max_q_len, void* k_cache_dev, void* v_cache_dev, const int32_t* block_tables_dev,
+                           int max_blocks_per_seq, int num_layers, int num_blocks, int block_size, int num_kv_heads,
+                           int head_dim, int dtype, ps_stream_t stream);
 
 /* ------------------------------------- (e) fused tensor-parallel all-reduce
  *

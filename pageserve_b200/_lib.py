@@ -23,7 +23,8 @@ PS_F32, PS_BF16, PS_F16, PS_I8 = 0, 1, 2, 3
 PS_OK, PS_ERR_INVALID, PS_ERR_INDEX, PS_ERR_CUDA, PS_ERR_UNSUPPORTED, PS_ERR_DEVICE, PS_ERR_TIMEOUT = range(7)
 
 DEVICE_ERRORS = {1: "block id outside the KV pool", 2: "slot outside the cache", 3: "token id outside the vocabulary",
-                 4: "bounded device wait timed out", 5: "per-sequence metadata inconsistent with launch bounds"}
+                 4: "bounded device wait timed out", 5: "per-sequence metadata inconsistent with launch bounds",
+                 6: "free block list too short for the step"}
 
 _P = c_void_p
 _I = c_int
@@ -70,6 +71,11 @@ _SIGNATURES = {
     "ps_copy_kv_blocks": (c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "ps_topk": (c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "ps_sample_topk": (c_int, [_P, _P, _P, _P, _I, _I, c_float, _P]),
+    "ps_build_step_tables": (c_int, [_P] * 13 + [_I] * 7 + [_P]),
+    "ps_tree_attention_workspace_size": (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "ps_tree_attention": (c_int, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P,
+                                  c_size_t, _P]),
+    "ps_accept_trees": (c_int, [_P] * 9 + [_I, _I, _I, _P, _P, _P] + [_I] * 7 + [_P]),
 }
 
 _lock = threading.Lock()

@@ -26,6 +26,7 @@ enum DeviceError : int {
   kErrTokenId = 3,      // embedding id outside [0, vocab)
   kErrTimeout = 4,      // a bounded spin-wait gave up
   kErrShape = 5,        // per-sequence metadata inconsistent with launch bounds
+  kErrNoBlocks = 6,     // the list of free blocks is too short for the step
 };
 
 // ----------------------------------------------------------------- types --
@@ -184,4 +185,4 @@ inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<u
 }  // namespace ps_host
 
 // Translation-unit ids for the device status words.
-enum PsUnit { PS_TU_KV = 0, PS_TU_ATTN = 1, PS_TU_GEMV = 2, PS_TU_GEMM = 3, PS_TU_MISC = 4, PS_TU_COMM = 5, PS_TU_COUNT = 6 };
+enum PsUnit { PS_TU_KV = 0, PS_TU_ATTN = 1, PS_TU_GEMV = 2, PS_TU_GEMM = 3, PS_TU_MISC = 4, PS_TU_COMM = 5, PS_TU_TREE = 6, PS_TU_COUNT = 7 };
