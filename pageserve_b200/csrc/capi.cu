@@ -50,6 +50,16 @@ int* status_word(int tu) {
   return g_status[dev] + tu;
 }
 
+bool reserve_smem(const void* kern, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+  const uint64_t bit = 1ull << dev;
+  if (done->load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 bool pdl_enabled() {
   static const bool v = [] {
     const char* e = std::getenv("PS_PDL");

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pageserve_b200.h"
 
 #define PS_DEVICE __device__ __forceinline__
@@ -180,6 +182,9 @@ void set_error(const char* fmt, ...);
 int check_launch(const char* what);
 void count_launch(int n = 1);
 int* status_word(int tu);  // device status word of translation unit `tu`
+// Raise `kern`'s dynamic shared-memory limit to `bytes` on the current device;
+// `done` (one per kernel, zeroed) remembers the devices where that was done.
+bool reserve_smem(const void* kern, int bytes, std::atomic<uint64_t>* done);
 // true for NULL or a pointer aligned to `bytes` (vector loads need it)
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 }  // namespace ps_host

@@ -548,7 +548,8 @@ template <typename T, int D>
 int launch_mma(TreeParams& p, cudaStream_t s) {
   auto kern = tree_mma_kernel<T, D>;
   const int smem = kStages * 2 * kKeys * D * 2;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+  static std::atomic<uint64_t> done{0};
+  if (!ps_host::reserve_smem(reinterpret_cast<const void*>(kern), smem, &done)) {
     ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", smem);
     return PS_ERR_CUDA;
   }

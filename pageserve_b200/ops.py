@@ -18,7 +18,8 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libpageserve_torch_ops.so"
 
 OPS = ("write_kv", "paged_attention", "quantize_per_channel", "tile_int8_weight", "w8a16_linear", "linear16",
-       "linear_swiglu", "rms_norm", "add_rms_norm", "apply_rope", "embedding", "argmax", "topk", "copy_kv_blocks")
+       "linear_swiglu", "rms_norm", "add_rms_norm", "apply_rope", "embedding", "argmax", "topk", "copy_kv_blocks",
+       "build_step_tables", "build_step_tables_out", "tree_attention", "tree_attention_out", "accept_trees")
 
 _loaded = False
 

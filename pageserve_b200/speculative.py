@@ -51,22 +51,19 @@ class Accepted(NamedTuple):
     start_pos: torch.Tensor  # (B,) tokens in the cache after the step
 
 
-def _int32(name: str, device: torch.device, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise TypeError(f"{name}: metadata must be contiguous int32")
-        if t.device != device:
-            raise ValueError(f"{name}: tensors on different devices ({t.device}, {device})")
+_ops = None
 
 
-def _mask_words(name: str, tree_mask: torch.Tensor, rows: int, max_q_len: int, device: torch.device) -> None:
-    if tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous():
-        raise TypeError(f"{name}: tree_mask must be contiguous int64")
-    if tree_mask.device != device:
-        raise ValueError(f"{name}: tensors on different devices ({tree_mask.device}, {device})")
-    if tree_mask.dim() != 2 or tree_mask.shape[0] < rows or tree_mask.shape[1] != (max_q_len + 63) // 64:
-        raise ValueError(f"{name}: tree_mask {tuple(tree_mask.shape)} does not hold {rows} rows of "
-                         f"{(max_q_len + 63) // 64} words")
+def _op(name: str):
+    """The torch operator (torch_ops/pageserve_ops.cpp: the argument checks,
+    the output allocations and the C call of each function below)."""
+    global _ops
+    if _ops is None:
+        from . import ops
+        ns = ops.load()
+        _ops = {n: getattr(ns, n).default for n in ("build_step_tables", "build_step_tables_out", "tree_attention",
+                                                    "tree_attention_out", "accept_trees")}
+    return _ops[name]
 
 
 def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
@@ -86,43 +83,16 @@ def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables
     the tables; it may be block_tables itself. A free list that is too short
     leaves -1 entries and slots, free_used above F and device error 6; lengths
     beyond the given bounds are device error 5 (``_lib.raise_on_device_error``)."""
-    _lib.require_cuda(seq_lens, q_lens, block_tables, held, free_blocks, parents, out)
-    dev = seq_lens.device
-    _int32("build_step_tables", dev, seq_lens, q_lens, block_tables, held, free_blocks)
-    B = seq_lens.numel()
-    if B == 0:
-        raise ValueError("build_step_tables: empty batch")
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or q_lens.numel() != B or held.numel() != B:
-        raise ValueError("build_step_tables: q_lens, held and block_tables need one entry per request")
-    width = block_tables.shape[1]
+    _lib.require_cuda(seq_lens)
     if out is None:
-        tables = torch.empty_like(block_tables)
+        r = _op("build_step_tables")(seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
+                                     total_tokens, parents, max_q_len)
     else:
-        _int32("build_step_tables", dev, out)
-        if out.shape != block_tables.shape:
-            raise ValueError("build_step_tables: out must have block_tables' shape")
-        tables = out
-    T = int(total_tokens)
-    if T < 0:
-        raise ValueError("build_step_tables: total_tokens below 0")
-    mask = None
-    if parents is not None:
-        _int32("build_step_tables", dev, parents)
-        if parents.numel() < T:
-            raise ValueError(f"build_step_tables: {parents.numel()} parents for {T} rows")
-        if max_q_len is None:
-            raise ValueError("build_step_tables: max_q_len bounds the trees; pass it with parents")
-        mask = torch.empty((T, (max_q_len + 63) // 64), dtype=torch.int64, device=dev)
-    # one allocation for the small int32 outputs
-    buf = torch.empty(2 * B + 2 + 2 * T, dtype=torch.int32, device=dev)
-    held_out, cu_q, used, positions, slots = buf.split([B, B + 1, 1, T, T])
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().ps_build_step_tables(
-            tables.data_ptr(), held_out.data_ptr(), cu_q.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-            _lib.ptr(mask), used.data_ptr(), block_tables.data_ptr(), held.data_ptr(), seq_lens.data_ptr(),
-            q_lens.data_ptr(), free_blocks.data_ptr(), _lib.ptr(parents), B, T, max_q_len or 0, width,
-            free_blocks.numel(), num_blocks, block_size, _lib.stream_ptr(dev)), "build_step_tables")
-    return StepTables(tables, held_out, cu_q, positions, slots, mask, used)
+        r = (out, *_op("build_step_tables_out")(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks,
+                                                block_size, total_tokens, parents, max_q_len))
+    if parents is None:
+        r = (*r[:5], None, r[6])
+    return StepTables._make(r)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -136,39 +106,17 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     Rows of ``out`` behind cu_q[-1] are left as they were. A workspace serves
     calls on one stream at a time; without one the scratch is allocated per
     call."""
-    _lib.require_cuda(q, k_cache, v_cache, block_tables, cu_q, start_pos, tree_mask, out)
-    if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2:
-        raise ValueError("tree_attention: q (T, Hq, D), caches (NB, bs, Hkv, D), block_tables (B, max_blocks)")
-    dev = q.device
-    total_q, hq, d = q.shape
-    nb, bs, hkv, d2 = k_cache.shape
-    if d2 != d or v_cache.shape != k_cache.shape:
-        raise ValueError("tree_attention: cache / query head_dim mismatch")
-    if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype:
-        raise TypeError("tree_attention: q and cache dtypes differ")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("tree_attention: the caches must be contiguous")
-    if k_cache.device != dev or v_cache.device != dev:
-        raise ValueError("tree_attention: tensors on different devices")
-    _int32("tree_attention", dev, block_tables, cu_q, start_pos)
-    B = start_pos.numel()
-    if block_tables.shape[0] != B or cu_q.numel() != B + 1:
-        raise ValueError("tree_attention: block_tables, cu_q and start_pos disagree on the batch")
-    _mask_words("tree_attention", tree_mask, total_q, max_q_len, dev)
-    q = q.contiguous()
+    _lib.require_cuda(q)
+    buf = None
+    if workspace is not None:
+        B, (_, hq, d), hkv = start_pos.numel(), q.shape, k_cache.shape[-2]
+        nbytes = _lib.load().ps_tree_attention_workspace_size(B, max_q_len, max_ctx, hq, hkv, d)
+        buf = workspace.get(nbytes, q.device)
     if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
-        raise ValueError("tree_attention: out must be contiguous, with q's shape, dtype and device")
-    lib = _lib.load()
-    nbytes = lib.ps_tree_attention_workspace_size(B, max_q_len, max_ctx, hq, hkv, d)
-    buf = (workspace or AttentionWorkspace()).get(nbytes, dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.ps_tree_attention(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                         block_tables.data_ptr(), block_tables.shape[1], cu_q.data_ptr(),
-                                         start_pos.data_ptr(), tree_mask.data_ptr(), B, total_q, max_q_len, max_ctx,
-                                         nb, bs, hq, hkv, d, _lib.dtype_code(q.dtype), _lib.ptr(buf), nbytes,
-                                         _lib.stream_ptr(dev)), "tree_attention")
+        return _op("tree_attention")(q, k_cache, v_cache, block_tables, cu_q, start_pos, tree_mask, max_q_len, max_ctx,
+                                     buf)
+    _op("tree_attention_out")(out, q, k_cache, v_cache, block_tables, cu_q, start_pos, tree_mask, max_q_len, max_ctx,
+                              buf)
     return out
 
 
@@ -184,41 +132,6 @@ def accept_trees(tokens: torch.Tensor, targets: torch.Tensor, tree_mask: torch.T
     tokens the step yields. With the caches ((L, NB, bs, Hkv, D), or one
     layer's (NB, bs, Hkv, D)) and block_tables, the path's keys and values move
     in place to the positions start_pos, start_pos + 1, ..."""
-    _lib.require_cuda(tokens, targets, tree_mask, cu_q, start_pos, k_cache, v_cache, block_tables)
-    dev = tokens.device
-    _int32("accept_trees", dev, targets, cu_q, start_pos)
-    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
-        raise TypeError("accept_trees: tokens must be contiguous int64")
-    T, B = tokens.numel(), start_pos.numel()
-    if targets.numel() != T or cu_q.numel() != B + 1:
-        raise ValueError("accept_trees: one target per token and one start position per request are needed")
-    if B == 0:
-        raise ValueError("accept_trees: empty batch")
-    _mask_words("accept_trees", tree_mask, T, max_q_len, dev)
-    L = nb = bs = hkv = d = width = code = 0
-    if k_cache is not None or v_cache is not None:
-        if k_cache is None or v_cache is None or block_tables is None:
-            raise ValueError("accept_trees: the move needs both caches and block_tables")
-        if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-            raise ValueError("accept_trees: K and V caches differ in shape or dtype")
-        if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or k_cache.device != dev or \
-                v_cache.device != dev:
-            raise ValueError("accept_trees: the caches must be contiguous and on the tokens' device")
-        _int32("accept_trees", dev, block_tables)
-        if block_tables.dim() != 2 or block_tables.shape[0] != B:
-            raise ValueError("accept_trees: block_tables needs one row per request")
-        if k_cache.dim() not in (4, 5):
-            raise ValueError("accept_trees: caches are (L, NB, bs, Hkv, D) or one layer's (NB, bs, Hkv, D)")
-        L = k_cache.shape[0] if k_cache.dim() == 5 else 1
-        nb, bs, hkv, d = k_cache.shape[-4:]
-        width = block_tables.shape[1]
-        code = _lib.dtype_code(k_cache.dtype)
-    num, start, nodes, out = torch.empty(2 * B + 2 * B * max_q_len, dtype=torch.int32, device=dev).split(
-        [B, B, B * max_q_len, B * max_q_len])
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().ps_accept_trees(
-            num.data_ptr(), nodes.data_ptr(), out.data_ptr(), start.data_ptr(), tokens.data_ptr(), targets.data_ptr(),
-            tree_mask.data_ptr(), cu_q.data_ptr(), start_pos.data_ptr(), B, T, max_q_len, _lib.ptr(k_cache),
-            _lib.ptr(v_cache), _lib.ptr(block_tables), width, L, nb, bs, hkv, d, code, _lib.stream_ptr(dev)),
-            "accept_trees")
-    return Accepted(num, nodes.view(B, max_q_len), out.view(B, max_q_len), start)
+    _lib.require_cuda(tokens)
+    return Accepted._make(_op("accept_trees")(tokens, targets, tree_mask, cu_q, start_pos, max_q_len, k_cache, v_cache,
+                                              block_tables))

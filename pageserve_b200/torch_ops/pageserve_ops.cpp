@@ -224,6 +224,204 @@ void copy_kv_blocks(at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& pa
         "copy_kv_blocks");
 }
 
+// ------------------------------------------------- trees of drafted tokens --
+// The checks live here, with the Python exception types of _lib.check, so that
+// pageserve_b200/speculative.py adds little to a call.
+
+void check_v(int rc, const char* what) {
+  TORCH_CHECK_VALUE(rc != PS_ERR_INVALID, what, ": ", ps_last_error());
+  check(rc, what);
+}
+
+void on_device(const at::Tensor& t, const at::Device& dev, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "pageserve_b200 kernels run on CUDA tensors only (no CPU fallback); got a tensor on ",
+              t.device());
+  TORCH_CHECK_VALUE(t.device() == dev, what, ": tensors on different devices (", t.device(), ", ", dev, ")");
+}
+
+void metadata(const at::Tensor& t, const at::Device& dev, const char* what) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt && t.is_contiguous(), what, ": metadata must be contiguous int32");
+  on_device(t, dev, what);
+}
+
+void cache_like(const at::Tensor& k, const at::Tensor& v, const at::Device& dev, const char* what) {
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), what, ": K and V caches differ in shape");
+  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), what, ": K and V caches differ in dtype");
+  TORCH_CHECK_VALUE(k.is_contiguous() && v.is_contiguous(), what, ": the caches must be contiguous");
+  on_device(k, dev, what);
+  on_device(v, dev, what);
+}
+
+void mask_words(const at::Tensor& m, int64_t rows, int64_t max_q_len, const at::Device& dev, const char* what) {
+  TORCH_CHECK_TYPE(m.scalar_type() == at::kLong && m.is_contiguous(), what, ": tree_mask must be contiguous int64");
+  on_device(m, dev, what);
+  const int64_t words = (max_q_len + 63) / 64;
+  TORCH_CHECK_VALUE(m.dim() == 2 && m.size(0) >= rows && m.size(1) == words, what, ": tree_mask ", m.sizes(),
+                    " does not hold ", rows, " rows of ", words, " words");
+}
+
+int int_arg(int64_t v, const char* what) {
+  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": ", v, " does not fit 32 bits");
+  return static_cast<int>(v);
+}
+
+using StepOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
+                              const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
+                              int64_t num_blocks, int64_t block_size, int64_t total_tokens,
+                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+  constexpr const char* what = "build_step_tables";
+  const at::Device dev = seq_lens.device();
+  metadata(seq_lens, dev, what);
+  metadata(q_lens, dev, what);
+  metadata(block_tables, dev, what);
+  metadata(held, dev, what);
+  metadata(free_blocks, dev, what);
+  metadata(out, dev, what);
+  const int64_t B = seq_lens.numel(), T = total_tokens;
+  TORCH_CHECK_VALUE(B > 0, what, ": empty batch");
+  TORCH_CHECK_VALUE(T >= 0, what, ": total_tokens below 0");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.size(0) == B && q_lens.numel() == B && held.numel() == B,
+                    what, ": q_lens, held and block_tables need one entry per request");
+  TORCH_CHECK_VALUE(out.sizes() == block_tables.sizes(), what, ": out must have block_tables' shape");
+  int64_t words = 0;
+  if (parents.has_value()) {
+    metadata(*parents, dev, what);
+    TORCH_CHECK_VALUE(parents->numel() >= T, what, ": ", parents->numel(), " parents for ", T, " rows");
+    TORCH_CHECK_VALUE(max_q_len.has_value(), what, ": max_q_len bounds the trees; pass it with parents");
+    words = (std::max<int64_t>(*max_q_len, 0) + 63) / 64;
+  }
+  c10::cuda::CUDAGuard g(dev);
+  const auto i32 = seq_lens.options();
+  at::Tensor held_out = at::empty({B}, i32), cu_q = at::empty({B + 1}, i32), used = at::empty({1}, i32);
+  at::Tensor positions = at::empty({T}, i32), slots = at::empty({T}, i32);
+  at::Tensor mask = parents.has_value() ? at::empty({T, words}, i32.dtype(at::kLong)) : at::empty({0}, i32.dtype(at::kLong));
+  check_v(ps_build_step_tables(out.data_ptr<int32_t>(), held_out.data_ptr<int32_t>(), cu_q.data_ptr<int32_t>(),
+                               positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
+                               parents.has_value() ? mask.data_ptr<int64_t>() : nullptr, used.data_ptr<int32_t>(),
+                               block_tables.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
+                               seq_lens.data_ptr<int32_t>(), q_lens.data_ptr<int32_t>(),
+                               free_blocks.data_ptr<int32_t>(),
+                               parents.has_value() ? parents->data_ptr<int32_t>() : nullptr, int_arg(B, what),
+                               int_arg(T, what), int_arg(max_q_len.value_or(0), what),
+                               int_arg(block_tables.size(1), what), int_arg(free_blocks.numel(), what),
+                               int_arg(num_blocks, what), int_arg(block_size, what), stream_of(seq_lens)),
+          what);
+  return {held_out, cu_q, positions, slots, mask, used};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_step_tables(
+    const at::Tensor& seq_lens, const at::Tensor& q_lens, const at::Tensor& block_tables, const at::Tensor& held,
+    const at::Tensor& free_blocks, int64_t num_blocks, int64_t block_size, int64_t total_tokens,
+    const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+  at::Tensor out = at::empty(block_tables.sizes(), block_tables.options());
+  auto r = build_step_tables_out(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
+                                 total_tokens, parents, max_q_len);
+  return {out, std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r), std::get<5>(r)};
+}
+
+void tree_attention_out(at::Tensor out, const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                        const at::Tensor& block_tables, const at::Tensor& cu_q, const at::Tensor& start_pos,
+                        const at::Tensor& tree_mask, int64_t max_q_len, int64_t max_ctx,
+                        const c10::optional<at::Tensor>& workspace) {
+  constexpr const char* what = "tree_attention";
+  TORCH_CHECK_VALUE(q_in.dim() == 3 && k_cache.dim() == 4 && block_tables.dim() == 2, what,
+                    ": q (T, Hq, D), caches (NB, bs, Hkv, D), block_tables (B, max_blocks)");
+  const at::Device dev = q_in.device();
+  const int64_t T = q_in.size(0), Hq = q_in.size(1), D = q_in.size(2), B = start_pos.numel();
+  TORCH_CHECK_VALUE(k_cache.size(3) == D, what, ": cache / query head_dim mismatch");
+  TORCH_CHECK_TYPE(q_in.scalar_type() == k_cache.scalar_type(), what, ": q and cache dtypes differ");
+  cache_like(k_cache, v_cache, dev, what);
+  metadata(block_tables, dev, what);
+  metadata(cu_q, dev, what);
+  metadata(start_pos, dev, what);
+  TORCH_CHECK_VALUE(block_tables.size(0) == B && cu_q.numel() == B + 1, what,
+                    ": block_tables, cu_q and start_pos disagree on the batch");
+  mask_words(tree_mask, T, max_q_len, dev, what);
+  TORCH_CHECK_VALUE(out.sizes() == q_in.sizes() && out.is_contiguous() && out.device() == dev &&
+                        out.scalar_type() == q_in.scalar_type(),
+                    what, ": out must be contiguous, with q's shape, dtype and device");
+  c10::cuda::CUDAGuard g(dev);
+  const at::Tensor q = q_in.contiguous();
+  const int nb = int_arg(k_cache.size(0), what), bs = int_arg(k_cache.size(1), what);
+  const int hq = int_arg(Hq, what), hkv = int_arg(k_cache.size(2), what), d = int_arg(D, what);
+  const int mq = int_arg(max_q_len, what), mc = int_arg(max_ctx, what), b = int_arg(B, what);
+  const size_t bytes = ps_tree_attention_workspace_size(b, mq, mc, hq, hkv, d);
+  at::Tensor ws;
+  if (workspace.has_value()) {
+    on_device(*workspace, dev, what);
+    TORCH_CHECK_VALUE(workspace->is_contiguous(), what, ": the workspace must be contiguous");
+    ws = *workspace;
+  } else {
+    ws = at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, q.options().dtype(at::kByte));
+  }
+  check_v(ps_tree_attention(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                            block_tables.data_ptr<int32_t>(), int_arg(block_tables.size(1), what),
+                            cu_q.data_ptr<int32_t>(), start_pos.data_ptr<int32_t>(), tree_mask.data_ptr<int64_t>(), b,
+                            int_arg(T, what), mq, mc, nb, bs, hq, hkv, d, dtype_code(q), ws.data_ptr(), ws.nbytes(),
+                            stream_of(q)),
+          what);
+}
+
+at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                          const at::Tensor& block_tables, const at::Tensor& cu_q, const at::Tensor& start_pos,
+                          const at::Tensor& tree_mask, int64_t max_q_len, int64_t max_ctx,
+                          const c10::optional<at::Tensor>& workspace) {
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  tree_attention_out(out, q, k_cache, v_cache, block_tables, cu_q, start_pos, tree_mask, max_q_len, max_ctx, workspace);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> accept_trees(
+    const at::Tensor& tokens, const at::Tensor& targets, const at::Tensor& tree_mask, const at::Tensor& cu_q,
+    const at::Tensor& start_pos, int64_t max_q_len, const c10::optional<at::Tensor>& k_cache,
+    const c10::optional<at::Tensor>& v_cache, const c10::optional<at::Tensor>& block_tables) {
+  constexpr const char* what = "accept_trees";
+  const at::Device dev = tokens.device();
+  metadata(targets, dev, what);
+  metadata(cu_q, dev, what);
+  metadata(start_pos, dev, what);
+  TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong && tokens.is_contiguous(), what,
+                   ": tokens must be contiguous int64");
+  const int64_t T = tokens.numel(), B = start_pos.numel();
+  TORCH_CHECK_VALUE(targets.numel() == T && cu_q.numel() == B + 1, what,
+                    ": one target per token and one start position per request are needed");
+  TORCH_CHECK_VALUE(B > 0, what, ": empty batch");
+  mask_words(tree_mask, T, max_q_len, dev, what);
+  int L = 0, nb = 0, bs = 0, hkv = 0, d = 0, width = 0, code = 0;
+  if (k_cache.has_value() || v_cache.has_value()) {
+    TORCH_CHECK_VALUE(k_cache.has_value() && v_cache.has_value() && block_tables.has_value(), what,
+                      ": the move needs both caches and block_tables");
+    const at::Tensor& k = *k_cache;
+    cache_like(k, *v_cache, dev, what);
+    metadata(*block_tables, dev, what);
+    TORCH_CHECK_VALUE(block_tables->dim() == 2 && block_tables->size(0) == B, what,
+                      ": block_tables needs one row per request");
+    TORCH_CHECK_VALUE(k.dim() == 4 || k.dim() == 5, what,
+                      ": caches are (L, NB, bs, Hkv, D) or one layer's (NB, bs, Hkv, D)");
+    L = k.dim() == 5 ? int_arg(k.size(0), what) : 1;
+    nb = int_arg(k.size(-4), what);
+    bs = int_arg(k.size(-3), what);
+    hkv = int_arg(k.size(-2), what);
+    d = int_arg(k.size(-1), what);
+    width = int_arg(block_tables->size(1), what);
+    code = dtype_code(k);
+  }
+  c10::cuda::CUDAGuard g(dev);
+  const auto i32 = start_pos.options();
+  at::Tensor num = at::empty({B}, i32), start = at::empty({B}, i32);
+  at::Tensor nodes = at::empty({B, max_q_len}, i32), out = at::empty({B, max_q_len}, i32);
+  check_v(ps_accept_trees(num.data_ptr<int32_t>(), nodes.data_ptr<int32_t>(), out.data_ptr<int32_t>(),
+                          start.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), targets.data_ptr<int32_t>(),
+                          tree_mask.data_ptr<int64_t>(), cu_q.data_ptr<int32_t>(), start_pos.data_ptr<int32_t>(),
+                          int_arg(B, what), int_arg(T, what), int_arg(max_q_len, what), ptr(k_cache), ptr(v_cache),
+                          k_cache.has_value() ? block_tables->data_ptr<int32_t>() : nullptr, width, L, nb, bs, hkv, d,
+                          code, stream_of(tokens)),
+          what);
+  return {num, nodes, out, start};
+}
+
 // ---------------------------------------------------------------- Meta ----
 // Output shapes only (torch.compile / fake-tensor tracing).
 
@@ -264,6 +462,31 @@ std::tuple<at::Tensor, at::Tensor> topk_meta(const at::Tensor& l, int64_t k) {
           at::empty({l.size(0), k}, l.options().dtype(at::kInt))};
 }
 
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_tables_meta(
+    const at::Tensor& seq_lens, const at::Tensor&, const at::Tensor& block_tables, const at::Tensor&,
+    const at::Tensor&, int64_t, int64_t, int64_t T, const c10::optional<at::Tensor>& parents,
+    c10::optional<int64_t> max_q_len) {
+  const auto i32 = seq_lens.options();
+  const int64_t B = seq_lens.numel();
+  auto mask = parents.has_value() ? at::empty({T, (max_q_len.value_or(0) + 63) / 64}, i32.dtype(at::kLong))
+                                  : at::empty({0}, i32.dtype(at::kLong));
+  return {at::empty(block_tables.sizes(), i32), at::empty({B}, i32), at::empty({B + 1}, i32), at::empty({T}, i32),
+          at::empty({T}, i32), mask, at::empty({1}, i32)};
+}
+at::Tensor tree_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t,
+                               const c10::optional<at::Tensor>&) {
+  return at::empty(q.sizes(), q.options());
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> accept_meta(
+    const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor& start_pos,
+    int64_t max_q_len, const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
+    const c10::optional<at::Tensor>&) {
+  const auto i32 = start_pos.options();
+  const int64_t B = start_pos.numel();
+  return {at::empty({B}, i32), at::empty({B, max_q_len}, i32), at::empty({B, max_q_len}, i32), at::empty({B}, i32)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(pageserve_b200, m) {
@@ -284,6 +507,19 @@ TORCH_LIBRARY(pageserve_b200, m) {
   m.def("argmax(Tensor logits) -> Tensor");
   m.def("topk(Tensor logits, int k) -> (Tensor, Tensor)");
   m.def("copy_kv_blocks(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor pairs) -> ()");
+  m.def("build_step_tables(Tensor seq_lens, Tensor q_lens, Tensor block_tables, Tensor held, Tensor free_blocks, "
+        "int num_blocks, int block_size, int total_tokens, Tensor? parents=None, int? max_q_len=None) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("build_step_tables_out(Tensor(a!) out, Tensor seq_lens, Tensor q_lens, Tensor block_tables, Tensor held, "
+        "Tensor free_blocks, int num_blocks, int block_size, int total_tokens, Tensor? parents=None, "
+        "int? max_q_len=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_q, Tensor start_pos, "
+        "Tensor tree_mask, int max_q_len, int max_ctx, Tensor? workspace=None) -> Tensor");
+  m.def("tree_attention_out(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+        "Tensor cu_q, Tensor start_pos, Tensor tree_mask, int max_q_len, int max_ctx, Tensor? workspace=None) -> ()");
+  m.def("accept_trees(Tensor tokens, Tensor targets, Tensor tree_mask, Tensor cu_q, Tensor start_pos, int max_q_len, "
+        "Tensor(a!)? k_cache=None, Tensor(b!)? v_cache=None, Tensor? block_tables=None) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(pageserve_b200, CUDA, m) {
@@ -301,6 +537,11 @@ TORCH_LIBRARY_IMPL(pageserve_b200, CUDA, m) {
   m.impl("argmax", &argmax);
   m.impl("topk", &topk);
   m.impl("copy_kv_blocks", &copy_kv_blocks);
+  m.impl("build_step_tables", &build_step_tables);
+  m.impl("build_step_tables_out", &build_step_tables_out);
+  m.impl("tree_attention", &tree_attention);
+  m.impl("tree_attention_out", &tree_attention_out);
+  m.impl("accept_trees", &accept_trees);
 }
 
 TORCH_LIBRARY_IMPL(pageserve_b200, Meta, m) {
@@ -314,4 +555,7 @@ TORCH_LIBRARY_IMPL(pageserve_b200, Meta, m) {
   m.impl("apply_rope", &apply_rope_meta);
   m.impl("argmax", &argmax_meta);
   m.impl("topk", &topk_meta);
+  m.impl("build_step_tables", &step_tables_meta);
+  m.impl("tree_attention", &tree_attention_meta);
+  m.impl("accept_trees", &accept_meta);
 }
