@@ -21,7 +21,7 @@
 #include <climits>
 #include <cstdlib>
 
-#include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace {
 
@@ -462,6 +462,532 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
   }
 }
 
+// ----------------------------------------------------------- tcgen05 kernel --
+// Block sizes of whole 16-key groups (the serving layouts). One CTA per SM, 128
+// query rows, 128-key tiles:
+//   warp 0     TMA producer: K and V tiles through one ring of equal slots in
+//              the order that the MMAs read them (K0 K1 V0 K2 V1 K3 ...), two
+//              boxes of 16 keys x 64 dims per 16-key group, one lane a box;
+//              16-key groups past the context or outside the pool are loads
+//              past the end of the tensor, which fill zeros
+//   warp 1     TMEM and the MMAs: S_w = Q K_j^T (both operands in shared
+//              memory), O_w += P_w V_j (P from TMEM, V read MN-major)
+//   warps 4-11 two softmax groups of 4 warps, one row per thread; group w takes
+//              the key tiles w, w + 2, ... with its own S, O, max and sum, so
+//              that one group's exponentials run under the other's MMAs; at the
+//              end of a row tile the two states are joined, each group storing
+//              half of the columns
+// A softmax thread reads its 128 scores twice from TMEM, 32 at a time (max, then
+// exponentials): holding them would need more than the 168 registers that 12
+// warps leave a thread.
+// TMEM: S0 | S1 | O0 | O1, 128 columns each; P_w overwrites S_w. MMAs of one
+// thread complete in order, so S_w(j) full also says that P_w(j - 2) V is done.
+// The ring and the barriers run on over the segments of a CTA's share: the next
+// segment's tiles load while the last one's output is stored.
+constexpr int kTcRows = 128;
+constexpr int kTcKeys = 128;
+constexpr int kTcThreads = 384;
+constexpr int kTcCtas = 148;
+
+template <int D>
+struct Tc {
+  static constexpr int kPanels = D / 64;                // 64-column panels of 128 rows x 128 bytes
+  static constexpr int kSlot = kTcKeys * D * 2;         // one K or V tile
+  static constexpr int kQ = kTcRows * D * 2;
+  static constexpr int kSlots = 192 * 1024 / kSlot;     // 6 (D = 128) or 12 (D = 64)
+  static constexpr int kSmem = kQ + kSlots * kSlot + 2560 /* barriers, (max, sum), flags */;
+};
+
+PS_DEVICE uint64_t desc_lbo(uint32_t addr, uint32_t lbo_bytes) {
+  return smem_desc_sw128(addr) | static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFF) << 16;
+}
+// B read MN-major ([k][n] rows of the V tile)
+__host__ __device__ constexpr uint32_t idesc_bmn(bool bf16, int m, int n) { return instr_desc(bf16, m, n) | (1u << 16); }
+
+PS_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// 32 columns of this warp's lanes, not waited for (tmem_ready orders the uses)
+PS_DEVICE void tmem_ld32_issue(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+PS_DEVICE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+PS_DEVICE void tmem_ready(float* v) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+PS_DEVICE float ex2_approx(float x) {  // relative error about 2^-22, 0 for -inf; far below P's rounding to 16 bits
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// After a wait gave up: let the copies or MMAs in flight end (bounded too).
+PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {
+  }
+}
+
+// Order of a segment's loads: K_j and V_j among its 2 * nt tiles.
+PS_DEVICE int k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
+PS_DEVICE int v_pos(int j, int nt) { return min(nt, j + 2) + j; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                const __grid_constant__ CUtensorMap vmap,
+                                                                const TreeParams p) {
+  pdl_wait();
+  pdl_trigger();
+  using C = Tc<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kNS = C::kSlots;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t q_sa = smem_u32(smem_raw);
+  unsigned char* gbase = smem_raw;
+  if (q_sa & 1023) {  // the swizzle needs the declared alignment
+    if (threadIdx.x == 0) record_error(p.status, kErrShape);
+    return;
+  }
+  const uint32_t ring = q_sa + C::kQ;
+  const uint32_t bars = ring + kNS * C::kSlot;
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (kNS + s); };
+  auto s_full = [&](int w) { return bars + 8 * (2 * kNS + w); };
+  auto p_full = [&](int w) { return bars + 8 * (2 * kNS + 2 + w); };
+  const uint32_t q_full = bars + 8 * (2 * kNS + 4);
+  const uint32_t o_full = bars + 8 * (2 * kNS + 5);
+  const uint32_t o_free = bars + 8 * (2 * kNS + 6);
+  const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
+  const uint32_t drained = bars + 8 * (2 * kNS + 8);
+  unsigned char* misc = gbase + C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
+  float2* s_ml = reinterpret_cast<float2*>(misc);                              // [2 groups][128 rows]
+  long long* s_share = reinterpret_cast<long long*>(misc + 2 * 128 * 8);       // begin, end, base, b
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 4);
+  volatile int* s_odd = abort_flag + 1;                                        // [2], by segment parity
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 4) + 3;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    long long begin, end, base;
+    int b;
+    find_share<kTcRows, kTcKeys>(p, lane, &begin, &end, &b, &base);
+    if (lane == 0) {
+      s_share[0] = begin;
+      s_share[1] = end;
+      s_share[2] = base;
+      s_share[3] = b;
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else if (threadIdx.x == 64) {
+    *abort_flag = 0;
+    s_odd[0] = s_odd[1] = 0;
+    for (int s = 0; s < kNS; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full(w), 1);
+      mbar_init(p_full(w), 4);
+    }
+    mbar_init(q_full, 8);
+    mbar_init(o_full, 1);
+    mbar_init(o_free, 8);
+    mbar_init(ml_full, 8);
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Segment<kTcRows, kTcKeys> sg;
+  sg.init(p, s_share[0], s_share[1], static_cast<int>(s_share[3]), s_share[2]);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer --
+    uint32_t seq = 0;
+    bool ok = true;
+    const int grp = lane & 7, panel = (lane >> 3) & 1;  // this lane's box of a tile
+    const bool mine = lane < 8 * C::kPanels;
+    while (ok && sg.next(p)) {
+      const int nt = sg.tile1 - sg.tile0;
+      const int ctx = sg.s.start + sg.s.n;
+      const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
+      const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
+      // row of this lane's 16-key group of tile j
+      auto row_of = [&](int j) {
+        const int key = (sg.tile0 + j) * kTcKeys + grp * 16;
+        if (!mine || j >= nt || key >= ctx) return past;
+        const int phys = table[key / p.block_size];
+        if (phys < 0 || phys >= p.num_blocks) {
+          record_error(p.status, kErrBlockId);
+          return past;
+        }
+        return phys * p.block_size + key % p.block_size;
+      };
+      auto load = [&](const CUtensorMap* map, int row) {
+        const int s = static_cast<int>(seq % kNS);
+        if (seq >= kNS && !warp_wait(empty(s), ((seq / kNS) - 1) & 1, abort_flag, p.status)) {
+          ok = false;
+          return;
+        }
+        if (lane == 0) mbar_expect_tx(full(s), C::kSlot);
+        __syncwarp();
+        if (mine) tma_load_3d(ring + s * C::kSlot + panel * (kTcKeys * 128) + grp * 2048, map, full(s), panel * 64, sg.h, row);
+        ++seq;
+      };
+      // rows of the tiles j, j + 1, j + 2 are looked up ahead of their loads
+      int r0 = row_of(0), r1 = row_of(1), r2 = row_of(2);
+      load(&kmap, r0);
+      if (ok && nt > 1) load(&kmap, r1);
+      for (int j = 0; ok && j < nt; ++j) {
+        const int r3 = row_of(j + 3);
+        load(&vmap, r0);
+        if (ok && j + 2 < nt) load(&kmap, r2);
+        r0 = r1;
+        r1 = r2;
+        r2 = r3;
+      }
+    }
+    if (!ok)
+      for (uint32_t i = seq > kNS ? seq - kNS : 0; i < seq; ++i) drain_wait(full(i % kNS), (i / kNS) & 1);
+  } else if (warp == 1) {
+    // --------------------------------------------------------------- MMA --
+    constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
+    constexpr uint32_t id_pv = idesc_bmn(kBf16, 128, D);
+    uint32_t seq = 0, seg = 0;
+    uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
+    bool ok = true;
+    while (ok && sg.next(p)) {
+      const int nt = sg.tile1 - sg.tile0;
+      auto qk = [&](int j) {
+        const uint32_t at = seq + k_pos(j);
+        const int s = static_cast<int>(at % kNS);
+        if (!warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
+            mma_f16(tmem + (j & 1) * 128, smem_desc_sw128(q_sa + off), smem_desc_sw128(ring + s * C::kSlot + off), id_qk,
+                    kk > 0 ? 1u : 0u);
+          }
+          mma_commit(empty(s));
+          mma_commit(s_full(j & 1));
+        }
+        __syncwarp();
+      };
+      ok = warp_wait(q_full, seg & 1, abort_flag, p.status);
+      if (!ok) break;
+      qk(0);
+      if (ok && nt > 1) qk(1);
+      if (ok && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+      for (int j = 0; ok && j < nt; ++j) {
+        const int w = j & 1;
+        const uint32_t at = seq + v_pos(j, nt);
+        const int s = static_cast<int>(at % kNS);
+        ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status) &&
+             warp_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
+        if (!ok) break;
+        ++tiles[w];
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int kk = 0; kk < kTcKeys / 16; ++kk)
+            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
+                   desc_lbo(ring + s * C::kSlot + kk * 16 * 128, kTcKeys * 128), id_pv, (j > 1 || kk > 0) ? 1u : 0u);
+          mma_commit(empty(s));
+          if (j == nt - 1) mma_commit(o_full);
+        }
+        __syncwarp();
+        if (j + 2 < nt) qk(j + 2);
+      }
+      seq += 2 * nt;
+      ++seg;
+    }
+    if (!ok) {
+      if (lane == 0) mma_commit(drained);
+      drain_wait(drained, 0);
+    }
+  } else if (warp >= 4) {
+    // ----------------------------------------------------------- softmax --
+    const int w = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // this thread's row of the tile (its TMEM lane)
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + w * 128 + lane_off;
+    constexpr int kQc = D / 16;  // 16-byte chunks of a row that this thread stages (half of the row)
+    uint4 qreg[kQc];
+    // this thread's half row of Q (rows past the request's are zeros)
+    auto load_q = [&](const Segment<kTcRows, kTcKeys>& g) {
+      const int row = g.row0 + r;
+      const bool on = row < g.s.n * p.G;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          static_cast<const T*>(p.q) +
+          (static_cast<long long>(g.s.q0 + (on ? row / p.G : 0)) * p.Hq + g.h * p.G + (on ? row % p.G : 0)) * D +
+          w * (D / 2));
+#pragma unroll
+      for (int c = 0; c < kQc; ++c) qreg[c] = on ? src[c] : make_uint4(0, 0, 0, 0);
+    };
+    auto store_q = [&] {
+#pragma unroll
+      for (int c = 0; c < kQc; ++c) {
+        const int chunk = w * kQc + c;  // of the row; 8 chunks a panel
+        *reinterpret_cast<uint4*>(gbase + (chunk >> 3) * (kTcRows * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) =
+            qreg[c];
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    uint32_t seq = 0, seg = 0, cnt = 0;
+    bool ok = true;
+    bool have = sg.next(p);
+    if (have) {
+      load_q(sg);
+      store_q();
+    }
+    while (ok && have) {
+      const int nt = sg.tile1 - sg.tile0;
+      const int n = sg.s.n, start = sg.s.start, ctx = start + n;
+      const int row = sg.row0 + r;
+      const bool row_on = row < n * p.G;
+      const bool warp_on = sg.row0 + quarter * 32 < n * p.G;
+      const int node = row_on ? row / p.G : 0;
+      const unsigned long long* mrow = p.mask + static_cast<long long>(sg.s.q0 + node) * p.words;
+      float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
+      for (int j = w; j < nt; j += 2) {
+        const int key0 = (sg.tile0 + j) * kTcKeys;
+        const bool tail = key0 + kTcKeys > start;
+        if (tail) {
+          // V rows past the context hold anything, and a drafted row's values
+          // that are not finite would reach rows that do not see it: clear them
+          const uint32_t at = seq + v_pos(j, nt);
+          const int s = static_cast<int>(at % kNS);
+          ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status);
+          if (!ok) break;
+          const int key = key0 + r;
+          if (key >= start) {
+            bool bad = false;
+#pragma unroll
+            for (int pn = 0; pn < C::kPanels; ++pn) {
+              uint4* line = reinterpret_cast<uint4*>(gbase + C::kQ + s * C::kSlot + pn * (kTcKeys * 128) + r * 128);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                uint4 x = key < ctx ? line[c] : make_uint4(0, 0, 0, 0);
+                uint16_t* h = reinterpret_cast<uint16_t*>(&x);
+                bool hit = key >= ctx;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (!finite16<T>(h[e])) {
+                    h[e] = 0;
+                    hit = bad = true;
+                  }
+                if (hit) line[c] = x;
+              }
+            }
+            if (bad) s_odd[seg & 1] = 1;
+          }
+          fence_proxy_async();
+        }
+        ok = warp_wait(s_full(w), cnt & 1, abort_flag, p.status);
+        if (!ok) break;
+        ++cnt;
+        tc_fence_after();
+        if (warp_on) {
+          // bits of the keys that this row sees (a row tile's unused rows: none)
+          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+          if (tail) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const unsigned long long v = row_on ? seen64(mrow, p.words, key0 + 64 * hf - start, n) : 0ull;
+              vis[2 * hf] = static_cast<uint32_t>(v);
+              vis[2 * hf + 1] = static_cast<uint32_t>(v >> 32);
+            }
+          }
+          float sv[2][32];
+          float mx = -INFINITY;
+          tmem_ld32_issue(t_s, sv[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld();
+            tmem_ready(sv[c & 1]);
+            if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv[(c + 1) & 1]);
+            if (tail) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((vis[c] >> i) & 1) mx = fmaxf(mx, sv[c & 1][i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mx = fmaxf(mx, sv[c & 1][i]);
+            }
+          }
+          mx *= p.scale_log2;
+          // O is rescaled only when a row's max has grown by more than 2^8:
+          // P <= 2^8 stays well inside the 16-bit types, and sum and O share m_ref
+          float alpha = 1.f;
+          const bool moved = mx > m_ref + 8.f;
+          if (moved) {
+            alpha = m_ref == -FLT_MAX ? 0.f : ex2_approx(m_ref - mx);
+            m_ref = mx;
+          }
+          if (j >= 2 && __any_sync(0xffffffffu, moved)) {
+            const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float v[32];
+              tmem_ld32(t_o + c * 32, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= alpha;
+              tmem_st16(t_o + c * 32, reinterpret_cast<const uint32_t*>(v));
+              tmem_st16(t_o + c * 32 + 16, reinterpret_cast<const uint32_t*>(v) + 16);
+            }
+          }
+          float sum = 0.f;
+          tmem_ld32_issue(t_s, sv[0]);
+          // P's 16-bit columns c * 16 .. lie below the scores still to be read
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld();
+            tmem_ready(sv[c & 1]);
+            if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv[(c + 1) & 1]);
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0 = fmaf(sv[c & 1][i], p.scale_log2, -m_ref), x1 = fmaf(sv[c & 1][i + 1], p.scale_log2, -m_ref);
+              if (tail) {
+                if (!((vis[c] >> i) & 1)) x0 = -INFINITY;
+                if (!((vis[c] >> (i + 1)) & 1)) x1 = -INFINITY;
+              }
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              sum += p0 + p1;
+              // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12
+              // (f16) of a term, as the output's own rounding
+              pk[i / 2] = pack2<T>(p0, p1);
+            }
+            tmem_st16(t_s + c * 16, pk);
+          }
+          tmem_wait_st();
+          l = l * alpha + sum;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(w));
+      }
+      if (!ok) break;
+      Segment<kTcRows, kTcKeys> nx = sg;
+      const bool more = nx.next(p);
+      if (more) load_q(nx);
+      ok = warp_wait(o_full, seg & 1, abort_flag, p.status);
+      if (!ok) break;
+      tc_fence_after();
+      if (threadIdx.x == 128) s_odd[(seg + 1) & 1] = 0;
+      s_ml[w * 128 + r] = make_float2(m_ref, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ml_full);
+      ok = warp_wait(ml_full, seg & 1, abort_flag, p.status);
+      if (!ok) break;
+      if (more) store_q();  // every MMA of this segment is done: Q may change
+      // join the two groups; group w stores the columns [w D/2, (w + 1) D/2)
+      if (warp_on) {
+        const float2 ml0 = s_ml[r], ml1 = s_ml[128 + r];
+        const bool two = nt > 1;
+        const float m = two ? fmaxf(ml0.x, ml1.x) : ml0.x;
+        float a0 = ex2_approx(ml0.x - m), a1 = two ? ex2_approx(ml1.x - m) : 0.f;
+        const float lt = two ? ml0.y * a0 + ml1.y * a1 : ml0.y;
+        const bool whole = sg.whole();
+        if (whole) {
+          const float inv = lt == 0.f ? 0.f : 1.f / lt;
+          a0 *= inv;
+          a1 *= inv;
+        }
+        const bool odd = s_odd[seg & 1] != 0;
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kTcRows + r;
+        T* dst = static_cast<T*>(p.out) +
+                 (static_cast<long long>(sg.s.q0 + node) * p.Hq + sg.h * p.G + row % p.G) * D + w * (D / 2);
+        float* pdst = p.part + pr * D + w * (D / 2);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          float o0[32], o1[32];
+          const uint32_t t_o = tmem + 256 + lane_off + w * (D / 2) + c * 32;
+          tmem_ld32_issue(t_o, o0);
+          if (two) tmem_ld32_issue(t_o + 128, o1);
+          tmem_wait_ld();
+          tmem_ready(o0);
+          if (two) tmem_ready(o1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            o0[i] *= a0;
+            if (two) o0[i] = fmaf(o1[i], a1, o0[i]);
+          }
+          if (odd && row_on) {
+            // the cleared values, to the rows that see them
+            const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
+            const int k1 = min(sg.tile1 * kTcKeys, ctx);
+            for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
+              const int jn = key - start;
+              if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
+              const int phys = table[key / p.block_size];
+              if (phys < 0 || phys >= p.num_blocks) continue;
+              const T* vr = static_cast<const T*>(p.v_cache) +
+                            ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
+                            w * (D / 2) + c * 32;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const T x = vr[i];
+                if (!finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) o0[i] += to_f32(x);
+              }
+            }
+          }
+          if (row_on) {
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o0 + i);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(pdst + c * 32 + i) = make_float4(o0[i], o0[i + 1], o0[i + 2], o0[i + 3]);
+            }
+          }
+        }
+        if (!whole && row_on && w == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m, lt);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      seq += 2 * nt;
+      ++seg;
+      sg = nx;
+      have = more;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
 // -------------------------------------------------------------- the joining --
 // One CTA column per boundary between two shares; the first boundary inside a
 // row tile joins all its parts, one warp per row.
@@ -522,19 +1048,26 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams p) {
 
 // ------------------------------------------------------------------- host --
 struct Plan {
+  bool tc;
   int rows, keys, ctas, min_share;
   size_t bytes;
 };
 
-Plan plan_for(int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv, int D) {
+// The tcgen05 kernel takes whole 16-key groups at 32-bit rows.
+bool tc_layout(int num_blocks, int block_size) {
+  return block_size % 16 == 0 && (static_cast<long long>(num_blocks) + 1) * block_size < INT32_MAX;
+}
+
+Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv, int D) {
   Plan pl{};
-  pl.rows = kRows;
-  pl.keys = kKeys;
+  pl.tc = tc;
+  pl.rows = tc ? kTcRows : kRows;
+  pl.keys = tc ? kTcKeys : kKeys;
   pl.min_share = 4;
   const long long rt = (static_cast<long long>(max_q_len) * (Hq / Hkv) + pl.rows - 1) / pl.rows;
   const long long kt = (static_cast<long long>(max_ctx) + pl.keys - 1) / pl.keys;
   const double items = static_cast<double>(num_seqs) * Hkv * rt * kt;
-  long long ctas = 148 * 2;
+  long long ctas = tc ? kTcCtas : 2 * kTcCtas;
   const double most = (items + pl.min_share - 1) / pl.min_share;
   if (most < ctas) ctas = static_cast<long long>(most);
   if (ctas < 1) ctas = 1;
@@ -563,6 +1096,47 @@ int launch_mma(TreeParams& p, cudaStream_t s) {
   return ps_host::check_launch("tree_attention(join)");
 }
 
+// One layer's cache as [num_blocks * block_size keys][Hkv][D], boxes of 16 keys
+// x 64 dims of one head, 128-byte swizzle.
+bool make_cache_map(CUtensorMap* map, const void* cache, bool bf16, int num_blocks, int block_size, int Hkv, int D) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(Hkv),
+                        static_cast<cuuint64_t>(num_blocks) * block_size};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(Hkv) * D * 2};
+  cuuint32_t box[3] = {64, 1, 16};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int launch_tc(TreeParams& p, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (!make_cache_map(&km, p.k_cache, bf16, p.num_blocks, p.block_size, p.Hkv, D) ||
+      !make_cache_map(&vm, p.v_cache, bf16, p.num_blocks, p.block_size, p.Hkv, D)) {
+    ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed for the KV cache");
+    return PS_ERR_CUDA;
+  }
+  auto kern = tree_tc_kernel<T, D>;
+  static std::atomic<uint64_t> done{0};
+  if (!ps_host::reserve_smem(reinterpret_cast<const void*>(kern), Tc<D>::kSmem, &done)) {
+    ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
+    return PS_ERR_CUDA;
+  }
+  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, km, vm, p);
+  ps_host::count_launch();
+  int rc = ps_host::check_launch("tree_attention");
+  if (rc != PS_OK || p.num_ctas == 1) return rc;
+  auto join = tree_join_kernel<T, D, kTcRows, kTcKeys>;
+  ps_host::launch(join, dim3(p.num_ctas - 1, kTcRows / 4), 128, 0, s, p);
+  ps_host::count_launch();
+  return ps_host::check_launch("tree_attention(join)");
+}
+
 }  // namespace
 
 extern "C" {
@@ -571,7 +1145,9 @@ size_t ps_tree_attention_workspace_size(int num_seqs, int max_q_len, int max_ctx
   if (num_seqs <= 0 || max_q_len <= 0 || max_q_len > kMaxNodes || max_ctx < max_q_len || Hq <= 0 || Hkv <= 0 ||
       Hq % Hkv != 0 || (D != 64 && D != 128))
     return 0;
-  return plan_for(num_seqs, max_q_len, max_ctx, Hq, Hkv, D).bytes;
+  const size_t a = plan_for(true, num_seqs, max_q_len, max_ctx, Hq, Hkv, D).bytes;
+  const size_t b = plan_for(false, num_seqs, max_q_len, max_ctx, Hq, Hkv, D).bytes;
+  return a > b ? a : b;
 }
 
 int ps_tree_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const int32_t* tables,
@@ -618,7 +1194,7 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
     ps_host::set_error("tree_attention: dtype must be bf16 or f16");
     return PS_ERR_UNSUPPORTED;
   }
-  const Plan pl = plan_for(num_seqs, max_q_len, max_ctx, Hq, Hkv, D);
+  const Plan pl = plan_for(tc_layout(num_blocks, block_size), num_seqs, max_q_len, max_ctx, Hq, Hkv, D);
   if (!workspace || workspace_bytes < pl.bytes) {
     ps_host::set_error("tree_attention: workspace of %zu bytes needed, %zu given", pl.bytes, workspace_bytes);
     return PS_ERR_INVALID;
@@ -654,6 +1230,11 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.min_share = pl.min_share;
   p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (pl.tc) {
+    if (dtype == PS_BF16)
+      return D == 128 ? launch_tc<__nv_bfloat16, 128>(p, s) : launch_tc<__nv_bfloat16, 64>(p, s);
+    return D == 128 ? launch_tc<__half, 128>(p, s) : launch_tc<__half, 64>(p, s);
+  }
   if (dtype == PS_BF16)
     return D == 128 ? launch_mma<__nv_bfloat16, 128>(p, s) : launch_mma<__nv_bfloat16, 64>(p, s);
   return D == 128 ? launch_mma<__half, 128>(p, s) : launch_mma<__half, 64>(p, s);
