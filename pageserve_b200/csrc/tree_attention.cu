@@ -29,6 +29,12 @@ using namespace ps;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxNodes = 256;
+constexpr int kMaxRows = 128;  // query rows per tile
+
+struct Part {  // the split row tile whose later part (slot 0) a CTA holds; c0 < 0: none
+  int q0, h, row0, rows, c0, c1;  // rows to store; CTAs c0 (slot 1) .. c1 (slot 0) hold its parts
+  int pad[2];
+};
 
 struct TreeParams {
   void* out;
@@ -39,10 +45,9 @@ struct TreeParams {
   const int32_t* cu_q;
   const int32_t* start_pos;
   const unsigned long long* mask;
-  float* part;          // [CTA][2][rows][D] of o, then [CTA][2][rows][2] of (max, sum)
-  float* part_ml;
-  long long* seq_base;  // [num_seqs + 1] first work item of each sequence
-  long long* share;     // work items per CTA
+  float* part;     // [CTA][2 slots][kMaxRows][D] of o
+  float* part_ml;  // [CTA][2 slots][kMaxRows][2] of (max, sum)
+  Part* parts;     // [CTA]
   int* status;
   int total_q;
   int words;
@@ -54,125 +59,141 @@ struct TreeParams {
   int max_ctx;
   int num_seqs;
   int num_ctas;
-  int min_share;        // fewest key tiles worth a CTA
+  int min_share;   // fewest key tiles worth a CTA
+  int tile_rows;   // query rows per tile
   float scale_log2;
 };
 
 // ------------------------------------------------------- division of work --
+// The work items of sequence b are (kv head, row tile, key tile), key tile
+// fastest; the host has checked that a call's items fit 31 bits.
 struct Seq {
   int q0, n, start, row_tiles, key_tiles;
+  PS_DEVICE int items(int Hkv) const { return Hkv * row_tiles * key_tiles; }
 };
 
-template <int ROWS, int KEYS>
+template <int KEYS>
 PS_DEVICE Seq seq_of(const TreeParams& p, int b, bool record) {
   Seq s;
   s.q0 = p.cu_q[b];
   s.n = p.cu_q[b + 1] - s.q0;
   s.start = p.start_pos[b];
   s.row_tiles = s.key_tiles = 0;
-  const long long ctx = static_cast<long long>(s.start) + s.n;
   if (s.n == 0) return s;
-  if (s.n < 0 || s.n > p.max_q_len || s.q0 < 0 || s.q0 + s.n > p.total_q || s.start < 0 || ctx > p.max_ctx ||
-      ctx > static_cast<long long>(p.max_blocks) * p.block_size) {
+  const long long ctx = static_cast<long long>(s.start) + s.n;
+  if (s.n < 0 || s.n > p.max_q_len || s.q0 < 0 || s.q0 + s.n > p.total_q || s.start < 0 || ctx > p.max_ctx) {
     if (record) record_error(p.status, kErrShape);
     s.n = 0;
     return s;
   }
-  s.row_tiles = (s.n * p.G + ROWS - 1) / ROWS;
+  s.row_tiles = (s.n * p.G + p.tile_rows - 1) / p.tile_rows;
   s.key_tiles = (static_cast<int>(ctx) + KEYS - 1) / KEYS;
   return s;
 }
 
-template <int ROWS, int KEYS>
-PS_DEVICE long long items_of(const TreeParams& p, int b, bool record) {
-  const Seq s = seq_of<ROWS, KEYS>(p, b, record);
-  return static_cast<long long>(p.Hkv) * s.row_tiles * s.key_tiles;
-}
+// A CTA's share of the work: items [begin, end), the sequence that holds begin
+// and that sequence's first item.
+struct Share {
+  int begin, end, per, b, base;
+  Seq s;
+};
 
-// By one whole warp: this CTA's share [*begin, *end) of the work, the sequence
-// that holds *begin and that sequence's first item. CTA 0 also writes the
-// sequences' first items for the joining kernel.
-template <int ROWS, int KEYS>
-PS_DEVICE void find_share(const TreeParams& p, int lane, long long* begin, long long* end, int* b_out,
-                          long long* base_out) {
+// By one whole warp. The sequences' lengths are kept in registers between the
+// sum and the search (up to 256 of them): one round of global latency.
+template <int KEYS>
+PS_DEVICE Share find_share(const TreeParams& p, int lane) {
+  constexpr int kKeep = 8;
   const bool lead = blockIdx.x == 0;
-  long long total = 0;
-  for (int b = lane; b < p.num_seqs; b += 32) total += items_of<ROWS, KEYS>(p, b, lead);
+  int items[kKeep];
+  int total = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  long long per = (total + p.num_ctas - 1) / p.num_ctas;
-  if (per < p.min_share) per = p.min_share;
-  const long long lo = per * blockIdx.x;
-  *begin = lo < total ? lo : total;
-  *end = lo + per < total ? lo + per : total;
-  *b_out = p.num_seqs;
-  *base_out = total;
-  if (lead && lane == 0) {
-    *p.share = per;
-    p.seq_base[p.num_seqs] = total;
+  for (int i = 0; i < kKeep; ++i) {
+    const int b = i * 32 + lane;
+    items[i] = b < p.num_seqs ? seq_of<KEYS>(p, b, lead).items(p.Hkv) : 0;
+    total += items[i];
   }
-  if (*begin >= *end && !lead) return;
-  long long run = 0;
-  bool found = false;
-  for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
-    const int b = b0 + lane;
-    const long long n = b < p.num_seqs ? items_of<ROWS, KEYS>(p, b, false) : 0;
-    long long incl = n;
+  for (int b = kKeep * 32 + lane; b < p.num_seqs; b += 32) total += seq_of<KEYS>(p, b, lead).items(p.Hkv);
+  total = __reduce_add_sync(0xffffffffu, total);
+  Share r;
+  r.per = max((total + p.num_ctas - 1) / p.num_ctas, p.min_share);
+  const long long lo = static_cast<long long>(r.per) * blockIdx.x;
+  r.begin = static_cast<int>(lo < total ? lo : total);
+  r.end = min(r.begin + r.per, total);
+  r.b = p.num_seqs;
+  r.base = total;
+  r.s = Seq{};
+  if (r.begin >= r.end) return r;
+  int run = 0;
+  for (int i = 0; i * 32 < p.num_seqs; ++i) {
+    const int b = i * 32 + lane;
+    int n = 0;
+    if (i < kKeep) {
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k)
+        if (k == i) n = items[k];
+    } else if (b < p.num_seqs) {
+      n = seq_of<KEYS>(p, b, false).items(p.Hkv);
+    }
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const long long first = run + incl - n;
-    if (lead && b < p.num_seqs) p.seq_base[b] = first;
-    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && *begin >= first && *begin < first + n);
-    if (hit && !found) {
+    const int first = run + incl - n;
+    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && r.begin >= first && r.begin < first + n);
+    if (hit) {
       const int src = __ffs(hit) - 1;
-      *b_out = b0 + src;
-      *base_out = __shfl_sync(0xffffffffu, first, src);
-      found = true;
-      if (!lead) return;
+      r.b = i * 32 + src;
+      r.base = __shfl_sync(0xffffffffu, first, src);
+      break;
     }
     run += __shfl_sync(0xffffffffu, incl, 31);
   }
+  r.s = seq_of<KEYS>(p, r.b, false);
+  return r;
 }
 
 // Walk over the segments (one row tile's key tiles) of a share.
-template <int ROWS, int KEYS>
+template <int KEYS>
 struct Segment {
-  long long cur, end, base;  // next item, share's end, first item of sequence b
-  int b;
+  int cur, end, base, b;  // next item, share's end, first item of sequence b
   Seq s;
   int h, row0, tile0, tile1;
 
-  PS_DEVICE void init(const TreeParams& p, long long begin, long long end_, int b_, long long base_) {
-    cur = begin;
-    end = end_;
-    b = b_;
-    base = base_;
-    if (cur < end) s = seq_of<ROWS, KEYS>(p, b, false);
+  PS_DEVICE void init(const Share& sh) {
+    cur = sh.begin;
+    end = sh.end;
+    b = sh.b;
+    base = sh.base;
+    s = sh.s;
   }
   PS_DEVICE bool next(const TreeParams& p) {
     if (cur >= end) return false;
-    long long items = static_cast<long long>(p.Hkv) * s.row_tiles * s.key_tiles;
+    int items = s.items(p.Hkv);
     while (cur >= base + items) {
       base += items;
-      s = seq_of<ROWS, KEYS>(p, ++b, false);
-      items = static_cast<long long>(p.Hkv) * s.row_tiles * s.key_tiles;
+      s = seq_of<KEYS>(p, ++b, false);
+      items = s.items(p.Hkv);
     }
-    const long long at = cur - base;
-    const long long pair = at / s.key_tiles;
+    const uint32_t at = cur - base;
+    const uint32_t pair = at / static_cast<uint32_t>(s.key_tiles);
     tile0 = static_cast<int>(at - pair * s.key_tiles);
-    h = static_cast<int>(pair / s.row_tiles);
-    row0 = static_cast<int>(pair - static_cast<long long>(h) * s.row_tiles) * ROWS;
-    const long long left = end - cur;
-    tile1 = left < s.key_tiles - tile0 ? tile0 + static_cast<int>(left) : s.key_tiles;
+    h = static_cast<int>(pair / static_cast<uint32_t>(s.row_tiles));
+    row0 = (static_cast<int>(pair) - h * s.row_tiles) * p.tile_rows;
+    tile1 = min(tile0 + end - cur, s.key_tiles);
     cur += tile1 - tile0;
     return true;
   }
   PS_DEVICE bool whole() const { return tile0 == 0 && tile1 == s.key_tiles; }
   // a row tile's first part is the last segment of its CTA, the others the first
   PS_DEVICE int slot() const { return tile0 > 0 ? 0 : 1; }
+  PS_DEVICE int rows(const TreeParams& p) const { return min(p.tile_rows, s.n * p.G - row0); }
+  // for a segment of slot 0
+  PS_DEVICE Part part(const TreeParams& p, int per) const {
+    const int first = cur - tile1;  // the row tile's first item
+    return Part{s.q0, h, row0, rows(p), first / per, (first + s.key_tiles - 1) / per, {0, 0}};
+  }
 };
 
 // Bits of the 64 keys from tree index `off` on (keys before the tree are seen
@@ -242,23 +263,18 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
   pdl_trigger();
   constexpr int kTile = kKeys * D * 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_share[3];
-  __shared__ int s_b;
+  __shared__ Share s_share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    long long begin, end, base;
-    int b;
-    find_share<kRows, kKeys>(p, lane, &begin, &end, &b, &base);
+    const Share sh = find_share<kKeys>(p, lane);
     if (lane == 0) {
-      s_share[0] = begin;
-      s_share[1] = end;
-      s_share[2] = base;
-      s_b = b;
+      s_share = sh;
+      p.parts[blockIdx.x].c0 = -1;
     }
   }
   __syncthreads();
-  Segment<kRows, kKeys> sg;
-  sg.init(p, s_share[0], s_share[1], s_b, s_share[2]);
+  Segment<kKeys> sg;
+  sg.init(s_share);
   const uint32_t base = smem_u32(smem);
   const int mat = lane >> 3;
   while (sg.next(p)) {
@@ -438,7 +454,8 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
       }
     }
     const bool whole = sg.whole();
-    const long long pslot = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kRows;
+    const long long pslot = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kMaxRows;
+    if (sg.tile0 > 0 && threadIdx.x == 0) p.parts[blockIdx.x] = sg.part(p, s_share.per);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int r = wrow + (lane >> 2) + hf * 8;
@@ -465,11 +482,14 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // ----------------------------------------------------------- tcgen05 kernel --
 // Block sizes of whole 16-key groups (the serving layouts). One CTA per SM, 128
 // query rows, 128-key tiles:
-//   warp 0     TMA producer: K and V tiles through one ring of equal slots in
-//              the order that the MMAs read them (K0 K1 V0 K2 V1 K3 ...), two
-//              boxes of 16 keys x 64 dims per 16-key group, one lane a box;
-//              16-key groups past the context or outside the pool are loads
-//              past the end of the tensor, which fill zeros
+//   warps 0, 3 TMA producers of K and of V: tiles go through one ring of equal
+//              slots in the order that the MMAs read them (K0 K1 V0 K2 V1 ...),
+//              as boxes of 16 keys x 64 dims, one lane a box; 16-key groups past
+//              the context or outside the pool are loads past the end of the
+//              tensor, which fill zeros. Boxes are issued at a bounded rate per
+//              warp: one warp for both tensors reached 4.7 TB/s, two 5.3
+//   warp 2     TMA producer of the Q tiles: 128 / G nodes x the G heads of the
+//              group (tile_rows = G * (128 / G) rows), again one box per 64 dims
 //   warp 1     TMEM and the MMAs: S_w = Q K_j^T (both operands in shared
 //              memory), O_w += P_w V_j (P from TMEM, V read MN-major)
 //   warps 4-11 two softmax groups of 4 warps, one row per thread; group w takes
@@ -488,6 +508,7 @@ constexpr int kTcRows = 128;
 constexpr int kTcKeys = 128;
 constexpr int kTcThreads = 384;
 constexpr int kTcCtas = 148;
+constexpr int kMinShare = 4;
 
 template <int D>
 struct Tc {
@@ -546,7 +567,8 @@ PS_DEVICE int k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
 PS_DEVICE int v_pos(int j, int nt) { return min(nt, j + 2) + j; }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap qmap,
+                                                                const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
                                                                 const TreeParams p) {
   pdl_wait();
@@ -568,28 +590,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   auto s_full = [&](int w) { return bars + 8 * (2 * kNS + w); };
   auto p_full = [&](int w) { return bars + 8 * (2 * kNS + 2 + w); };
   const uint32_t q_full = bars + 8 * (2 * kNS + 4);
-  const uint32_t o_full = bars + 8 * (2 * kNS + 5);
-  const uint32_t o_free = bars + 8 * (2 * kNS + 6);
-  const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
-  const uint32_t drained = bars + 8 * (2 * kNS + 8);
+  const uint32_t q_empty = bars + 8 * (2 * kNS + 5);
+  const uint32_t o_full = bars + 8 * (2 * kNS + 6);
+  const uint32_t o_free = bars + 8 * (2 * kNS + 7);
+  const uint32_t ml_full = bars + 8 * (2 * kNS + 8);
+  const uint32_t drained = bars + 8 * (2 * kNS + 9);
   unsigned char* misc = gbase + C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
-  float2* s_ml = reinterpret_cast<float2*>(misc);                              // [2 groups][128 rows]
-  long long* s_share = reinterpret_cast<long long*>(misc + 2 * 128 * 8);       // begin, end, base, b
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 4);
-  volatile int* s_odd = abort_flag + 1;                                        // [2], by segment parity
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 4) + 3;
+  float2* s_ml = reinterpret_cast<float2*>(misc);  // [2 groups][128 rows]
+  Share* s_share = reinterpret_cast<Share*>(misc + 2 * 128 * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 1);
+  volatile int* s_odd = abort_flag + 1;  // [2], by segment parity
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 1) + 3;
+  volatile uint32_t* s_at = tmem_slot + 1;  // [kNS] the tile last loaded into each slot
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    long long begin, end, base;
-    int b;
-    find_share<kTcRows, kTcKeys>(p, lane, &begin, &end, &b, &base);
-    if (lane == 0) {
-      s_share[0] = begin;
-      s_share[1] = end;
-      s_share[2] = base;
-      s_share[3] = b;
-    }
+    const Share sh = find_share<kTcKeys>(p, lane);
+    if (lane == 0) *s_share = sh;
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512));
@@ -600,36 +617,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     for (int s = 0; s < kNS; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
+      s_at[s] = ~0u;
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full(w), 1);
       mbar_init(p_full(w), 4);
     }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, 8);
     mbar_init(ml_full, 8);
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  } else if (threadIdx.x == 96) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Segment<kTcRows, kTcKeys> sg;
-  sg.init(p, s_share[0], s_share[1], static_cast<int>(s_share[3]), s_share[2]);
+  Segment<kTcKeys> sg;
+  sg.init(*s_share);
 
-  if (warp == 0) {
-    // ---------------------------------------------------------- producer --
+  if (warp == 0 || warp == 3) {
+    // ---------------------------------------------------- K, V producers --
+    const bool is_v = warp == 3;
+    const CUtensorMap* map = is_v ? &vmap : &kmap;
     uint32_t seq = 0;
     bool ok = true;
     const int grp = lane & 7, panel = (lane >> 3) & 1;  // this lane's box of a tile
     const bool mine = lane < 8 * C::kPanels;
+    const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
     while (ok && sg.next(p)) {
       const int nt = sg.tile1 - sg.tile0;
       const int ctx = sg.s.start + sg.s.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-      const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
       // row of this lane's 16-key group of tile j
       auto row_of = [&](int j) {
         const int key = (sg.tile0 + j) * kTcKeys + grp * 16;
@@ -641,32 +666,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         }
         return phys * p.block_size + key % p.block_size;
       };
-      auto load = [&](const CUtensorMap* map, int row) {
-        const int s = static_cast<int>(seq % kNS);
-        if (seq >= kNS && !warp_wait(empty(s), ((seq / kNS) - 1) & 1, abort_flag, p.status)) {
+      // rows are looked up two tiles ahead of their loads
+      int r0 = row_of(0), r1 = row_of(1);
+      for (int j = 0; j < nt; ++j) {
+        const int r2 = row_of(j + 2);
+        const uint32_t at = seq + (is_v ? v_pos(j, nt) : k_pos(j));
+        const int s = static_cast<int>(at % kNS);
+        if (at >= kNS && !warp_wait(empty(s), ((at / kNS) - 1) & 1, abort_flag, p.status)) {
           ok = false;
-          return;
+          break;
         }
-        if (lane == 0) mbar_expect_tx(full(s), C::kSlot);
+        if (lane == 0) {
+          mbar_expect_tx(full(s), C::kSlot);
+          s_at[s] = at;
+        }
         __syncwarp();
-        if (mine) tma_load_3d(ring + s * C::kSlot + panel * (kTcKeys * 128) + grp * 2048, map, full(s), panel * 64, sg.h, row);
-        ++seq;
-      };
-      // rows of the tiles j, j + 1, j + 2 are looked up ahead of their loads
-      int r0 = row_of(0), r1 = row_of(1), r2 = row_of(2);
-      load(&kmap, r0);
-      if (ok && nt > 1) load(&kmap, r1);
-      for (int j = 0; ok && j < nt; ++j) {
-        const int r3 = row_of(j + 3);
-        load(&vmap, r0);
-        if (ok && j + 2 < nt) load(&kmap, r2);
+        if (mine)
+          tma_load_3d(ring + s * C::kSlot + panel * (kTcKeys * 128) + grp * 2048, map, full(s), panel * 64, sg.h, r0);
         r0 = r1;
         r1 = r2;
-        r2 = r3;
       }
+      seq += 2 * nt;
     }
     if (!ok)
-      for (uint32_t i = seq > kNS ? seq - kNS : 0; i < seq; ++i) drain_wait(full(i % kNS), (i / kNS) & 1);
+      for (int s = 0; s < kNS; ++s)
+        if (s_at[s] != ~0u) drain_wait(full(s), (s_at[s] / kNS) & 1);
+  } else if (warp == 2) {
+    // -------------------------------------------------------- Q producer --
+    uint32_t seg = 0;
+    bool ok = true;
+    while (ok && sg.next(p)) {
+      if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1, abort_flag, p.status)) {
+        ok = false;
+        break;
+      }
+      if (lane == 0) {
+        mbar_expect_tx(q_full, C::kPanels * p.tile_rows * 128);
+        for (int pn = 0; pn < C::kPanels; ++pn)
+          tma_load_3d(q_sa + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G, sg.s.q0 + sg.row0 / p.G);
+      }
+      __syncwarp();
+      ++seg;
+    }
+    if (!ok && seg) drain_wait(q_full, (seg - 1) & 1);
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA --
     constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
@@ -674,8 +716,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     uint32_t seq = 0, seg = 0;
     uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
     bool ok = true;
-    while (ok && sg.next(p)) {
+    bool have = sg.next(p);
+    while (ok && have) {
       const int nt = sg.tile1 - sg.tile0;
+      have = sg.next(p);  // the next segment's lengths arrive under this one's MMAs
       auto qk = [&](int j) {
         const uint32_t at = seq + k_pos(j);
         const int s = static_cast<int>(at % kNS);
@@ -693,6 +737,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           }
           mma_commit(empty(s));
           mma_commit(s_full(j & 1));
+          if (j == nt - 1) mma_commit(q_empty);
         }
         __syncwarp();
       };
@@ -735,43 +780,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const int r = quarter * 32 + lane;  // this thread's row of the tile (its TMEM lane)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + w * 128 + lane_off;
-    constexpr int kQc = D / 16;  // 16-byte chunks of a row that this thread stages (half of the row)
-    uint4 qreg[kQc];
-    // this thread's half row of Q (rows past the request's are zeros)
-    auto load_q = [&](const Segment<kTcRows, kTcKeys>& g) {
-      const int row = g.row0 + r;
-      const bool on = row < g.s.n * p.G;
-      const uint4* src = reinterpret_cast<const uint4*>(
-          static_cast<const T*>(p.q) +
-          (static_cast<long long>(g.s.q0 + (on ? row / p.G : 0)) * p.Hq + g.h * p.G + (on ? row % p.G : 0)) * D +
-          w * (D / 2));
-#pragma unroll
-      for (int c = 0; c < kQc; ++c) qreg[c] = on ? src[c] : make_uint4(0, 0, 0, 0);
-    };
-    auto store_q = [&] {
-#pragma unroll
-      for (int c = 0; c < kQc; ++c) {
-        const int chunk = w * kQc + c;  // of the row; 8 chunks a panel
-        *reinterpret_cast<uint4*>(gbase + (chunk >> 3) * (kTcRows * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) =
-            qreg[c];
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    };
     uint32_t seq = 0, seg = 0, cnt = 0;
     bool ok = true;
     bool have = sg.next(p);
-    if (have) {
-      load_q(sg);
-      store_q();
-    }
+    if (threadIdx.x == 128 && !(have && sg.tile0 > 0)) p.parts[blockIdx.x].c0 = -1;
     while (ok && have) {
       const int nt = sg.tile1 - sg.tile0;
       const int n = sg.s.n, start = sg.s.start, ctx = start + n;
       const int row = sg.row0 + r;
-      const bool row_on = row < n * p.G;
-      const bool warp_on = sg.row0 + quarter * 32 < n * p.G;
+      const int rows = sg.rows(p);
+      const bool row_on = r < rows;
+      const bool warp_on = quarter * 32 < rows;
       const int node = row_on ? row / p.G : 0;
       const unsigned long long* mrow = p.mask + static_cast<long long>(sg.s.q0 + node) * p.words;
       float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
@@ -894,9 +913,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         if (lane == 0) mbar_arrive(p_full(w));
       }
       if (!ok) break;
-      Segment<kTcRows, kTcKeys> nx = sg;
-      const bool more = nx.next(p);
-      if (more) load_q(nx);
       ok = warp_wait(o_full, seg & 1, abort_flag, p.status);
       if (!ok) break;
       tc_fence_after();
@@ -906,7 +922,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       if (lane == 0) mbar_arrive(ml_full);
       ok = warp_wait(ml_full, seg & 1, abort_flag, p.status);
       if (!ok) break;
-      if (more) store_q();  // every MMA of this segment is done: Q may change
       // join the two groups; group w stores the columns [w D/2, (w + 1) D/2)
       if (warp_on) {
         const float2 ml0 = s_ml[r], ml1 = s_ml[128 + r];
@@ -921,7 +936,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           a1 *= inv;
         }
         const bool odd = s_odd[seg & 1] != 0;
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kTcRows + r;
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kMaxRows + r;
+        if (threadIdx.x == 128 && sg.tile0 > 0) p.parts[blockIdx.x] = sg.part(p, s_share->per);
         T* dst = static_cast<T*>(p.out) +
                  (static_cast<long long>(sg.s.q0 + node) * p.Hq + sg.h * p.G + row % p.G) * D + w * (D / 2);
         float* pdst = p.part + pr * D + w * (D / 2);
@@ -976,8 +992,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       if (lane == 0) mbar_arrive(o_free);
       seq += 2 * nt;
       ++seg;
-      sg = nx;
-      have = more;
+      have = sg.next(p);
     }
   }
   tc_fence_before();
@@ -989,92 +1004,115 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 }
 
 // -------------------------------------------------------------- the joining --
-// One CTA column per boundary between two shares; the first boundary inside a
-// row tile joins all its parts, one warp per row.
-template <typename T, int D, int ROWS, int KEYS>
-__global__ void __launch_bounds__(128) tree_join_kernel(const TreeParams p) {
+// A split row tile's parts lie in the CTAs c0 (slot 1) and c0 + 1 .. c1 (slot
+// 0); the block columns c0 + 1 .. c1 join its rows, an equal number each, so the
+// work is even whatever the number of parts. Few parts: a warp per row; many: a
+// row's parts are dealt to the warps of the block and summed in warp order.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinY = 4;  // blocks per column
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeParams p) {
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long per = *p.share;
-  const long long total = p.seq_base[p.num_seqs];
-  const long long x = per * (blockIdx.x + 1);
-  if (x >= total) return;
-  // the sequence of item x: the last with seq_base <= x (empty ones share a
-  // base with the next and are passed over)
-  int lo = 0, hi = p.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.seq_base[mid] <= x) lo = mid;
-    else hi = mid - 1;
-  }
-  const int b = lo;
-  const Seq s = seq_of<ROWS, KEYS>(p, b, false);
-  if (s.key_tiles == 0) return;
-  const long long at = x - p.seq_base[b];
-  const long long pair = at / s.key_tiles;
-  const long long first = p.seq_base[b] + pair * s.key_tiles, last = first + s.key_tiles - 1;
-  const int c0 = static_cast<int>(first / per), c1 = static_cast<int>(last / per);
-  if (first == x || c0 != static_cast<int>(blockIdx.x)) return;
-  const int h = static_cast<int>(pair / s.row_tiles);
-  const int row0 = static_cast<int>(pair - static_cast<long long>(h) * s.row_tiles) * ROWS;
-  const int r = blockIdx.y * 4 + warp;
-  if (row0 + r >= s.n * p.G) return;
   constexpr int DPL = D / 32;
-  float mx = -FLT_MAX;
-  for (int c = c0 + lane; c <= c1; c += 32)
-    mx = fmaxf(mx, p.part_ml[((static_cast<long long>(c) * 2 + (c == c0)) * ROWS + r) * 2]);
-  mx = warp_max(mx);
-  float acc[DPL], l = 0.f;
+  __shared__ float s_acc[kJoinWarps][D];
+  __shared__ float s_l[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = blockIdx.x + 1;
+  const Part pt = p.parts[c];
+  if (pt.c0 < 0) return;
+  const int helpers = pt.c1 - pt.c0, parts = helpers + 1;
+  const int units = helpers * kJoinY;  // blocks that share this row tile
+  const int unit = (c - pt.c0 - 1) * kJoinY + blockIdx.y;
+  const int r_begin = pt.rows * unit / units, r_end = pt.rows * (unit + 1) / units;
+  const bool deal = parts > kJoinWarps;  // deal a row's parts to the warps
+  auto base_of = [&](int k, int r) { return (static_cast<long long>(pt.c0 + k) * 2 + (k == 0)) * kMaxRows + r; };
+  for (int r0 = r_begin; r0 < r_end; r0 += deal ? 1 : kJoinWarps) {
+    const int r = deal ? r0 : r0 + warp;
+    const bool on = r < r_end;
+    float acc[DPL], l = 0.f;
 #pragma unroll
-  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+    for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+    if (on) {
+      float mx = -FLT_MAX;
+      for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, p.part_ml[base_of(k, r) * 2]);
+      mx = warp_max(mx);
+      const int step = deal ? kJoinWarps : 1;
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const long long pr = (static_cast<long long>(c) * 2 + (c == c0)) * ROWS + r;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + pr * 2);
-    const float w = exp2f(ml.x - mx);
-    l += w * ml.y;
-    const float* o = p.part + pr * D + lane * DPL;
+      for (int k = deal ? warp : 0; k < parts; k += step) {
+        const long long pr = base_of(k, r);
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + pr * 2);
+        const float* o = p.part + pr * D + lane * DPL;
+        const float w = exp2f(ml.x - mx);
+        l = fmaf(w, ml.y, l);
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] += w * o[i];
+        for (int i = 0; i < DPL; ++i) acc[i] = fmaf(w, o[i], acc[i]);
+      }
+    }
+    if (deal) {
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) s_acc[warp][lane * DPL + i] = acc[i];
+      if (lane == 0) s_l[warp] = l;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kJoinWarps; ++w) {
+          l += s_l[w];
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) acc[i] += s_acc[w][lane * DPL + i];
+        }
+      }
+      __syncthreads();
+    }
+    if (on && (!deal || warp == 0)) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int row = pt.row0 + r;
+      T* dst = static_cast<T*>(p.out) + (static_cast<long long>(pt.q0 + row / p.G) * p.Hq + pt.h * p.G + row % p.G) * D +
+               lane * DPL;
+#pragma unroll
+      for (int i = 0; i < DPL; i += 2)
+        *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+    }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int row = row0 + r;
-  T* dst = static_cast<T*>(p.out) + (static_cast<long long>(s.q0 + row / p.G) * p.Hq + h * p.G + row % p.G) * D +
-           lane * DPL;
-#pragma unroll
-  for (int i = 0; i < DPL; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
 }
 
 // ------------------------------------------------------------------- host --
 struct Plan {
   bool tc;
-  int rows, keys, ctas, min_share;
+  int tile_rows, ctas, min_share;
+  double items;  // bound of the call's work items
   size_t bytes;
 };
 
-// The tcgen05 kernel takes whole 16-key groups at 32-bit rows.
-bool tc_layout(int num_blocks, int block_size) {
-  return block_size % 16 == 0 && (static_cast<long long>(num_blocks) + 1) * block_size < INT32_MAX;
+// The tcgen05 kernel takes whole 16-key groups at 32-bit rows and the heads of
+// a group in one tile.
+bool tc_layout(int num_blocks, int block_size, int G) {
+  return block_size % 16 == 0 && (static_cast<long long>(num_blocks) + 1) * block_size < INT32_MAX && G <= kTcRows;
 }
 
 Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv, int D) {
   Plan pl{};
+  const int G = Hq / Hkv, keys = tc ? kTcKeys : kKeys;
   pl.tc = tc;
-  pl.rows = tc ? kTcRows : kRows;
-  pl.keys = tc ? kTcKeys : kKeys;
-  pl.min_share = 4;
-  const long long rt = (static_cast<long long>(max_q_len) * (Hq / Hkv) + pl.rows - 1) / pl.rows;
-  const long long kt = (static_cast<long long>(max_ctx) + pl.keys - 1) / pl.keys;
-  const double items = static_cast<double>(num_seqs) * Hkv * rt * kt;
-  long long ctas = tc ? kTcCtas : 2 * kTcCtas;
-  const double most = (items + pl.min_share - 1) / pl.min_share;
-  if (most < ctas) ctas = static_cast<long long>(most);
-  if (ctas < 1) ctas = 1;
-  pl.ctas = static_cast<int>(ctas);
-  const size_t parts = static_cast<size_t>(pl.ctas) * 2 * pl.rows;
-  pl.bytes = 256 + parts * (D + 2) * sizeof(float) + (static_cast<size_t>(num_seqs) + 2) * sizeof(long long);
+  pl.tile_rows = tc ? kTcRows / G * G : kRows;
+  const int key_tiles = (max_ctx + keys - 1) / keys;
+  // a share of fewer key tiles would pay more for its joining than it saves
+  pl.min_share = key_tiles < kMinShare ? key_tiles : kMinShare;
+  const int row_tiles = pl.tile_rows ? (max_q_len * G + pl.tile_rows - 1) / pl.tile_rows : 1;
+  pl.items = static_cast<double>(num_seqs) * Hkv * row_tiles * key_tiles;
+  const double most = pl.items / pl.min_share + 1;
+  const int ctas = tc ? kTcCtas : 2 * kTcCtas;
+  pl.ctas = most < ctas ? static_cast<int>(most) : ctas;
+  pl.bytes = 256 + static_cast<size_t>(pl.ctas) * (2 * kMaxRows * (D + 2) * sizeof(float) + sizeof(Part));
   return pl;
+}
+
+template <typename T, int D>
+int launch_join(const TreeParams& p, cudaStream_t s) {
+  if (p.num_ctas == 1) return PS_OK;
+  ps_host::launch(tree_join_kernel<T, D>, dim3(p.num_ctas - 1, kJoinY), kJoinWarps * 32, 0, s, p);
+  ps_host::count_launch();
+  return ps_host::check_launch("tree_attention(join)");
 }
 
 template <typename T, int D>
@@ -1088,37 +1126,36 @@ int launch_mma(TreeParams& p, cudaStream_t s) {
   }
   ps_host::launch(kern, p.num_ctas, kThreads, smem, s, p);
   ps_host::count_launch();
-  int rc = ps_host::check_launch("tree_attention");
-  if (rc != PS_OK || p.num_ctas == 1) return rc;
-  auto join = tree_join_kernel<T, D, kRows, kKeys>;
-  ps_host::launch(join, dim3(p.num_ctas - 1, kRows / 4), 128, 0, s, p);
-  ps_host::count_launch();
-  return ps_host::check_launch("tree_attention(join)");
+  const int rc = ps_host::check_launch("tree_attention");
+  return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
 }
 
-// One layer's cache as [num_blocks * block_size keys][Hkv][D], boxes of 16 keys
-// x 64 dims of one head, 128-byte swizzle.
-bool make_cache_map(CUtensorMap* map, const void* cache, bool bf16, int num_blocks, int block_size, int Hkv, int D) {
+// [rows][heads][D] of 16-bit values in boxes of box_rows x box_heads x 64 dims,
+// 128-byte swizzle: one layer's cache (16 keys of one head) or q (the nodes of
+// a tile, the heads of a group).
+bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, long long rows, int heads, int D, int box_heads,
+                   int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(Hkv),
-                        static_cast<cuuint64_t>(num_blocks) * block_size};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(Hkv) * D * 2};
-  cuuint32_t box[3] = {64, 1, 16};
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(heads) * D * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-            const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D>
 int launch_tc(TreeParams& p, cudaStream_t s) {
-  CUtensorMap km, vm;
+  CUtensorMap qm, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  if (!make_cache_map(&km, p.k_cache, bf16, p.num_blocks, p.block_size, p.Hkv, D) ||
-      !make_cache_map(&vm, p.v_cache, bf16, p.num_blocks, p.block_size, p.Hkv, D)) {
-    ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed for the KV cache");
+  const long long rows = static_cast<long long>(p.num_blocks) * p.block_size;
+  if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
+      !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 16) ||
+      !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 16)) {
+    ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
     return PS_ERR_CUDA;
   }
   auto kern = tree_tc_kernel<T, D>;
@@ -1127,14 +1164,10 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
     ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
     return PS_ERR_CUDA;
   }
-  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, km, vm, p);
+  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, km, vm, p);
   ps_host::count_launch();
-  int rc = ps_host::check_launch("tree_attention");
-  if (rc != PS_OK || p.num_ctas == 1) return rc;
-  auto join = tree_join_kernel<T, D, kTcRows, kTcKeys>;
-  ps_host::launch(join, dim3(p.num_ctas - 1, kTcRows / 4), 128, 0, s, p);
-  ps_host::count_launch();
-  return ps_host::check_launch("tree_attention(join)");
+  const int rc = ps_host::check_launch("tree_attention");
+  return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
 }
 
 }  // namespace
@@ -1194,7 +1227,12 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
     ps_host::set_error("tree_attention: dtype must be bf16 or f16");
     return PS_ERR_UNSUPPORTED;
   }
-  const Plan pl = plan_for(tc_layout(num_blocks, block_size), num_seqs, max_q_len, max_ctx, Hq, Hkv, D);
+  const Plan pl = plan_for(tc_layout(num_blocks, block_size, Hq / Hkv), num_seqs, max_q_len, max_ctx, Hq, Hkv, D);
+  if (pl.items > INT32_MAX - 1024) {
+    ps_host::set_error("tree_attention: %d sequences at context %d are more work items than 32 bits count", num_seqs,
+                       max_ctx);
+    return PS_ERR_UNSUPPORTED;
+  }
   if (!workspace || workspace_bytes < pl.bytes) {
     ps_host::set_error("tree_attention: workspace of %zu bytes needed, %zu given", pl.bytes, workspace_bytes);
     return PS_ERR_INVALID;
@@ -1209,11 +1247,10 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.start_pos = start_pos;
   p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
   const uintptr_t w = (reinterpret_cast<uintptr_t>(workspace) + 127) & ~static_cast<uintptr_t>(127);
-  const size_t parts = static_cast<size_t>(pl.ctas) * 2 * pl.rows;
+  const size_t parts = static_cast<size_t>(pl.ctas) * 2 * kMaxRows;
   p.part = reinterpret_cast<float*>(w);
   p.part_ml = p.part + parts * D;
-  p.seq_base = reinterpret_cast<long long*>(p.part_ml + parts * 2);
-  p.share = p.seq_base + num_seqs + 1;
+  p.parts = reinterpret_cast<Part*>(p.part_ml + parts * 2);
   p.status = ps_host::status_word(PS_TU_TREE);
   p.total_q = total_q;
   p.words = (max_q_len + 63) / 64;
@@ -1228,6 +1265,7 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.num_seqs = num_seqs;
   p.num_ctas = pl.ctas;
   p.min_share = pl.min_share;
+  p.tile_rows = pl.tile_rows;
   p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pl.tc) {
