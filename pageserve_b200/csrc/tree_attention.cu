@@ -61,6 +61,9 @@ struct TreeParams {
   int num_ctas;
   int min_share;   // fewest key tiles worth a CTA
   int tile_rows;   // query rows per tile
+  uint32_t rt_mul, rt_add, rt_magic;  // row tiles of n nodes: ((n * mul + add) * magic) >> 16
+  int box_shift;   // log2 of the keys per TMA box
+  int out32;       // out is 32-byte aligned
   float scale_log2;
 };
 
@@ -72,23 +75,24 @@ struct Seq {
   PS_DEVICE int items(int Hkv) const { return Hkv * row_tiles * key_tiles; }
 };
 
+// From the raw lengths; a sequence that breaks the call's bounds has no work.
 template <int KEYS>
-PS_DEVICE Seq seq_of(const TreeParams& p, int b, bool record) {
+PS_DEVICE Seq make_seq(const TreeParams& p, int q0, int q1, int start, bool* bad) {
   Seq s;
-  s.q0 = p.cu_q[b];
-  s.n = p.cu_q[b + 1] - s.q0;
-  s.start = p.start_pos[b];
-  s.row_tiles = s.key_tiles = 0;
-  if (s.n == 0) return s;
-  const long long ctx = static_cast<long long>(s.start) + s.n;
-  if (s.n < 0 || s.n > p.max_q_len || s.q0 < 0 || s.q0 + s.n > p.total_q || s.start < 0 || ctx > p.max_ctx) {
-    if (record) record_error(p.status, kErrShape);
-    s.n = 0;
-    return s;
-  }
-  s.row_tiles = (s.n * p.G + p.tile_rows - 1) / p.tile_rows;
-  s.key_tiles = (static_cast<int>(ctx) + KEYS - 1) / KEYS;
+  s.q0 = q0;
+  s.n = q1 - q0;
+  s.start = start;
+  const long long ctx = static_cast<long long>(start) + s.n;
+  *bad = s.n != 0 && (s.n < 0 || s.n > p.max_q_len || q0 < 0 || q1 > p.total_q || start < 0 || ctx > p.max_ctx);
+  if (*bad) s.n = 0;
+  s.row_tiles = ((s.n * p.rt_mul + p.rt_add) * p.rt_magic) >> 16;
+  s.key_tiles = s.n ? (static_cast<int>(ctx) + KEYS - 1) / KEYS : 0;
   return s;
+}
+template <int KEYS>
+PS_DEVICE Seq seq_of(const TreeParams& p, int b) {
+  bool bad;
+  return make_seq<KEYS>(p, p.cu_q[b], p.cu_q[b + 1], p.start_pos[b], &bad);
 }
 
 // A CTA's share of the work: items [begin, end), the sequence that holds begin
@@ -98,21 +102,41 @@ struct Share {
   Seq s;
 };
 
-// By one whole warp. The sequences' lengths are kept in registers between the
-// sum and the search (up to 256 of them): one round of global latency.
+// By one whole warp. The first 256 sequences' lengths are loaded at once and
+// kept in registers between the sum and the search: one round of latency.
 template <int KEYS>
 PS_DEVICE Share find_share(const TreeParams& p, int lane) {
   constexpr int kKeep = 8;
-  const bool lead = blockIdx.x == 0;
-  int items[kKeep];
-  int total = 0;
+  int q0[kKeep], q1[kKeep], st[kKeep], items[kKeep];
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
-    const int b = i * 32 + lane;
-    items[i] = b < p.num_seqs ? seq_of<KEYS>(p, b, lead).items(p.Hkv) : 0;
-    total += items[i];
+    const int b = min(i * 32 + lane, p.num_seqs - 1);
+    const bool on = i * 32 < p.num_seqs;  // warp-uniform
+    q0[i] = on ? p.cu_q[b] : 0;
+    q1[i] = on ? p.cu_q[b + 1] : 0;
+    st[i] = on ? p.start_pos[b] : 0;
   }
-  for (int b = kKeep * 32 + lane; b < p.num_seqs; b += 32) total += seq_of<KEYS>(p, b, lead).items(p.Hkv);
+  int total = 0;
+  bool any_bad = false;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    items[i] = 0;
+    if (i * 32 < p.num_seqs) {
+      bool bad;
+      const Seq s = make_seq<KEYS>(p, q0[i], q1[i], st[i], &bad);
+      if (i * 32 + lane < p.num_seqs) {
+        items[i] = s.items(p.Hkv);
+        any_bad |= bad;
+      }
+      total += items[i];
+    }
+  }
+  for (int b = kKeep * 32 + lane; b < p.num_seqs; b += 32) {
+    bool bad;
+    total += make_seq<KEYS>(p, p.cu_q[b], p.cu_q[b + 1], p.start_pos[b], &bad).items(p.Hkv);
+    any_bad |= bad;
+  }
+  if (any_bad && blockIdx.x == 0) record_error(p.status, kErrShape);
   total = __reduce_add_sync(0xffffffffu, total);
   Share r;
   r.per = max((total + p.num_ctas - 1) / p.num_ctas, p.min_share);
@@ -124,16 +148,7 @@ PS_DEVICE Share find_share(const TreeParams& p, int lane) {
   r.s = Seq{};
   if (r.begin >= r.end) return r;
   int run = 0;
-  for (int i = 0; i * 32 < p.num_seqs; ++i) {
-    const int b = i * 32 + lane;
-    int n = 0;
-    if (i < kKeep) {
-#pragma unroll
-      for (int k = 0; k < kKeep; ++k)
-        if (k == i) n = items[k];
-    } else if (b < p.num_seqs) {
-      n = seq_of<KEYS>(p, b, false).items(p.Hkv);
-    }
+  auto look = [&](int b0, int n) {
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -142,15 +157,30 @@ PS_DEVICE Share find_share(const TreeParams& p, int lane) {
     }
     const int first = run + incl - n;
     const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && r.begin >= first && r.begin < first + n);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      r.b = i * 32 + src;
-      r.base = __shfl_sync(0xffffffffu, first, src);
-      break;
-    }
     run += __shfl_sync(0xffffffffu, incl, 31);
+    if (!hit) return -1;
+    const int src = __ffs(hit) - 1;
+    r.b = b0 + src;
+    r.base = __shfl_sync(0xffffffffu, first, src);
+    return src;
+  };
+  bool found = false, bad;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    if (!found && i * 32 < p.num_seqs) {
+      const int src = look(i * 32, items[i]);
+      if (src >= 0) {
+        found = true;
+        r.s = make_seq<KEYS>(p, __shfl_sync(0xffffffffu, q0[i], src), __shfl_sync(0xffffffffu, q1[i], src),
+                             __shfl_sync(0xffffffffu, st[i], src), &bad);
+      }
+    }
   }
-  r.s = seq_of<KEYS>(p, r.b, false);
+  for (int b0 = kKeep * 32; !found && b0 < p.num_seqs; b0 += 32) {
+    const int b = b0 + lane;
+    found = look(b0, b < p.num_seqs ? seq_of<KEYS>(p, b).items(p.Hkv) : 0) >= 0;
+    if (found) r.s = seq_of<KEYS>(p, r.b);
+  }
   return r;
 }
 
@@ -173,7 +203,7 @@ struct Segment {
     int items = s.items(p.Hkv);
     while (cur >= base + items) {
       base += items;
-      s = seq_of<KEYS>(p, ++b, false);
+      s = seq_of<KEYS>(p, ++b);
       items = s.items(p.Hkv);
     }
     const uint32_t at = cur - base;
@@ -214,9 +244,33 @@ PS_DEVICE unsigned long long seen64(const unsigned long long* row, int words, in
   return v;
 }
 
+// Bits of the 128 keys from tree index `off` on; none for a row that is not used.
+PS_DEVICE uint4 seen128(bool on, const unsigned long long* row, int words, int off, int n) {
+  const unsigned long long a = on ? seen64(row, words, off, n) : 0ull, b = on ? seen64(row, words, off + 64, n) : 0ull;
+  return make_uint4(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
+                    static_cast<uint32_t>(b >> 32));
+}
+PS_DEVICE uint32_t pick(const uint4& v, int c) { return c < 2 ? (c ? v.y : v.x) : (c == 2 ? v.z : v.w); }
+
 template <typename T>
 PS_DEVICE bool finite16(uint16_t x) {
   return std::is_same<T, __half>::value ? (x & 0x7C00u) != 0x7C00u : (x & 0x7F80u) != 0x7F80u;
+}
+
+// Clears the values of 8 that are not finite; true if there were any.
+template <typename T>
+PS_DEVICE bool clear_odd(uint4& x) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+  bool hit = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (w[i] & kExp) == kExp, hi = (w[i] & (kExp << 16)) == (kExp << 16);
+    hit |= lo | hi;
+    if (lo) w[i] &= 0xFFFF0000u;
+    if (hi) w[i] &= 0x0000FFFFu;
+  }
+  return hit;
 }
 
 // --------------------------------------------------------- mma.sync kernel --
@@ -484,14 +538,15 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // query rows, 128-key tiles:
 //   warps 0, 3 TMA producers of K and of V: tiles go through one ring of equal
 //              slots in the order that the MMAs read them (K0 K1 V0 K2 V1 ...),
-//              as boxes of 16 keys x 64 dims, one lane a box; 16-key groups past
-//              the context or outside the pool are loads past the end of the
-//              tensor, which fill zeros. Boxes are issued at a bounded rate per
-//              warp: one warp for both tensors reached 4.7 TB/s, two 5.3
-//   warp 2     TMA producer of the Q tiles: 128 / G nodes x the G heads of the
-//              group (tile_rows = G * (128 / G) rows), again one box per 64 dims
-//   warp 1     TMEM and the MMAs: S_w = Q K_j^T (both operands in shared
-//              memory), O_w += P_w V_j (P from TMEM, V read MN-major)
+//              as boxes of up to 128 keys of one block x 64 dims, one lane a box;
+//              keys past the context or outside the pool are loads past the end
+//              of the tensor, which fill zeros. A warp issues boxes at a bounded
+//              rate: alone, 2 KB boxes (16-key blocks) streamed 4.9 TB/s from HBM
+//              with one warp, 5.95 with two, 6.3 with four. Dealing each tile to
+//              three warps was slower (445 against 423 us for the largest case)
+//   warp 1     TMEM, the Q tiles (128 / G nodes x the G heads of the group, one
+//              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
+//              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major)
 //   warps 4-11 two softmax groups of 4 warps, one row per thread; group w takes
 //              the key tiles w, w + 2, ... with its own S, O, max and sum, so
 //              that one group's exponentials run under the other's MMAs; at the
@@ -549,10 +604,104 @@ PS_DEVICE void tmem_ready(float* v) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
+PS_DEVICE void st_global_32(void* p, const uint32_t* v) {  // 32 bytes, 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 PS_DEVICE float ex2_approx(float x) {  // relative error about 2^-22, 0 for -inf; far below P's rounding to 16 bits
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two floats in one register pair, for the packed FMA pipe.
+typedef unsigned long long f32x2;
+PS_DEVICE f32x2 pack_f2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+PS_DEVICE void unpack_f2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+PS_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+PS_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+PS_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+PS_DEVICE float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values by 2^round(x) * q(x - round(x)), q the least relative error
+// polynomial of degree 5 for 2^r on [-1/2, 1/2] (fitted by iteratively
+// reweighted least squares): 2^-22, as ex2.approx. x is kept above -125 (2^-125
+// is nothing beside a sum of at least 2^-kSlack); NaN becomes 2^-125.
+PS_DEVICE f32x2 ex2_poly2(f32x2 x) {
+  float x0, x1;
+  unpack_f2(x, x0, x1);
+  x = pack_f2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const f32x2 big = pack_f2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are round(x)
+  const f32x2 t = add2(x, big);
+  const f32x2 r = fma2(add2(t, pack_f2(-12582912.f, -12582912.f)), pack_f2(-1.f, -1.f), x);
+  f32x2 q = pack_f2(0.00132764725f, 0.00132764725f);
+  q = fma2(q, r, pack_f2(0.00967554189f, 0.00967554189f));
+  q = fma2(q, r, pack_f2(0.0555071309f, 0.0555071309f));
+  q = fma2(q, r, pack_f2(0.240221202f, 0.240221202f));
+  q = fma2(q, r, pack_f2(0.693146944f, 0.693146944f));
+  q = fma2(q, r, pack_f2(1.00000012f, 1.00000012f));
+  float q0, q1, t0, t1;
+  unpack_f2(q, q0, q1);
+  unpack_f2(t, t0, t1);
+  return pack_f2(__uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23)),
+                 __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
+}
+// The max that P, O and the sum refer to stays until a row's scores pass it by
+// 2^kSlack: P <= 2^8 is well inside the 16-bit types.
+constexpr float kSlack = 8.f;
+// This thread's O row times alpha.
+template <int D>
+PS_DEVICE void scale_o(uint32_t t_o, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    float v[32];
+    tmem_ld32(t_o + c * 32, v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= alpha;
+    tmem_st16(t_o + c * 32, reinterpret_cast<const uint32_t*>(v));
+    tmem_st16(t_o + c * 32 + 16, reinterpret_cast<const uint32_t*>(v) + 16);
+  }
+  tmem_wait_st();
+}
+// The first n 16-column groups of this thread's P row times alpha (a power of
+// two: exact).
+template <typename T>
+PS_DEVICE void scale_p(uint32_t t_p, int n, float alpha) {
+  tmem_wait_st();
+#pragma unroll 1
+  for (int c = 0; c < n; ++c) {
+    float v[16];
+    tmem_ld16(t_p + c * 16, v);
+    uint32_t u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t in = __float_as_uint(v[i]);
+      const T* h = reinterpret_cast<const T*>(&in);
+      u[i] = pack2<T>(to_f32(h[0]) * alpha, to_f32(h[1]) * alpha);
+    }
+    tmem_st16(t_p + c * 16, u);
+  }
+  tmem_wait_st();
 }
 
 // After a wait gave up: let the copies or MMAs in flight end (bounded too).
@@ -590,11 +739,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   auto s_full = [&](int w) { return bars + 8 * (2 * kNS + w); };
   auto p_full = [&](int w) { return bars + 8 * (2 * kNS + 2 + w); };
   const uint32_t q_full = bars + 8 * (2 * kNS + 4);
-  const uint32_t q_empty = bars + 8 * (2 * kNS + 5);
-  const uint32_t o_full = bars + 8 * (2 * kNS + 6);
-  const uint32_t o_free = bars + 8 * (2 * kNS + 7);
-  const uint32_t ml_full = bars + 8 * (2 * kNS + 8);
-  const uint32_t drained = bars + 8 * (2 * kNS + 9);
+  const uint32_t o_full = bars + 8 * (2 * kNS + 5);
+  const uint32_t o_free = bars + 8 * (2 * kNS + 6);
+  const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
+  const uint32_t drained = bars + 8 * (2 * kNS + 8);
   unsigned char* misc = gbase + C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
   float2* s_ml = reinterpret_cast<float2*>(misc);  // [2 groups][128 rows]
   Share* s_share = reinterpret_cast<Share*>(misc + 2 * 128 * 8);
@@ -624,7 +772,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       mbar_init(p_full(w), 4);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, 8);
     mbar_init(ml_full, 8);
@@ -646,18 +793,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     // ---------------------------------------------------- K, V producers --
     const bool is_v = warp == 3;
     const CUtensorMap* map = is_v ? &vmap : &kmap;
+    const int groups = kTcKeys >> p.box_shift;  // boxes of a 64-dim panel
+    const int boxes = groups * C::kPanels;
+    const bool mine = lane < boxes;             // this lane's box of a tile
+    const int panel = lane / groups, grp = lane - panel * groups;
+    const uint32_t dst = ring + panel * (kTcKeys * 128) + (grp << p.box_shift) * 128;
+    const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
     uint32_t seq = 0;
     bool ok = true;
-    const int grp = lane & 7, panel = (lane >> 3) & 1;  // this lane's box of a tile
-    const bool mine = lane < 8 * C::kPanels;
-    const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
     while (ok && sg.next(p)) {
       const int nt = sg.tile1 - sg.tile0;
       const int ctx = sg.s.start + sg.s.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-      // row of this lane's 16-key group of tile j
+      // row of this lane's box of tile j
       auto row_of = [&](int j) {
-        const int key = (sg.tile0 + j) * kTcKeys + grp * 16;
+        const int key = (sg.tile0 + j) * kTcKeys + (grp << p.box_shift);
         if (!mine || j >= nt || key >= ctx) return past;
         const int phys = table[key / p.block_size];
         if (phys < 0 || phys >= p.num_blocks) {
@@ -681,8 +831,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           s_at[s] = at;
         }
         __syncwarp();
-        if (mine)
-          tma_load_3d(ring + s * C::kSlot + panel * (kTcKeys * 128) + grp * 2048, map, full(s), panel * 64, sg.h, r0);
+        if (mine) tma_load_3d(dst + s * C::kSlot, map, full(s), panel * 64, sg.h, r0);
         r0 = r1;
         r1 = r2;
       }
@@ -691,24 +840,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     if (!ok)
       for (int s = 0; s < kNS; ++s)
         if (s_at[s] != ~0u) drain_wait(full(s), (s_at[s] / kNS) & 1);
-  } else if (warp == 2) {
-    // -------------------------------------------------------- Q producer --
-    uint32_t seg = 0;
-    bool ok = true;
-    while (ok && sg.next(p)) {
-      if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1, abort_flag, p.status)) {
-        ok = false;
-        break;
-      }
-      if (lane == 0) {
-        mbar_expect_tx(q_full, C::kPanels * p.tile_rows * 128);
-        for (int pn = 0; pn < C::kPanels; ++pn)
-          tma_load_3d(q_sa + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G, sg.s.q0 + sg.row0 / p.G);
-      }
-      __syncwarp();
-      ++seg;
-    }
-    if (!ok && seg) drain_wait(q_full, (seg - 1) & 1);
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA --
     constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
@@ -717,6 +848,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
     bool ok = true;
     bool have = sg.next(p);
+    auto load_q = [&] {
+      if (lane == 0) {
+        mbar_expect_tx(q_full, C::kPanels * p.tile_rows * 128);
+        for (int pn = 0; pn < C::kPanels; ++pn)
+          tma_load_3d(q_sa + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G, sg.s.q0 + sg.row0 / p.G);
+      }
+      __syncwarp();
+    };
+    if (have) load_q();
     while (ok && have) {
       const int nt = sg.tile1 - sg.tile0;
       have = sg.next(p);  // the next segment's lengths arrive under this one's MMAs
@@ -737,33 +877,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           }
           mma_commit(empty(s));
           mma_commit(s_full(j & 1));
-          if (j == nt - 1) mma_commit(q_empty);
         }
         __syncwarp();
       };
       ok = warp_wait(q_full, seg & 1, abort_flag, p.status);
       if (!ok) break;
-      qk(0);
-      if (ok && nt > 1) qk(1);
-      if (ok && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-      for (int j = 0; ok && j < nt; ++j) {
-        const int w = j & 1;
-        const uint32_t at = seq + v_pos(j, nt);
-        const int s = static_cast<int>(at % kNS);
-        ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status) &&
-             warp_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
-        if (!ok) break;
-        ++tiles[w];
-        tc_fence_after();
-        if (lane == 0) {
+      for (int j = -2; ok && j < nt; ++j) {  // QK runs two tiles ahead of PV
+        if (j >= 0) {
+          const int w = j & 1;
+          const uint32_t at = seq + v_pos(j, nt);
+          const int s = static_cast<int>(at % kNS);
+          if (j == 0 && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+          ok = ok && warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status) &&
+               warp_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
+          if (!ok) break;
+          ++tiles[w];
+          if (j == nt - 1 && have) load_q();  // the last P is there, so every QK of this segment is done with Q
+          tc_fence_after();
+          if (lane == 0) {
 #pragma unroll
-          for (int kk = 0; kk < kTcKeys / 16; ++kk)
-            mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
-                   desc_lbo(ring + s * C::kSlot + kk * 16 * 128, kTcKeys * 128), id_pv, (j > 1 || kk > 0) ? 1u : 0u);
-          mma_commit(empty(s));
-          if (j == nt - 1) mma_commit(o_full);
+            for (int kk = 0; kk < kTcKeys / 16; ++kk)
+              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
+                     desc_lbo(ring + s * C::kSlot + kk * 16 * 128, kTcKeys * 128), id_pv, (j > 1 || kk > 0) ? 1u : 0u);
+            mma_commit(empty(s));
+            if (j == nt - 1) mma_commit(o_full);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         if (j + 2 < nt) qk(j + 2);
       }
       seq += 2 * nt;
@@ -772,6 +912,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     if (!ok) {
       if (lane == 0) mma_commit(drained);
       drain_wait(drained, 0);
+      drain_wait(q_full, seg & 1);
     }
   } else if (warp >= 4) {
     // ----------------------------------------------------------- softmax --
@@ -793,6 +934,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       const bool warp_on = quarter * 32 < rows;
       const int node = row_on ? row / p.G : 0;
       const unsigned long long* mrow = p.mask + static_cast<long long>(sg.s.q0 + node) * p.words;
+      // a row of one mask word is fetched before it is needed
+      const bool in_tree = sg.tile1 * kTcKeys > start;
+      const unsigned long long mword = in_tree && row_on ? mrow[0] : 0ull;
       float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
       for (int j = w; j < nt; j += 2) {
         const int key0 = (sg.tile0 + j) * kTcKeys;
@@ -807,22 +951,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           const int key = key0 + r;
           if (key >= start) {
             bool bad = false;
-#pragma unroll
-            for (int pn = 0; pn < C::kPanels; ++pn) {
-              uint4* line = reinterpret_cast<uint4*>(gbase + C::kQ + s * C::kSlot + pn * (kTcKeys * 128) + r * 128);
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                uint4 x = key < ctx ? line[c] : make_uint4(0, 0, 0, 0);
-                uint16_t* h = reinterpret_cast<uint16_t*>(&x);
-                bool hit = key >= ctx;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (!finite16<T>(h[e])) {
-                    h[e] = 0;
-                    hit = bad = true;
-                  }
-                if (hit) line[c] = x;
-              }
+            unsigned char* line = gbase + C::kQ + s * C::kSlot + r * 128;
+#pragma unroll 1
+            for (int i = 0; i < 8 * C::kPanels; ++i) {
+              // the lanes' lines share their banks: each starts at another chunk
+              uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * (kTcKeys * 128) + (((i ^ r) & 7) << 4));
+              uint4 x = key < ctx ? *at16 : make_uint4(0, 0, 0, 0);
+              const bool hit = clear_odd<T>(x);
+              bad |= hit;
+              if (hit || key >= ctx) *at16 = x;
             }
             if (bad) s_odd[seg & 1] = 1;
           }
@@ -833,80 +970,117 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         ++cnt;
         tc_fence_after();
         if (warp_on) {
-          // bits of the keys that this row sees (a row tile's unused rows: none)
-          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-          if (tail) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const unsigned long long v = row_on ? seen64(mrow, p.words, key0 + 64 * hf - start, n) : 0ull;
-              vis[2 * hf] = static_cast<uint32_t>(v);
-              vis[2 * hf + 1] = static_cast<uint32_t>(v >> 32);
-            }
-          }
-          float sv[2][32];
-          float mx = -INFINITY;
-          tmem_ld32_issue(t_s, sv[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld();
-            tmem_ready(sv[c & 1]);
-            if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv[(c + 1) & 1]);
-            if (tail) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if ((vis[c] >> i) & 1) mx = fmaxf(mx, sv[c & 1][i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) mx = fmaxf(mx, sv[c & 1][i]);
-            }
-          }
-          mx *= p.scale_log2;
-          // O is rescaled only when a row's max has grown by more than 2^8:
-          // P <= 2^8 stays well inside the 16-bit types, and sum and O share m_ref
-          float alpha = 1.f;
-          const bool moved = mx > m_ref + 8.f;
-          if (moved) {
-            alpha = m_ref == -FLT_MAX ? 0.f : ex2_approx(m_ref - mx);
-            m_ref = mx;
-          }
-          if (j >= 2 && __any_sync(0xffffffffu, moved)) {
-            const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
+          const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
+          float sv[32];
+          f32x2 sum = 0;
+          // the loops over 32-key groups stay rolled: unrolled, the kernel's code
+          // (168 KB) ran from beyond the instruction caches
+          if (tail || j < 2) {
+            // a group's first tile, and tiles with masked keys: the max, then the
+            // exponentials, in two passes over the scores
+            const uint4 vis = tail ? seen128(row_on, p.words == 1 ? &mword : mrow, p.words, key0 - start, n)
+                                   : make_uint4(~0u, ~0u, ~0u, ~0u);
+            float mx = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float v[32];
-              tmem_ld32(t_o + c * 32, v);
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld32_issue(t_s + c * 32, sv);
+              const uint32_t vc = pick(vis, c);
+              tmem_wait_ld();
+              tmem_ready(sv);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= alpha;
-              tmem_st16(t_o + c * 32, reinterpret_cast<const uint32_t*>(v));
-              tmem_st16(t_o + c * 32 + 16, reinterpret_cast<const uint32_t*>(v) + 16);
+              for (int i = 0; i < 32; i += 2)
+                mx = max3_nan(mx, (vc >> i) & 1 ? sv[i] : -INFINITY, (vc >> (i + 1)) & 1 ? sv[i + 1] : -INFINITY);
             }
-          }
-          float sum = 0.f;
-          tmem_ld32_issue(t_s, sv[0]);
-          // P's 16-bit columns c * 16 .. lie below the scores still to be read
+            mx *= p.scale_log2;
+            float alpha = 1.f;
+            const bool moved = row_on && !(mx <= m_ref + kSlack);
+            if (moved) {
+              // an infinite or NaN score makes the row NaN, as the formula does
+              if (!(mx <= FLT_MAX)) mx = NAN;
+              alpha = m_ref == -FLT_MAX ? 0.f : ex2_approx(m_ref - mx);
+              m_ref = mx;
+            }
+            if (j >= 2 && __any_sync(0xffffffffu, moved)) scale_o<D>(t_o, alpha);
+            l *= alpha;
+            // P's 16-bit columns c * 16 .. lie below the scores still to be read
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld32_issue(t_s + c * 32, sv);
+              const uint32_t vc = pick(vis, c);
+              tmem_wait_ld();
+              tmem_ready(sv);
+              uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld();
-            tmem_ready(sv[c & 1]);
-            if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv[(c + 1) & 1]);
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float x0 = fmaf(sv[c & 1][i], p.scale_log2, -m_ref), x1 = fmaf(sv[c & 1][i + 1], p.scale_log2, -m_ref);
-              if (tail) {
-                if (!((vis[c] >> i) & 1)) x0 = -INFINITY;
-                if (!((vis[c] >> (i + 1)) & 1)) x1 = -INFINITY;
+              for (int i = 0; i < 32; i += 2) {
+                const float p0 = ex2_approx((vc >> i) & 1 ? fmaf(sv[i], p.scale_log2, -m_ref) : -INFINITY);
+                const float p1 = ex2_approx((vc >> (i + 1)) & 1 ? fmaf(sv[i + 1], p.scale_log2, -m_ref) : -INFINITY);
+                sum = add2(sum, pack_f2(p0, p1));
+                // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12
+                // (f16) of a term, as the output's own rounding
+                pk[i / 2] = pack2<T>(p0, p1);
               }
-              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-              sum += p0 + p1;
-              // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12
-              // (f16) of a term, as the output's own rounding
-              pk[i / 2] = pack2<T>(p0, p1);
+              tmem_st16(t_s + c * 16, pk);
             }
-            tmem_st16(t_s + c * 16, pk);
+          } else {
+            // one pass against the max so far: a row whose scores have grown by
+            // more than 2^kSlack since (rare) rescales O, the sum and the P
+            // columns already stored by an exact power of two
+            const f32x2 scale2 = pack_f2(p.scale_log2, p.scale_log2);
+            tmem_ld32_issue(t_s, sv);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              tmem_wait_ld();
+              tmem_ready(sv);
+              f32x2 x[16];
+              const f32x2 neg_m = pack_f2(-m_ref, -m_ref);
+              float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                x[i] = fma2(pack_f2(sv[2 * i], sv[2 * i + 1]), scale2, neg_m);
+                float x0, x1;
+                unpack_f2(x[i], x0, x1);
+                if (i & 1) mx = max3_nan(mx, x0, x1);
+                else my = max3_nan(my, x0, x1);
+              }
+              if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv);  // under this group's exponentials
+              mx = max3_nan(mx, my, my);
+              const bool moved = row_on && !(mx <= kSlack);
+              if (__any_sync(0xffffffffu, moved)) {
+                const float up = !moved ? 0.f : (mx <= FLT_MAX ? ceilf(mx) : NAN);
+                const float alpha =
+                    up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
+                scale_o<D>(t_o, alpha);
+                scale_p<T>(t_s, c, alpha);
+                l *= alpha;
+                sum = mul2(sum, pack_f2(alpha, alpha));
+                m_ref += up;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = add2(x[i], pack_f2(-up, -up));
+              }
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float p0, p1;
+                if (i % 8 == 1 || i % 8 == 4 || i % 8 == 7) {
+                  // 3 of 8 on the FMA pipe: the special-function unit's 16
+                  // results a clock would bound the tile
+                  unpack_f2(ex2_poly2(x[i]), p0, p1);
+                } else {
+                  float x0, x1;
+                  unpack_f2(x[i], x0, x1);
+                  p0 = ex2_approx(x0);
+                  p1 = ex2_approx(x1);
+                }
+                sum = add2(sum, pack_f2(p0, p1));
+                pk[i] = pack2<T>(p0, p1);
+              }
+              tmem_st16(t_s + c * 16, pk);
+            }
           }
+          float s0, s1;
+          unpack_f2(sum, s0, s1);
+          l += s0 + s1;
           tmem_wait_st();
-          l = l * alpha + sum;
         }
         tc_fence_before();
         __syncwarp();
@@ -935,7 +1109,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           a0 *= inv;
           a1 *= inv;
         }
-        const bool odd = s_odd[seg & 1] != 0;
         const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kMaxRows + r;
         if (threadIdx.x == 128 && sg.tile0 > 0) p.parts[blockIdx.x] = sg.part(p, s_share->per);
         T* dst = static_cast<T*>(p.out) +
@@ -955,37 +1128,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             o0[i] *= a0;
             if (two) o0[i] = fmaf(o1[i], a1, o0[i]);
           }
-          if (odd && row_on) {
-            // the cleared values, to the rows that see them
-            const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-            const int k1 = min(sg.tile1 * kTcKeys, ctx);
-            for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
-              const int jn = key - start;
-              if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
-              const int phys = table[key / p.block_size];
-              if (phys < 0 || phys >= p.num_blocks) continue;
-              const T* vr = static_cast<const T*>(p.v_cache) +
-                            ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
-                            w * (D / 2) + c * 32;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const T x = vr[i];
-                if (!finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) o0[i] += to_f32(x);
-              }
-            }
-          }
           if (row_on) {
-            if (whole) {
+            // a store of a warp touches 32 rows, one line each: the wider the better
+            if (!whole) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o0 + i);
+              for (int i = 0; i < 32; i += 8) st_global_32(pdst + c * 32 + i, reinterpret_cast<const uint32_t*>(o0 + i));
+            } else if (p.out32) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 16) {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o0[i + 2 * e], o0[i + 2 * e + 1]);
+                st_global_32(dst + c * 32 + i, v);
+              }
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(pdst + c * 32 + i) = make_float4(o0[i], o0[i + 1], o0[i + 2], o0[i + 3]);
+              for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o0 + i);
             }
           }
         }
         if (!whole && row_on && w == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m, lt);
+        if (s_odd[seg & 1] != 0 && row_on) {
+          // the cleared values, added to what this thread has stored for a row that sees them
+          const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
+          const int k1 = min(sg.tile1 * kTcKeys, ctx);
+#pragma unroll 1
+          for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
+            const int jn = key - start;
+            if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
+            const int phys = table[key / p.block_size];
+            if (phys < 0 || phys >= p.num_blocks) continue;
+            const T* vr = static_cast<const T*>(p.v_cache) +
+                          ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
+                          w * (D / 2);
+#pragma unroll 1
+            for (int i = 0; i < D / 2; ++i) {
+              const T x = vr[i];
+              if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
+              if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
+              else pdst[i] += to_f32(x);
+            }
+          }
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -1016,8 +1200,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
   pdl_wait();
   pdl_trigger();
   constexpr int DPL = D / 32;
-  __shared__ float s_acc[kJoinWarps][D];
-  __shared__ float s_l[kJoinWarps];
+  __shared__ __align__(16) float s_acc[kJoinWarps][D];
+  __shared__ float2 s_ml[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x + 1;
   const Part pt = p.parts[c];
@@ -1031,37 +1215,50 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
   for (int r0 = r_begin; r0 < r_end; r0 += deal ? 1 : kJoinWarps) {
     const int r = deal ? r0 : r0 + warp;
     const bool on = r < r_end;
-    float acc[DPL], l = 0.f;
+    float acc[DPL], l = 0.f, m = -FLT_MAX;
 #pragma unroll
     for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-    if (on) {
-      float mx = -FLT_MAX;
-      for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, p.part_ml[base_of(k, r) * 2]);
-      mx = warp_max(mx);
-      const int step = deal ? kJoinWarps : 1;
-#pragma unroll 4
-      for (int k = deal ? warp : 0; k < parts; k += step) {
-        const long long pr = base_of(k, r);
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + pr * 2);
-        const float* o = p.part + pr * D + lane * DPL;
-        const float w = exp2f(ml.x - mx);
-        l = fmaf(w, ml.y, l);
+    // (max, sum, o) of one more part; the loads of kAhead parts are out at once
+    auto add = [&](float pm, float pl, const float* po) {
+      const float mn = fmaxf(m, pm);
+      const float a = exp2f(m - mn), w = exp2f(pm - mn);
+      m = mn;
+      l = l * a + w * pl;
 #pragma unroll
-        for (int i = 0; i < DPL; ++i) acc[i] = fmaf(w, o[i], acc[i]);
+      for (int i = 0; i < DPL; ++i) acc[i] = acc[i] * a + w * po[i];
+    };
+    if (on) {
+      constexpr int kAhead = 4;
+      const int step = deal ? kJoinWarps : 1;
+      for (int k0 = deal ? warp : 0; k0 < parts; k0 += kAhead * step) {
+        float2 ml[kAhead];
+        float o[kAhead][DPL];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int k = k0 + j * step;
+          if (k < parts) {
+            const long long pr = base_of(k, r);
+            ml[j] = *reinterpret_cast<const float2*>(p.part_ml + pr * 2);
+            const float* src = p.part + pr * D + lane * DPL;
+            if (DPL == 4) {
+              *reinterpret_cast<float4*>(o[j]) = *reinterpret_cast<const float4*>(src);
+            } else {
+              *reinterpret_cast<float2*>(o[j]) = *reinterpret_cast<const float2*>(src);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+          if (k0 + j * step < parts) add(ml[j].x, ml[j].y, o[j]);
       }
     }
     if (deal) {
 #pragma unroll
       for (int i = 0; i < DPL; ++i) s_acc[warp][lane * DPL + i] = acc[i];
-      if (lane == 0) s_l[warp] = l;
+      if (lane == 0) s_ml[warp] = make_float2(m, l);
       __syncthreads();
-      if (warp == 0) {
-        for (int w = 1; w < kJoinWarps; ++w) {
-          l += s_l[w];
-#pragma unroll
-          for (int i = 0; i < DPL; ++i) acc[i] += s_acc[w][lane * DPL + i];
-        }
-      }
+      if (warp == 0)
+        for (int w = 1; w < kJoinWarps; ++w) add(s_ml[w].x, s_ml[w].y, &s_acc[w][lane * DPL]);
       __syncthreads();
     }
     if (on && (!deal || warp == 0)) {
@@ -1152,9 +1349,12 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   CUtensorMap qm, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const long long rows = static_cast<long long>(p.num_blocks) * p.block_size;
+  p.box_shift = 4;  // the largest power of two of keys that lie together in a block, at most a tile
+  while (p.box_shift < 7 && p.block_size % (2 << p.box_shift) == 0) ++p.box_shift;
+  p.out32 = ps_host::aligned(p.out, 32);
   if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
-      !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 16) ||
-      !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 16)) {
+      !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift) ||
+      !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift)) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
     return PS_ERR_CUDA;
   }
@@ -1266,6 +1466,17 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.num_ctas = pl.ctas;
   p.min_share = pl.min_share;
   p.tile_rows = pl.tile_rows;
+  if (pl.tc) {
+    // ceil(n / t), t = tile_rows / G <= 128 nodes: exact, since (n + t - 1) * t < 2^16 for n <= 256
+    const uint32_t t = pl.tile_rows / p.G;
+    p.rt_mul = 1;
+    p.rt_add = t - 1;
+    p.rt_magic = (65536 + t - 1) / t;
+  } else {
+    p.rt_mul = p.G;
+    p.rt_add = kRows - 1;
+    p.rt_magic = 65536 / kRows;
+  }
   p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pl.tc) {
