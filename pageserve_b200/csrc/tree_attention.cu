@@ -7,9 +7,9 @@
 //
 // Rows are (node, q head of the kv head's group) pairs, row r = node * G + g,
 // so that a K/V tile is read once for the whole group. The work of a call is
-// the list of (sequence, kv head, row tile, key tile) in that order; its length
+// the list of (sequence, kv head, row group, key tile) in that order; its length
 // is known on the device only, and each CTA takes an equal, contiguous share of
-// it. A row tile whose key tiles fall into several shares leaves (o, max, sum)
+// it. A row group whose key tiles fall into several shares leaves (o, max, sum)
 // partials in the workspace (at most two per CTA, whatever the contexts), and
 // a second kernel joins them in order: no atomics, the same bits every time.
 //
@@ -29,9 +29,8 @@ using namespace ps;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxNodes = 256;
-constexpr int kMaxRows = 128;  // query rows per tile
 
-struct Part {  // the split row tile whose later part (slot 0) a CTA holds; c0 < 0: none
+struct Part {  // the split row group whose later part (slot 0) a CTA holds; c0 < 0: none
   int q0, h, row0, rows, c0, c1;  // rows to store; CTAs c0 (slot 1) .. c1 (slot 0) hold its parts
   int pad[2];
 };
@@ -45,8 +44,8 @@ struct TreeParams {
   const int32_t* cu_q;
   const int32_t* start_pos;
   const unsigned long long* mask;
-  float* part;     // [CTA][2 slots][kMaxRows][D] of o
-  float* part_ml;  // [CTA][2 slots][kMaxRows][2] of (max, sum)
+  float* part;     // [CTA][2 slots][group_rows][D] of o
+  float* part_ml;  // [CTA][2 slots][group_rows][2] of (max, sum)
   Part* parts;     // [CTA]
   int* status;
   int total_q;
@@ -61,18 +60,19 @@ struct TreeParams {
   int num_ctas;
   int min_share;   // fewest key tiles worth a CTA
   int tile_rows;   // query rows per tile
-  uint32_t rt_mul, rt_add, rt_magic;  // row tiles of n nodes: ((n * mul + add) * magic) >> 16
+  int group_rows;  // query rows per work item: one tile or two
+  uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
   int box_shift;   // log2 of the keys per TMA box
   int out32;       // out is 32-byte aligned
   float scale_log2;
 };
 
 // ------------------------------------------------------- division of work --
-// The work items of sequence b are (kv head, row tile, key tile), key tile
+// The work items of sequence b are (kv head, row group, key tile), key tile
 // fastest; the host has checked that a call's items fit 31 bits.
 struct Seq {
-  int q0, n, start, row_tiles, key_tiles;
-  PS_DEVICE int items(int Hkv) const { return Hkv * row_tiles * key_tiles; }
+  int q0, n, start, row_groups, key_tiles;
+  PS_DEVICE int items(int Hkv) const { return Hkv * row_groups * key_tiles; }
 };
 
 // From the raw lengths; a sequence that breaks the call's bounds has no work.
@@ -85,7 +85,7 @@ PS_DEVICE Seq make_seq(const TreeParams& p, int q0, int q1, int start, bool* bad
   const long long ctx = static_cast<long long>(start) + s.n;
   *bad = s.n != 0 && (s.n < 0 || s.n > p.max_q_len || q0 < 0 || q1 > p.total_q || start < 0 || ctx > p.max_ctx);
   if (*bad) s.n = 0;
-  s.row_tiles = ((s.n * p.rt_mul + p.rt_add) * p.rt_magic) >> 16;
+  s.row_groups = ((s.n * p.rg_mul + p.rg_add) * p.rg_magic) >> p.rg_shift;
   s.key_tiles = s.n ? (static_cast<int>(ctx) + KEYS - 1) / KEYS : 0;
   return s;
 }
@@ -184,7 +184,7 @@ PS_DEVICE Share find_share(const TreeParams& p, int lane) {
   return r;
 }
 
-// Walk over the segments (one row tile's key tiles) of a share.
+// Walk over the segments (one row group's key tiles) of a share.
 template <int KEYS>
 struct Segment {
   int cur, end, base, b;  // next item, share's end, first item of sequence b
@@ -209,19 +209,19 @@ struct Segment {
     const uint32_t at = cur - base;
     const uint32_t pair = at / static_cast<uint32_t>(s.key_tiles);
     tile0 = static_cast<int>(at - pair * s.key_tiles);
-    h = static_cast<int>(pair / static_cast<uint32_t>(s.row_tiles));
-    row0 = (static_cast<int>(pair) - h * s.row_tiles) * p.tile_rows;
+    h = static_cast<int>(pair / static_cast<uint32_t>(s.row_groups));
+    row0 = (static_cast<int>(pair) - h * s.row_groups) * p.group_rows;
     tile1 = min(tile0 + end - cur, s.key_tiles);
     cur += tile1 - tile0;
     return true;
   }
   PS_DEVICE bool whole() const { return tile0 == 0 && tile1 == s.key_tiles; }
-  // a row tile's first part is the last segment of its CTA, the others the first
+  // a row group's first part is the last segment of its CTA, the others the first
   PS_DEVICE int slot() const { return tile0 > 0 ? 0 : 1; }
-  PS_DEVICE int rows(const TreeParams& p) const { return min(p.tile_rows, s.n * p.G - row0); }
+  PS_DEVICE int rows(const TreeParams& p) const { return min(p.group_rows, s.n * p.G - row0); }
   // for a segment of slot 0
   PS_DEVICE Part part(const TreeParams& p, int per) const {
-    const int first = cur - tile1;  // the row tile's first item
+    const int first = cur - tile1;  // the row group's first item
     return Part{s.q0, h, row0, rows(p), first / per, (first + s.key_tiles - 1) / per, {0, 0}};
   }
 };
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
       }
     }
     const bool whole = sg.whole();
-    const long long pslot = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kMaxRows;
+    const long long pslot = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * p.group_rows;
     if (sg.tile0 > 0 && threadIdx.x == 0) p.parts[blockIdx.x] = sg.part(p, s_share.per);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -547,16 +547,20 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 //   warp 1     TMEM, the Q tiles (128 / G nodes x the G heads of the group, one
 //              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
 //              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major)
-//   warps 4-11 two softmax groups of 4 warps, one row per thread; group w takes
-//              the key tiles w, w + 2, ... with its own S, O, max and sum, so
-//              that one group's exponentials run under the other's MMAs; at the
-//              end of a row tile the two states are joined, each group storing
-//              half of the columns
-// A softmax thread reads its 128 scores twice from TMEM, 32 at a time (max, then
-// exponentials): holding them would need more than the 168 registers that 12
-// warps leave a thread.
-// TMEM: S0 | S1 | O0 | O1, 128 columns each; P_w overwrites S_w. MMAs of one
-// thread complete in order, so S_w(j) full also says that P_w(j - 2) V is done.
+//   warps 4-11 two softmax groups of 4 warps, one row per thread, each with its
+//              own S, O, max and sum. Of one row tile (up to 128 rows) group w
+//              takes the key tiles w, w + 2, ... and the two states are joined at
+//              the end of the row tile, each group storing half of the columns;
+//              of two row tiles group w takes tile w, and every key tile is
+//              loaded once for both
+// One group's exponentials run under the other's MMAs: step t (a key tile of
+// group t & 1) is QK(t), softmax, PV(t), and the MMA warp issues PV(t) QK(t + 2)
+// together, with one commit: what a commit costs the pipe is about one MMA, so
+// ring slots are given back by the softmax groups, for which S(t) complete says
+// that K of step t and V of step t - 2 have been read (MMAs complete in order).
+// A softmax thread reads its scores from TMEM 32 at a time: holding 128 would
+// need more than the 168 registers that 12 warps leave a thread.
+// TMEM: S0 | S1 | O0 | O1, 128 columns each; P_w overwrites S_w.
 // The ring and the barriers run on over the segments of a CTA's share: the next
 // segment's tiles load while the last one's output is stored.
 constexpr int kTcRows = 128;
@@ -570,8 +574,8 @@ struct Tc {
   static constexpr int kPanels = D / 64;                // 64-column panels of 128 rows x 128 bytes
   static constexpr int kSlot = kTcKeys * D * 2;         // one K or V tile
   static constexpr int kQ = kTcRows * D * 2;
-  static constexpr int kSlots = 192 * 1024 / kSlot;     // 6 (D = 128) or 12 (D = 64)
-  static constexpr int kSmem = kQ + kSlots * kSlot + 2560 /* barriers, (max, sum), flags */;
+  static constexpr int kSlots = (224 * 1024 - 2 * kQ) / kSlot;  // 5 (D = 128) or 12 (D = 64)
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 2560 /* barriers, (max, sum), flags */;
 };
 
 PS_DEVICE uint64_t desc_lbo(uint32_t addr, uint32_t lbo_bytes) {
@@ -711,9 +715,10 @@ PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
-// Order of a segment's loads: K_j and V_j among its 2 * nt tiles.
-PS_DEVICE int k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
-PS_DEVICE int v_pos(int j, int nt) { return min(nt, j + 2) + j; }
+// Order of a segment's loads, K_j and V_j among its 2 * nt tiles: as the MMAs
+// read them, QK two steps ahead of PV.
+PS_DEVICE int k_pos(int j, bool two) { return two ? 2 * j : (j < 2 ? j : 2 * j - 1); }
+PS_DEVICE int v_pos(int j, int nt, bool two) { return two ? 2 * j + 1 : min(nt, j + 2) + j; }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap qmap,
@@ -732,7 +737,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     if (threadIdx.x == 0) record_error(p.status, kErrShape);
     return;
   }
-  const uint32_t ring = q_sa + C::kQ;
+  const uint32_t ring = q_sa + 2 * C::kQ;
   const uint32_t bars = ring + kNS * C::kSlot;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (kNS + s); };
@@ -743,12 +748,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   const uint32_t o_free = bars + 8 * (2 * kNS + 6);
   const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
   const uint32_t drained = bars + 8 * (2 * kNS + 8);
-  unsigned char* misc = gbase + C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
+  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
   float2* s_ml = reinterpret_cast<float2*>(misc);  // [2 groups][128 rows]
   Share* s_share = reinterpret_cast<Share*>(misc + 2 * 128 * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 1);
-  volatile int* s_odd = abort_flag + 1;  // [2], by segment parity
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 1) + 3;
+  volatile int* s_odd = abort_flag + 1;  // [3], by segment mod 3
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 1) + 4;
   volatile uint32_t* s_at = tmem_slot + 1;  // [kNS] the tile last loaded into each slot
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -761,7 +766,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (threadIdx.x == 64) {
     *abort_flag = 0;
-    s_odd[0] = s_odd[1] = 0;
+    s_odd[0] = s_odd[1] = s_odd[2] = 0;
     for (int s = 0; s < kNS; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
@@ -799,10 +804,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const int panel = lane / groups, grp = lane - panel * groups;
     const uint32_t dst = ring + panel * (kTcKeys * 128) + (grp << p.box_shift) * 128;
     const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
-    uint32_t seq = 0;
+    uint32_t at = 0;  // position in the ring
     bool ok = true;
     while (ok && sg.next(p)) {
       const int nt = sg.tile1 - sg.tile0;
+      const bool two = sg.rows(p) > p.tile_rows;
       const int ctx = sg.s.start + sg.s.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
       // row of this lane's box of tile j
@@ -816,26 +822,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         }
         return phys * p.block_size + key % p.block_size;
       };
-      // rows are looked up two tiles ahead of their loads
-      int r0 = row_of(0), r1 = row_of(1);
-      for (int j = 0; j < nt; ++j) {
-        const int r2 = row_of(j + 2);
-        const uint32_t at = seq + (is_v ? v_pos(j, nt) : k_pos(j));
+      // Both producers walk all positions of the ring, so that neither is ever
+      // two phases away from a slot's barrier; each issues its own tensor's.
+      auto turn = [&](bool v, int row) {
         const int s = static_cast<int>(at % kNS);
         if (at >= kNS && !warp_wait(empty(s), ((at / kNS) - 1) & 1, abort_flag, p.status)) {
           ok = false;
-          break;
+          return;
         }
-        if (lane == 0) {
-          mbar_expect_tx(full(s), C::kSlot);
-          s_at[s] = at;
+        if (v == is_v) {
+          if (lane == 0) {
+            mbar_expect_tx(full(s), C::kSlot);
+            s_at[s] = at;
+          }
+          __syncwarp();
+          if (mine) tma_load_3d(dst + s * C::kSlot, map, full(s), panel * 64, sg.h, row);
         }
-        __syncwarp();
-        if (mine) tma_load_3d(dst + s * C::kSlot, map, full(s), panel * 64, sg.h, r0);
-        r0 = r1;
-        r1 = r2;
+        ++at;
+      };
+      // K_0 [K_1] V_0 K_2 V_1 ... of one row tile, K_0 V_0 K_1 V_1 ... of two;
+      // rows are looked up about two tiles ahead of their loads
+      const int ahead = two ? 1 : 2;
+      int row[3] = {row_of(0), row_of(1), row_of(2)};  // of the tiles j, j + 1, j + 2
+      turn(false, row[0]);
+      if (ok && !two && nt > 1) turn(false, row[1]);
+      for (int j = 0; ok && j < nt; ++j) {
+        const int next = row_of(j + 3);
+        turn(true, row[0]);
+        if (ok && j + ahead < nt) turn(false, two ? row[1] : row[2]);
+        row[0] = row[1];
+        row[1] = row[2];
+        row[2] = next;
       }
-      seq += 2 * nt;
     }
     if (!ok)
       for (int s = 0; s < kNS; ++s)
@@ -848,63 +866,59 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
     bool ok = true;
     bool have = sg.next(p);
-    auto load_q = [&] {
-      if (lane == 0) {
-        mbar_expect_tx(q_full, C::kPanels * p.tile_rows * 128);
+    auto load_q = [&] {  // by lane 0, of the segment in sg
+      const int tiles_q = sg.rows(p) > p.tile_rows ? 2 : 1;
+      mbar_expect_tx(q_full, tiles_q * C::kPanels * p.tile_rows * 128);
+      const int nodes = p.tile_rows / p.G;
+      for (int i = 0; i < tiles_q; ++i)
         for (int pn = 0; pn < C::kPanels; ++pn)
-          tma_load_3d(q_sa + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G, sg.s.q0 + sg.row0 / p.G);
-      }
-      __syncwarp();
+          tma_load_3d(q_sa + i * C::kQ + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G,
+                      sg.s.q0 + sg.row0 / p.G + i * nodes);
     };
-    if (have) load_q();
+    if (have && lane == 0) load_q();
+    __syncwarp();
     while (ok && have) {
       const int nt = sg.tile1 - sg.tile0;
+      const bool two = sg.rows(p) > p.tile_rows;
+      const int steps = two ? 2 * nt : nt;
       have = sg.next(p);  // the next segment's lengths arrive under this one's MMAs
-      auto qk = [&](int j) {
-        const uint32_t at = seq + k_pos(j);
-        const int s = static_cast<int>(at % kNS);
-        if (!warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status)) {
-          ok = false;
-          return;
+      ok = warp_wait(q_full, seg & 1, abort_flag, p.status);
+      for (int t = -2; ok && t < steps; ++t) {
+        const int w = t & 1;
+        const bool pv = t >= 0, qk = t + 2 < steps;
+        const uint32_t at_v = seq + v_pos(two ? t >> 1 : t, nt, two), at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
+        const int sv = static_cast<int>(at_v % kNS), sk = static_cast<int>(at_k % kNS);
+        if (pv) {
+          if (t == 0 && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+          ok = ok && warp_wait(full(sv), (at_v / kNS) & 1, abort_flag, p.status);
         }
+        if (ok && qk) ok = warp_wait(full(sk), (at_k / kNS) & 1, abort_flag, p.status);
+        if (ok && pv) ok = warp_wait(p_full(w), tiles[w]++ & 1, abort_flag, p.status);
+        if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
-            mma_f16(tmem + (j & 1) * 128, smem_desc_sw128(q_sa + off), smem_desc_sw128(ring + s * C::kSlot + off), id_qk,
-                    kk > 0 ? 1u : 0u);
-          }
-          mma_commit(empty(s));
-          mma_commit(s_full(j & 1));
-        }
-        __syncwarp();
-      };
-      ok = warp_wait(q_full, seg & 1, abort_flag, p.status);
-      if (!ok) break;
-      for (int j = -2; ok && j < nt; ++j) {  // QK runs two tiles ahead of PV
-        if (j >= 0) {
-          const int w = j & 1;
-          const uint32_t at = seq + v_pos(j, nt);
-          const int s = static_cast<int>(at % kNS);
-          if (j == 0 && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-          ok = ok && warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status) &&
-               warp_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
-          if (!ok) break;
-          ++tiles[w];
-          if (j == nt - 1 && have) load_q();  // the last P is there, so every QK of this segment is done with Q
-          tc_fence_after();
-          if (lane == 0) {
+          if (pv) {
+            const uint32_t v = ring + sv * C::kSlot;
 #pragma unroll
             for (int kk = 0; kk < kTcKeys / 16; ++kk)
-              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
-                     desc_lbo(ring + s * C::kSlot + kk * 16 * 128, kTcKeys * 128), id_pv, (j > 1 || kk > 0) ? 1u : 0u);
-            mma_commit(empty(s));
-            if (j == nt - 1) mma_commit(o_full);
+              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
+                     (t > 1 || kk > 0) ? 1u : 0u);
           }
-          __syncwarp();
+          if (qk) {
+            const uint32_t q = q_sa + (two ? w * C::kQ : 0), k = ring + sk * C::kSlot;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
+              mma_f16(tmem + w * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), id_qk, kk > 0 ? 1u : 0u);
+            }
+            mma_commit(s_full(w));
+          }
+          if (t == steps - 1) {
+            mma_commit(o_full);
+            if (have) load_q();  // the last P is there, so every QK of this segment is done with Q
+          }
         }
-        if (j + 2 < nt) qk(j + 2);
+        __syncwarp();
       }
       seq += 2 * nt;
       ++seg;
@@ -921,37 +935,55 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const int r = quarter * 32 + lane;  // this thread's row of the tile (its TMEM lane)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + w * 128 + lane_off;
-    uint32_t seq = 0, seg = 0, cnt = 0;
+    uint32_t seq = 0, seg = 0, cnt = 0, joined = 0;
     bool ok = true;
     bool have = sg.next(p);
     if (threadIdx.x == 128 && !(have && sg.tile0 > 0)) p.parts[blockIdx.x].c0 = -1;
     while (ok && have) {
       const int nt = sg.tile1 - sg.tile0;
       const int n = sg.s.n, start = sg.s.start, ctx = start + n;
-      const int row = sg.row0 + r;
-      const int rows = sg.rows(p);
+      const bool two = sg.rows(p) > p.tile_rows;
+      const int steps = two ? 2 * nt : nt;
+      const int lr = two ? w * p.tile_rows + r : r;  // row within the group
+      const int row = sg.row0 + lr;
+      const int rows = two ? min(p.tile_rows, sg.rows(p) - w * p.tile_rows) : sg.rows(p);
       const bool row_on = r < rows;
       const bool warp_on = quarter * 32 < rows;
       const int node = row_on ? row / p.G : 0;
+      // one thread of a group gives back the ring slots that its steps were the last to read
+      const bool gives = quarter == 0 && lane == 0 && (!two || w == 1);
+      auto give = [&](uint32_t at) { mbar_arrive(empty(static_cast<int>(at % kNS))); };
+      // s_odd of the next segment: last read two segments ago, next written after this segment's PVs
+      if (threadIdx.x == 128) s_odd[(seg + 1) % 3] = 0;
       const unsigned long long* mrow = p.mask + static_cast<long long>(sg.s.q0 + node) * p.words;
       // a row of one mask word is fetched before it is needed
       const bool in_tree = sg.tile1 * kTcKeys > start;
       const unsigned long long mword = in_tree && row_on ? mrow[0] : 0ull;
       float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
-      for (int j = w; j < nt; j += 2) {
+      for (int t = w; t < steps; t += 2) {
+        const int j = two ? t >> 1 : t;
         const int key0 = (sg.tile0 + j) * kTcKeys;
         const bool tail = key0 + kTcKeys > start;
-        if (tail) {
+        ok = warp_wait(s_full(w), cnt & 1, abort_flag, p.status);
+        if (!ok) break;
+        ++cnt;
+        if (gives) {
+          give(seq + k_pos(j, two));
+          if (t >= 2) give(seq + v_pos(two ? j - 1 : j - 2, nt, two));
+        }
+        if (tail && (!two || w == 0)) {
           // V rows past the context hold anything, and a drafted row's values
-          // that are not finite would reach rows that do not see it: clear them
-          const uint32_t at = seq + v_pos(j, nt);
+          // that are not finite would reach rows that do not see it: clear them.
+          // (S(t) is there, so the slot's last tile has been read and the wait
+          // below is for this V's phase and no earlier one.)
+          const uint32_t at = seq + v_pos(j, nt, two);
           const int s = static_cast<int>(at % kNS);
           ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status);
           if (!ok) break;
           const int key = key0 + r;
           if (key >= start) {
             bool bad = false;
-            unsigned char* line = gbase + C::kQ + s * C::kSlot + r * 128;
+            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + r * 128;
 #pragma unroll 1
             for (int i = 0; i < 8 * C::kPanels; ++i) {
               // the lanes' lines share their banks: each starts at another chunk
@@ -961,13 +993,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               bad |= hit;
               if (hit || key >= ctx) *at16 = x;
             }
-            if (bad) s_odd[seg & 1] = 1;
+            if (bad) s_odd[seg % 3] = 1;
           }
           fence_proxy_async();
         }
-        ok = warp_wait(s_full(w), cnt & 1, abort_flag, p.status);
-        if (!ok) break;
-        ++cnt;
         tc_fence_after();
         if (warp_on) {
           const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
@@ -975,7 +1004,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           f32x2 sum = 0;
           // the loops over 32-key groups stay rolled: unrolled, the kernel's code
           // (168 KB) ran from beyond the instruction caches
-          if (tail || j < 2) {
+          if (tail || t < 2) {
             // a group's first tile, and tiles with masked keys: the max, then the
             // exponentials, in two passes over the scores
             const uint4 vis = tail ? seen128(row_on, p.words == 1 ? &mword : mrow, p.words, key0 - start, n)
@@ -1000,7 +1029,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               alpha = m_ref == -FLT_MAX ? 0.f : ex2_approx(m_ref - mx);
               m_ref = mx;
             }
-            if (j >= 2 && __any_sync(0xffffffffu, moved)) scale_o<D>(t_o, alpha);
+            if (t >= 2 && __any_sync(0xffffffffu, moved)) scale_o<D>(t_o, alpha);
             l *= alpha;
             // P's 16-bit columns c * 16 .. lie below the scores still to be read
 #pragma unroll 1
@@ -1090,43 +1119,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       ok = warp_wait(o_full, seg & 1, abort_flag, p.status);
       if (!ok) break;
       tc_fence_after();
-      if (threadIdx.x == 128) s_odd[(seg + 1) & 1] = 0;
-      s_ml[w * 128 + r] = make_float2(m_ref, l);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ml_full);
-      ok = warp_wait(ml_full, seg & 1, abort_flag, p.status);
-      if (!ok) break;
-      // join the two groups; group w stores the columns [w D/2, (w + 1) D/2)
-      if (warp_on) {
+      if (gives && w < steps) give(seq + v_pos(two ? nt - 1 : ((steps - 1 - w) & ~1) + w, nt, two));
+      const bool whole = sg.whole();
+      float m = m_ref, lt = l, a0 = 1.f, a1 = 0.f;
+      const bool merge = !two && nt > 1;
+      if (merge) {
+        s_ml[w * 128 + r] = make_float2(m_ref, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ml_full);
+        ok = warp_wait(ml_full, joined++ & 1, abort_flag, p.status);
+        if (!ok) break;
         const float2 ml0 = s_ml[r], ml1 = s_ml[128 + r];
-        const bool two = nt > 1;
-        const float m = two ? fmaxf(ml0.x, ml1.x) : ml0.x;
-        float a0 = ex2_approx(ml0.x - m), a1 = two ? ex2_approx(ml1.x - m) : 0.f;
-        const float lt = two ? ml0.y * a0 + ml1.y * a1 : ml0.y;
-        const bool whole = sg.whole();
+        m = fmaxf(ml0.x, ml1.x);
+        a0 = ex2_approx(ml0.x - m);
+        a1 = ex2_approx(ml1.x - m);
+        lt = ml0.y * a0 + ml1.y * a1;
+      }
+      // one row tile: group w stores the columns [w D/2, (w + 1) D/2) of both
+      // groups' joined O (of one key tile: group 0 all of its own); two: its own
+      if (warp_on && (merge || two || w == 0)) {
         if (whole) {
           const float inv = lt == 0.f ? 0.f : 1.f / lt;
           a0 *= inv;
           a1 *= inv;
         }
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * kMaxRows + r;
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * p.group_rows + lr;
         if (threadIdx.x == 128 && sg.tile0 > 0) p.parts[blockIdx.x] = sg.part(p, s_share->per);
+        const int col0 = merge ? w * (D / 2) : 0, cols = merge ? D / 2 : D;
         T* dst = static_cast<T*>(p.out) +
-                 (static_cast<long long>(sg.s.q0 + node) * p.Hq + sg.h * p.G + row % p.G) * D + w * (D / 2);
-        float* pdst = p.part + pr * D + w * (D / 2);
+                 (static_cast<long long>(sg.s.q0 + node) * p.Hq + sg.h * p.G + row % p.G) * D + col0;
+        float* pdst = p.part + pr * D + col0;
+        const uint32_t t_own = tmem + 256 + (two ? w * 128 : 0) + lane_off + col0;
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
+        for (int c = 0; c < cols / 32; ++c) {
           float o0[32], o1[32];
-          const uint32_t t_o = tmem + 256 + lane_off + w * (D / 2) + c * 32;
-          tmem_ld32_issue(t_o, o0);
-          if (two) tmem_ld32_issue(t_o + 128, o1);
+          tmem_ld32_issue(t_own + c * 32, o0);
+          if (merge) tmem_ld32_issue(t_own + 128 + c * 32, o1);
           tmem_wait_ld();
           tmem_ready(o0);
-          if (two) tmem_ready(o1);
+          if (merge) tmem_ready(o1);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             o0[i] *= a0;
-            if (two) o0[i] = fmaf(o1[i], a1, o0[i]);
+            if (merge) o0[i] = fmaf(o1[i], a1, o0[i]);
           }
           if (row_on) {
             // a store of a warp touches 32 rows, one line each: the wider the better
@@ -1147,8 +1182,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
           }
         }
-        if (!whole && row_on && w == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m, lt);
-        if (s_odd[seg & 1] != 0 && row_on) {
+        if (!whole && row_on && col0 == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m, lt);
+        if (s_odd[seg % 3] != 0 && row_on) {
           // the cleared values, added to what this thread has stored for a row that sees them
           const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
           const int k1 = min(sg.tile1 * kTcKeys, ctx);
@@ -1160,9 +1195,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             if (phys < 0 || phys >= p.num_blocks) continue;
             const T* vr = static_cast<const T*>(p.v_cache) +
                           ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
-                          w * (D / 2);
+                          col0;
 #pragma unroll 1
-            for (int i = 0; i < D / 2; ++i) {
+            for (int i = 0; i < cols; ++i) {
               const T x = vr[i];
               if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
               if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
@@ -1188,7 +1223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 }
 
 // -------------------------------------------------------------- the joining --
-// A split row tile's parts lie in the CTAs c0 (slot 1) and c0 + 1 .. c1 (slot
+// A split row group's parts lie in the CTAs c0 (slot 1) and c0 + 1 .. c1 (slot
 // 0); the block columns c0 + 1 .. c1 join its rows, an equal number each, so the
 // work is even whatever the number of parts. Few parts: a warp per row; many: a
 // row's parts are dealt to the warps of the block and summed in warp order.
@@ -1207,11 +1242,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
   const Part pt = p.parts[c];
   if (pt.c0 < 0) return;
   const int helpers = pt.c1 - pt.c0, parts = helpers + 1;
-  const int units = helpers * kJoinY;  // blocks that share this row tile
+  const int units = helpers * kJoinY;  // blocks that share this row group
   const int unit = (c - pt.c0 - 1) * kJoinY + blockIdx.y;
   const int r_begin = pt.rows * unit / units, r_end = pt.rows * (unit + 1) / units;
   const bool deal = parts > kJoinWarps;  // deal a row's parts to the warps
-  auto base_of = [&](int k, int r) { return (static_cast<long long>(pt.c0 + k) * 2 + (k == 0)) * kMaxRows + r; };
+  auto base_of = [&](int k, int r) { return (static_cast<long long>(pt.c0 + k) * 2 + (k == 0)) * p.group_rows + r; };
   for (int r0 = r_begin; r0 < r_end; r0 += deal ? 1 : kJoinWarps) {
     const int r = deal ? r0 : r0 + warp;
     const bool on = r < r_end;
@@ -1276,7 +1311,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
 // ------------------------------------------------------------------- host --
 struct Plan {
   bool tc;
-  int tile_rows, ctas, min_share;
+  int tile_rows, group_rows, ctas, min_share;
   double items;  // bound of the call's work items
   size_t bytes;
 };
@@ -1292,15 +1327,16 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   const int G = Hq / Hkv, keys = tc ? kTcKeys : kKeys;
   pl.tc = tc;
   pl.tile_rows = tc ? kTcRows / G * G : kRows;
+  pl.group_rows = tc ? 2 * pl.tile_rows : kRows;
   const int key_tiles = (max_ctx + keys - 1) / keys;
   // a share of fewer key tiles would pay more for its joining than it saves
   pl.min_share = key_tiles < kMinShare ? key_tiles : kMinShare;
-  const int row_tiles = pl.tile_rows ? (max_q_len * G + pl.tile_rows - 1) / pl.tile_rows : 1;
-  pl.items = static_cast<double>(num_seqs) * Hkv * row_tiles * key_tiles;
+  const int row_groups = pl.group_rows ? (max_q_len * G + pl.group_rows - 1) / pl.group_rows : 1;
+  pl.items = static_cast<double>(num_seqs) * Hkv * row_groups * key_tiles;
   const double most = pl.items / pl.min_share + 1;
   const int ctas = tc ? kTcCtas : 2 * kTcCtas;
   pl.ctas = most < ctas ? static_cast<int>(most) : ctas;
-  pl.bytes = 256 + static_cast<size_t>(pl.ctas) * (2 * kMaxRows * (D + 2) * sizeof(float) + sizeof(Part));
+  pl.bytes = 256 + static_cast<size_t>(pl.ctas) * (2 * static_cast<size_t>(pl.group_rows) * (D + 2) * sizeof(float) + sizeof(Part));
   return pl;
 }
 
@@ -1447,7 +1483,7 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.start_pos = start_pos;
   p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
   const uintptr_t w = (reinterpret_cast<uintptr_t>(workspace) + 127) & ~static_cast<uintptr_t>(127);
-  const size_t parts = static_cast<size_t>(pl.ctas) * 2 * kMaxRows;
+  const size_t parts = static_cast<size_t>(pl.ctas) * 2 * pl.group_rows;
   p.part = reinterpret_cast<float*>(w);
   p.part_ml = p.part + parts * D;
   p.parts = reinterpret_cast<Part*>(p.part_ml + parts * 2);
@@ -1466,16 +1502,19 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.num_ctas = pl.ctas;
   p.min_share = pl.min_share;
   p.tile_rows = pl.tile_rows;
+  p.group_rows = pl.group_rows;
   if (pl.tc) {
-    // ceil(n / t), t = tile_rows / G <= 128 nodes: exact, since (n + t - 1) * t < 2^16 for n <= 256
-    const uint32_t t = pl.tile_rows / p.G;
-    p.rt_mul = 1;
-    p.rt_add = t - 1;
-    p.rt_magic = (65536 + t - 1) / t;
-  } else {
-    p.rt_mul = p.G;
-    p.rt_add = kRows - 1;
-    p.rt_magic = 65536 / kRows;
+    // ceil(n / t), t = group_rows / G <= 256 nodes: exact, since (n + t - 1) * t < 2^20 for n <= 256
+    const uint32_t t = pl.group_rows / p.G;
+    p.rg_mul = 1;
+    p.rg_add = t - 1;
+    p.rg_shift = 20;
+    p.rg_magic = ((1u << 20) + t - 1) / t;
+  } else {  // ceil(n * G / 64)
+    p.rg_mul = p.G;
+    p.rg_add = kRows - 1;
+    p.rg_shift = 6;
+    p.rg_magic = 1;
   }
   p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
