@@ -44,7 +44,7 @@ struct TreeParams {
   const int32_t* cu_q;
   const int32_t* start_pos;
   const unsigned long long* mask;
-  float* part;     // [CTA][2 slots][group_rows][D] of o
+  float* part;     // [CTA][2 slots][D / 8][group_rows][8] of o
   float* part_ml;  // [CTA][2 slots][group_rows][2] of (max, sum)
   Part* parts;     // [CTA]
   int* status;
@@ -62,7 +62,9 @@ struct TreeParams {
   int tile_rows;   // query rows per tile
   int group_rows;  // query rows per work item: one tile or two
   uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
+  int half_rows;   // rows of a Q tile that holds each row twice
   int box_shift;   // log2 of the keys per TMA box
+  int block_shift; // log2 of the block size, or -1
   int out32;       // out is 32-byte aligned
   float scale_log2;
 };
@@ -95,136 +97,155 @@ PS_DEVICE Seq seq_of(const TreeParams& p, int b) {
   return make_seq<KEYS>(p, p.cu_q[b], p.cu_q[b + 1], p.start_pos[b], &bad);
 }
 
-// A CTA's share of the work: items [begin, end), the sequence that holds begin
-// and that sequence's first item.
-struct Share {
-  int begin, end, per, b, base;
-  Seq s;
+// A CTA's share of the work, as segments (one row group's key tiles). Equal
+// shares cut row groups, which then have to be joined; where whole row groups,
+// an equal number per CTA, take at most kJoinCost key tiles longer, they are not
+// cut (64 sequences x 2 heads at equal contexts: 17 key tiles per CTA against 15
+// and a joining of about 6 us).
+constexpr int kJoinCost = 4;
+
+struct Cut {  // one segment
+  int b, q0, n, start;   // sequence, its first row, nodes and context
+  int h, row0, rows;     // kv head, rows [row0, row0 + rows) of the (node, head) rows
+  int tile0, nt, whole;  // key tiles [tile0, tile0 + nt); all of them
 };
 
-// By one whole warp. The first 256 sequences' lengths are loaded at once and
-// kept in registers between the sum and the search: one round of latency.
 template <int KEYS>
-PS_DEVICE Share find_share(const TreeParams& p, int lane) {
-  constexpr int kKeep = 8;
-  int q0[kKeep], q1[kKeep], st[kKeep], items[kKeep];
-#pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int b = min(i * 32 + lane, p.num_seqs - 1);
-    const bool on = i * 32 < p.num_seqs;  // warp-uniform
-    q0[i] = on ? p.cu_q[b] : 0;
-    q1[i] = on ? p.cu_q[b + 1] : 0;
-    st[i] = on ? p.start_pos[b] : 0;
-  }
-  int total = 0;
-  bool any_bad = false;
-#pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    items[i] = 0;
-    if (i * 32 < p.num_seqs) {
-      bool bad;
-      const Seq s = make_seq<KEYS>(p, q0[i], q1[i], st[i], &bad);
-      if (i * 32 + lane < p.num_seqs) {
-        items[i] = s.items(p.Hkv);
-        any_bad |= bad;
-      }
-      total += items[i];
-    }
-  }
-  for (int b = kKeep * 32 + lane; b < p.num_seqs; b += 32) {
-    bool bad;
-    total += make_seq<KEYS>(p, p.cu_q[b], p.cu_q[b + 1], p.start_pos[b], &bad).items(p.Hkv);
-    any_bad |= bad;
-  }
-  if (any_bad && blockIdx.x == 0) record_error(p.status, kErrShape);
-  total = __reduce_add_sync(0xffffffffu, total);
-  Share r;
-  r.per = max((total + p.num_ctas - 1) / p.num_ctas, p.min_share);
-  const long long lo = static_cast<long long>(r.per) * blockIdx.x;
-  r.begin = static_cast<int>(lo < total ? lo : total);
-  r.end = min(r.begin + r.per, total);
-  r.b = p.num_seqs;
-  r.base = total;
-  r.s = Seq{};
-  if (r.begin >= r.end) return r;
-  int run = 0;
-  auto look = [&](int b0, int n) {
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const int first = run + incl - n;
-    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && r.begin >= first && r.begin < first + n);
-    run += __shfl_sync(0xffffffffu, incl, 31);
-    if (!hit) return -1;
-    const int src = __ffs(hit) - 1;
-    r.b = b0 + src;
-    r.base = __shfl_sync(0xffffffffu, first, src);
-    return src;
-  };
-  bool found = false, bad;
-#pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    if (!found && i * 32 < p.num_seqs) {
-      const int src = look(i * 32, items[i]);
-      if (src >= 0) {
-        found = true;
-        r.s = make_seq<KEYS>(p, __shfl_sync(0xffffffffu, q0[i], src), __shfl_sync(0xffffffffu, q1[i], src),
-                             __shfl_sync(0xffffffffu, st[i], src), &bad);
-      }
-    }
-  }
-  for (int b0 = kKeep * 32; !found && b0 < p.num_seqs; b0 += 32) {
-    const int b = b0 + lane;
-    found = look(b0, b < p.num_seqs ? seq_of<KEYS>(p, b).items(p.Hkv) : 0) >= 0;
-    if (found) r.s = seq_of<KEYS>(p, r.b);
-  }
-  return r;
-}
-
-// Walk over the segments (one row group's key tiles) of a share.
-template <int KEYS>
-struct Segment {
-  int cur, end, base, b;  // next item, share's end, first item of sequence b
+struct Share {
+  int quota, unit, per, b, pair, tile0;  // quota: row groups (unit 1) or key tiles (unit 0) left
   Seq s;
-  int h, row0, tile0, tile1;
 
-  PS_DEVICE void init(const Share& sh) {
-    cur = sh.begin;
-    end = sh.end;
-    b = sh.b;
-    base = sh.base;
-    s = sh.s;
-  }
-  PS_DEVICE bool next(const TreeParams& p) {
-    if (cur >= end) return false;
-    int items = s.items(p.Hkv);
-    while (cur >= base + items) {
-      base += items;
-      s = seq_of<KEYS>(p, ++b);
-      items = s.items(p.Hkv);
+  // By one whole warp. The first 256 sequences' lengths are loaded at once and
+  // kept in registers between the sums and the search: one round of latency.
+  PS_DEVICE void find(const TreeParams& p, int lane) {
+    constexpr int kKeep = 8;
+    int q0[kKeep], q1[kKeep], st[kKeep], pairs[kKeep], tiles[kKeep];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+      const int b0 = min(i * 32 + lane, p.num_seqs - 1);
+      const bool on = i * 32 < p.num_seqs;  // warp-uniform
+      q0[i] = on ? p.cu_q[b0] : 0;
+      q1[i] = on ? p.cu_q[b0 + 1] : 0;
+      st[i] = on ? p.start_pos[b0] : 0;
     }
-    const uint32_t at = cur - base;
-    const uint32_t pair = at / static_cast<uint32_t>(s.key_tiles);
-    tile0 = static_cast<int>(at - pair * s.key_tiles);
-    h = static_cast<int>(pair / static_cast<uint32_t>(s.row_groups));
-    row0 = (static_cast<int>(pair) - h * s.row_groups) * p.group_rows;
-    tile1 = min(tile0 + end - cur, s.key_tiles);
-    cur += tile1 - tile0;
+    int total = 0, groups = 0, longest = 0;
+    bool any_bad = false;
+    auto count = [&](const Seq& q, bool bad) {
+      groups += p.Hkv * q.row_groups;
+      total += q.items(p.Hkv);
+      longest = max(longest, q.key_tiles);
+      any_bad |= bad;
+    };
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+      pairs[i] = tiles[i] = 0;
+      if (i * 32 + lane < p.num_seqs) {
+        bool bad;
+        const Seq q = make_seq<KEYS>(p, q0[i], q1[i], st[i], &bad);
+        pairs[i] = p.Hkv * q.row_groups;
+        tiles[i] = q.key_tiles;
+        count(q, bad);
+      }
+    }
+    for (int i = kKeep * 32 + lane; i < p.num_seqs; i += 32) {
+      bool bad;
+      const Seq q = make_seq<KEYS>(p, p.cu_q[i], p.cu_q[i + 1], p.start_pos[i], &bad);
+      count(q, bad);
+    }
+    if (any_bad && blockIdx.x == 0) record_error(p.status, kErrShape);
+    total = __reduce_add_sync(0xffffffffu, total);
+    groups = __reduce_add_sync(0xffffffffu, groups);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    per = max((total + p.num_ctas - 1) / p.num_ctas, p.min_share);
+    const int whole = (groups + p.num_ctas - 1) / p.num_ctas;
+    unit = static_cast<long long>(whole) * longest <= per + kJoinCost;
+    const long long lo = static_cast<long long>(unit ? whole : per) * blockIdx.x;
+    const int all = unit ? groups : total;
+    const int begin = static_cast<int>(lo < all ? lo : all);
+    quota = min(unit ? whole : per, all - begin);
+    if (quota <= 0) return;
+    int run = 0;
+    auto look = [&](int b0, int n) {  // the lane whose sequence holds `begin`, or -1
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const int first = run + incl - n;
+      const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && begin >= first && begin < first + n);
+      run += __shfl_sync(0xffffffffu, incl, 31);
+      if (!hit) return -1;
+      const int src = __ffs(hit) - 1;
+      b = b0 + src;
+      pair = begin - __shfl_sync(0xffffffffu, first, src);  // items for now
+      return src;
+    };
+    bool found = false, bad;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+      if (!found && i * 32 < p.num_seqs) {
+        const int src = look(i * 32, unit ? pairs[i] : pairs[i] * tiles[i]);
+        if (src >= 0) {
+          found = true;
+          s = make_seq<KEYS>(p, __shfl_sync(0xffffffffu, q0[i], src), __shfl_sync(0xffffffffu, q1[i], src),
+                             __shfl_sync(0xffffffffu, st[i], src), &bad);
+        }
+      }
+    }
+    for (int b0 = kKeep * 32; !found && b0 < p.num_seqs; b0 += 32) {
+      const Seq q = seq_of<KEYS>(p, min(b0 + lane, p.num_seqs - 1));
+      found = look(b0, b0 + lane < p.num_seqs ? (unit ? p.Hkv * q.row_groups : q.items(p.Hkv)) : 0) >= 0;
+      if (found) s = seq_of<KEYS>(p, b);
+    }
+    tile0 = 0;
+    if (!unit) {
+      const int items = pair;
+      pair = items / s.key_tiles;
+      tile0 = items - pair * s.key_tiles;
+    }
+  }
+
+  PS_DEVICE bool next(const TreeParams& p, Cut& c) {
+    if (quota <= 0) return false;
+    while (pair >= p.Hkv * s.row_groups) {  // the next sequence with work
+      s = seq_of<KEYS>(p, ++b);
+      pair = 0;
+    }
+    c.b = b;
+    c.q0 = s.q0;
+    c.n = s.n;
+    c.start = s.start;
+    c.h = pair / s.row_groups;
+    c.row0 = (pair - c.h * s.row_groups) * p.group_rows;
+    c.rows = min(p.group_rows, s.n * p.G - c.row0);
+    c.tile0 = tile0;
+    c.nt = unit ? s.key_tiles : min(s.key_tiles - tile0, quota);
+    c.whole = c.nt == s.key_tiles;
+    quota -= unit ? 1 : c.nt;
+    tile0 += c.nt;
+    if (tile0 == s.key_tiles) {
+      tile0 = 0;
+      ++pair;
+    }
     return true;
   }
-  PS_DEVICE bool whole() const { return tile0 == 0 && tile1 == s.key_tiles; }
-  // a row group's first part is the last segment of its CTA, the others the first
-  PS_DEVICE int slot() const { return tile0 > 0 ? 0 : 1; }
-  PS_DEVICE int rows(const TreeParams& p) const { return min(p.group_rows, s.n * p.G - row0); }
-  // for a segment of slot 0
-  PS_DEVICE Part part(const TreeParams& p, int per) const {
-    const int first = cur - tile1;  // the row group's first item
-    return Part{s.q0, h, row0, rows(p), first / per, (first + s.key_tiles - 1) / per, {0, 0}};
+  // Where the parts of a cut row group lie that began in an earlier CTA (c.tile0 > 0)
+  PS_DEVICE Part part(const Cut& c) const {
+    const int first = per * static_cast<int>(blockIdx.x) - c.tile0;  // the row group's first item
+    return Part{c.q0, c.h, c.row0, c.rows, first / per, (first + s.key_tiles - 1) / per, {0, 0}};
   }
 };
+// a row group's first part is the last segment of its CTA, the others the first
+PS_DEVICE int part_slot(const Cut& c) { return c.tile0 > 0 ? 0 : 1; }
+// Partial o of (CTA, slot): 8-column chunks of all rows, so that a warp whose
+// lanes hold a row each writes whole lines.
+PS_DEVICE float* part_o(const TreeParams& p, int cta, int slot, int row, int chunk, int D) {
+  return p.part + (static_cast<long long>(cta * 2 + slot) * (D / 8) + chunk) * p.group_rows * 8 + row * 8;
+}
+PS_DEVICE float2* part_ml(const TreeParams& p, int cta, int slot, int row) {
+  return reinterpret_cast<float2*>(p.part_ml) + static_cast<long long>(cta * 2 + slot) * p.group_rows + row;
+}
 
 // Bits of the 64 keys from tree index `off` on (keys before the tree are seen
 // by every node, keys behind it by none).
@@ -317,25 +338,26 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
   pdl_trigger();
   constexpr int kTile = kKeys * D * 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ Share s_share;
+  __shared__ Share<kKeys> s_share;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    const Share sh = find_share<kKeys>(p, lane);
+    Share<kKeys> sh;
+    sh.find(p, lane);
     if (lane == 0) {
       s_share = sh;
       p.parts[blockIdx.x].c0 = -1;
     }
   }
   __syncthreads();
-  Segment<kKeys> sg;
-  sg.init(s_share);
+  Share<kKeys> share = s_share;
+  Cut sg;
   const uint32_t base = smem_u32(smem);
   const int mat = lane >> 3;
-  while (sg.next(p)) {
-    const int ctx = sg.s.start + sg.s.n;
-    const int R = sg.s.n * p.G;
+  while (share.next(p, sg)) {
+    const int ctx = sg.start + sg.n;
+    const int R = sg.n * p.G;
     const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-    const int ntiles = sg.tile1 - sg.tile0;
+    const int ntiles = sg.nt;
     const int first_key = sg.tile0 * kKeys;
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
@@ -354,7 +376,7 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
       node[hf] = ok ? r / p.G : -1;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
           static_cast<const T*>(p.q) +
-          (static_cast<long long>(sg.s.q0 + (ok ? r / p.G : 0)) * p.Hq + sg.h * p.G + (ok ? r % p.G : 0)) * D);
+          (static_cast<long long>(sg.q0 + (ok ? r / p.G : 0)) * p.Hq + sg.h * p.G + (ok ? r % p.G : 0)) * D);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         qa[ks][hf] = ok ? src[ks * 8 + (lane & 3)] : 0u;
@@ -381,14 +403,14 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
       const uint32_t ks = base + (j % kStages) * 2 * kTile;
       const uint32_t vs = ks + kTile;
       const int t0 = first_key + j * kKeys;
-      const bool tail = t0 + kKeys > sg.s.start;  // drafted keys (or the end) in this tile
+      const bool tail = t0 + kKeys > sg.start;  // drafted keys (or the end) in this tile
       if (tail) {
         // clear drafted V values that are not finite: 0 * inf would reach rows that do not see them
         bool bad = false;
         uint16_t* vt = reinterpret_cast<uint16_t*>(smem + (vs - base));
         for (int i = threadIdx.x; i < kKeys * D; i += kThreads) {
           const int r = i / D, c = i % D;
-          if (t0 + r < sg.s.start || t0 + r >= ctx) continue;
+          if (t0 + r < sg.start || t0 + r >= ctx) continue;
           uint16_t* x = vt + swz(r, c >> 3, D * 2) / 2 + (c & 7);
           if (!finite16<T>(*x)) {
             bad = true;
@@ -403,8 +425,8 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
           vis[hf] = node[hf] < 0 ? 0ull
-                                 : seen64(p.mask + static_cast<long long>(sg.s.q0 + node[hf]) * p.words, p.words,
-                                          t0 - sg.s.start, sg.s.n);
+                                 : seen64(p.mask + static_cast<long long>(sg.q0 + node[hf]) * p.words, p.words,
+                                          t0 - sg.start, sg.n);
       }
       float s[8][4];
 #pragma unroll
@@ -485,17 +507,17 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
     }
     if (odd_values) {
       // add the cleared values to the rows that see them
-      const int k0 = max(first_key, sg.s.start), k1 = min(sg.tile1 * kKeys, ctx);
+      const int k0 = max(first_key, sg.start), k1 = min((sg.tile0 + sg.nt) * kKeys, ctx);
       for (int key = k0; key < k1; ++key) {
         const int phys = table[key / p.block_size];
         if (phys < 0 || phys >= p.num_blocks) continue;
         const T* vr = static_cast<const T*>(p.v_cache) +
                       ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D;
-        const int jn = key - sg.s.start;
+        const int jn = key - sg.start;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           if (node[hf] < 0 ||
-              !((p.mask[static_cast<long long>(sg.s.q0 + node[hf]) * p.words + (jn >> 6)] >> (jn & 63)) & 1))
+              !((p.mask[static_cast<long long>(sg.q0 + node[hf]) * p.words + (jn >> 6)] >> (jn & 63)) & 1))
             continue;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
@@ -507,27 +529,25 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
         }
       }
     }
-    const bool whole = sg.whole();
-    const long long pslot = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * p.group_rows;
-    if (sg.tile0 > 0 && threadIdx.x == 0) p.parts[blockIdx.x] = sg.part(p, s_share.per);
+    const int slot = part_slot(sg);
+    if (sg.tile0 > 0 && threadIdx.x == 0) p.parts[blockIdx.x] = share.part(sg);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int r = wrow + (lane >> 2) + hf * 8;
       if (r >= R) continue;
-      if (whole) {
+      if (sg.whole) {
         const float inv = l[hf] == 0.f ? 0.f : 1.f / l[hf];
         T* dst = static_cast<T*>(p.out) +
-                 (static_cast<long long>(sg.s.q0 + r / p.G) * p.Hq + sg.h * p.G + r % p.G) * D + 2 * (lane & 3);
+                 (static_cast<long long>(sg.q0 + r / p.G) * p.Hq + sg.h * p.G + r % p.G) * D + 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
           *reinterpret_cast<uint32_t*>(dst + i * 8) = pack2<T>(o[i][2 * hf] * inv, o[i][2 * hf + 1] * inv);
       } else {
-        const long long pr = pslot + r - sg.row0;
-        float* dst = p.part + pr * D + 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
-        if ((lane & 3) == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m[hf], l[hf]);
+          *reinterpret_cast<float2*>(part_o(p, blockIdx.x, slot, r - sg.row0, i, D) + 2 * (lane & 3)) =
+              make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
+        if ((lane & 3) == 0) *part_ml(p, blockIdx.x, slot, r - sg.row0) = make_float2(m[hf], l[hf]);
       }
     }
   }
@@ -544,15 +564,20 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 //              rate: alone, 2 KB boxes (16-key blocks) streamed 4.9 TB/s from HBM
 //              with one warp, 5.95 with two, 6.3 with four. Dealing each tile to
 //              three warps was slower (445 against 423 us for the largest case)
+//   warp 2     walks the CTA's share and hands its segments to the other roles
 //   warp 1     TMEM, the Q tiles (128 / G nodes x the G heads of the group, one
 //              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
-//              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major)
+//              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major), all
+//              by one thread
 //   warps 4-11 two softmax groups of 4 warps, one row per thread, each with its
 //              own S, O, max and sum. Of one row tile (up to 128 rows) group w
 //              takes the key tiles w, w + 2, ... and the two states are joined at
 //              the end of the row tile, each group storing half of the columns;
 //              of two row tiles group w takes tile w, and every key tile is
-//              loaded once for both
+//              loaded once for both. Of at most 64 rows the Q tile holds each row
+//              twice and group 1 works on the upper copies: a softmax step is
+//              bound by its SM sub-partition (TMEM lanes are fixed to warps), and
+//              this puts the groups on different ones
 // One group's exponentials run under the other's MMAs: step t (a key tile of
 // group t & 1) is QK(t), softmax, PV(t), and the MMA warp issues PV(t) QK(t + 2)
 // together, with one commit: what a commit costs the pipe is about one MMA, so
@@ -575,7 +600,7 @@ struct Tc {
   static constexpr int kSlot = kTcKeys * D * 2;         // one K or V tile
   static constexpr int kQ = kTcRows * D * 2;
   static constexpr int kSlots = (224 * 1024 - 2 * kQ) / kSlot;  // 5 (D = 128) or 12 (D = 64)
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 2560 /* barriers, (max, sum), flags */;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 3072 /* barriers, (max, sum), flags */;
 };
 
 PS_DEVICE uint64_t desc_lbo(uint32_t addr, uint32_t lbo_bytes) {
@@ -720,8 +745,33 @@ PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
 PS_DEVICE int k_pos(int j, bool two) { return two ? 2 * j : (j < 2 ? j : 2 * j - 1); }
 PS_DEVICE int v_pos(int j, int nt, bool two) { return two ? 2 * j + 1 : min(nt, j + 2) + j; }
 
+// A segment as the roles read it.
+struct Seg {
+  int b, q0, n, start, h, row0, rows, tile0, nt;
+  int flags;
+};
+enum SegFlags : int { kSegStop = 1, kSegWhole = 2, kSegTwo = 4, kSegDup = 8 };
+constexpr int kSegRing = 4;
+constexpr int kSegReaders = 11;  // two producers, the MMA thread, eight softmax warps
+
+// Bounded wait of one thread (see warp_wait).
+PS_DEVICE bool thread_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *abort_flag = 1;
+      record_error(status, kErrTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap qmap,
+                                                                const __grid_constant__ CUtensorMap qhalf,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
                                                                 const TreeParams p) {
@@ -748,23 +798,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   const uint32_t o_free = bars + 8 * (2 * kNS + 6);
   const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
   const uint32_t drained = bars + 8 * (2 * kNS + 8);
-  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10);
+  auto seg_full = [&](int i) { return bars + 8 * (2 * kNS + 9 + i); };
+  auto seg_empty = [&](int i) { return bars + 8 * (2 * kNS + 9 + kSegRing + i); };
+  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10 + 2 * kSegRing);
   float2* s_ml = reinterpret_cast<float2*>(misc);  // [2 groups][128 rows]
-  Share* s_share = reinterpret_cast<Share*>(misc + 2 * 128 * 8);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 1);
+  Seg* s_seg = reinterpret_cast<Seg*>(misc + 2 * 128 * 8);  // [kSegRing]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_seg + kSegRing);
   volatile int* s_odd = abort_flag + 1;  // [3], by segment mod 3
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_share + 1) + 4;
+  uint32_t* tmem_slot = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(abort_flag + 4));
   volatile uint32_t* s_at = tmem_slot + 1;  // [kNS] the tile last loaded into each slot
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    const Share sh = find_share<kTcKeys>(p, lane);
-    if (lane == 0) *s_share = sh;
-  } else if (warp == 1) {
+  if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else if (threadIdx.x == 64) {
+  } else if (threadIdx.x == 0) {
     *abort_flag = 0;
     s_odd[0] = s_odd[1] = s_odd[2] = 0;
     for (int s = 0; s < kNS; ++s) {
@@ -781,20 +830,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     mbar_init(o_free, 8);
     mbar_init(ml_full, 8);
     mbar_init(drained, 1);
+    for (int i = 0; i < kSegRing; ++i) {
+      mbar_init(seg_full(i), 1);
+      mbar_init(seg_empty(i), kSegReaders);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   } else if (threadIdx.x == 96) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qhalf)) : "memory");
   }
+  Share<kTcKeys> share;
+  if (warp == 2) share.find(p, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Segment<kTcKeys> sg;
-  sg.init(*s_share);
+  const int tile_nodes = p.tile_rows / p.G, half_rows = p.half_rows;
 
-  if (warp == 0 || warp == 3) {
+  // segment i for a reading warp; false: there is none, or a wait gave up
+  auto read_seg = [&](uint32_t i, Seg& sg) {
+    if (!warp_wait(seg_full(i % kSegRing), (i / kSegRing) & 1, abort_flag, p.status)) return false;
+    sg = s_seg[i % kSegRing];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(seg_empty(i % kSegRing));
+    return !(sg.flags & kSegStop);
+  };
+
+  if (warp == 2) {
+    // ----------------------------------------------------------- planner --
+    if (lane == 0) p.parts[blockIdx.x].c0 = -1;
+    bool more = true, ok = true;
+    for (uint32_t i = 0; ok && more; ++i) {
+      Cut c;
+      more = share.next(p, c);
+      if (i >= kSegRing) ok = warp_wait(seg_empty(i % kSegRing), ((i / kSegRing) - 1) & 1, abort_flag, p.status);
+      if (ok && lane == 0) {
+        Seg sg{};
+        sg.flags = kSegStop;
+        if (more) {
+          sg = Seg{c.b, c.q0, c.n, c.start, c.h, c.row0, c.rows, c.tile0, c.nt, 0};
+          if (c.whole) sg.flags |= kSegWhole;
+          if (c.rows > p.tile_rows) sg.flags |= kSegTwo;
+          else if (c.rows <= half_rows && c.nt > 1) sg.flags |= kSegDup;
+          if (c.tile0 > 0) p.parts[blockIdx.x] = share.part(c);
+        }
+        s_seg[i % kSegRing] = sg;
+        mbar_arrive(seg_full(i % kSegRing));
+      }
+      __syncwarp();
+    }
+  } else if (warp == 0 || warp == 3) {
     // ---------------------------------------------------- K, V producers --
     const bool is_v = warp == 3;
     const CUtensorMap* map = is_v ? &vmap : &kmap;
@@ -806,21 +893,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
     uint32_t at = 0;  // position in the ring
     bool ok = true;
-    while (ok && sg.next(p)) {
-      const int nt = sg.tile1 - sg.tile0;
-      const bool two = sg.rows(p) > p.tile_rows;
-      const int ctx = sg.s.start + sg.s.n;
+    Seg sg;
+    for (uint32_t i = 0; ok && read_seg(i, sg); ++i) {
+      const int nt = sg.nt;
+      const bool two = sg.flags & kSegTwo;
+      const int ctx = sg.start + sg.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
       // row of this lane's box of tile j
       auto row_of = [&](int j) {
         const int key = (sg.tile0 + j) * kTcKeys + (grp << p.box_shift);
         if (!mine || j >= nt || key >= ctx) return past;
-        const int phys = table[key / p.block_size];
+        const int entry = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
+        const int phys = table[entry];
         if (phys < 0 || phys >= p.num_blocks) {
           record_error(p.status, kErrBlockId);
           return past;
         }
-        return phys * p.block_size + key % p.block_size;
+        return phys * p.block_size + key - entry * p.block_size;
       };
       // Both producers walk all positions of the ring, so that neither is ever
       // two phases away from a slot's barrier; each issues its own tensor's.
@@ -843,60 +932,77 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       // K_0 [K_1] V_0 K_2 V_1 ... of one row tile, K_0 V_0 K_1 V_1 ... of two;
       // rows are looked up about two tiles ahead of their loads
       const int ahead = two ? 1 : 2;
-      int row[3] = {row_of(0), row_of(1), row_of(2)};  // of the tiles j, j + 1, j + 2
-      turn(false, row[0]);
-      if (ok && !two && nt > 1) turn(false, row[1]);
+      int row0 = row_of(0), row1 = row_of(1), row2 = row_of(2);  // of the tiles j, j + 1, j + 2
+      turn(false, row0);
+      if (ok && !two && nt > 1) turn(false, row1);
       for (int j = 0; ok && j < nt; ++j) {
         const int next = row_of(j + 3);
-        turn(true, row[0]);
-        if (ok && j + ahead < nt) turn(false, two ? row[1] : row[2]);
-        row[0] = row[1];
-        row[1] = row[2];
-        row[2] = next;
+        turn(true, row0);
+        if (ok && j + ahead < nt) turn(false, two ? row1 : row2);
+        row0 = row1;
+        row1 = row2;
+        row2 = next;
       }
     }
-    if (!ok)
+    if (*abort_flag)
       for (int s = 0; s < kNS; ++s)
         if (s_at[s] != ~0u) drain_wait(full(s), (s_at[s] / kNS) & 1);
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA --
-    constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
-    constexpr uint32_t id_pv = idesc_bmn(kBf16, 128, D);
-    uint32_t seq = 0, seg = 0;
-    uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
-    bool ok = true;
-    bool have = sg.next(p);
-    auto load_q = [&] {  // by lane 0, of the segment in sg
-      const int tiles_q = sg.rows(p) > p.tile_rows ? 2 : 1;
-      mbar_expect_tx(q_full, tiles_q * C::kPanels * p.tile_rows * 128);
-      const int nodes = p.tile_rows / p.G;
-      for (int i = 0; i < tiles_q; ++i)
-        for (int pn = 0; pn < C::kPanels; ++pn)
-          tma_load_3d(q_sa + i * C::kQ + pn * (kTcRows * 128), &qmap, q_full, pn * 64, sg.h * p.G,
-                      sg.s.q0 + sg.row0 / p.G + i * nodes);
-    };
-    if (have && lane == 0) load_q();
-    __syncwarp();
-    while (ok && have) {
-      const int nt = sg.tile1 - sg.tile0;
-      const bool two = sg.rows(p) > p.tile_rows;
-      const int steps = two ? 2 * nt : nt;
-      have = sg.next(p);  // the next segment's lengths arrive under this one's MMAs
-      ok = warp_wait(q_full, seg & 1, abort_flag, p.status);
-      for (int t = -2; ok && t < steps; ++t) {
-        const int w = t & 1;
-        const bool pv = t >= 0, qk = t + 2 < steps;
-        const uint32_t at_v = seq + v_pos(two ? t >> 1 : t, nt, two), at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
-        const int sv = static_cast<int>(at_v % kNS), sk = static_cast<int>(at_k % kNS);
-        if (pv) {
-          if (t == 0 && seg > 0) ok = warp_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-          ok = ok && warp_wait(full(sv), (at_v / kNS) & 1, abort_flag, p.status);
+    if (lane == 0) {
+      constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
+      constexpr uint32_t id_pv = idesc_bmn(kBf16, 128, D);
+      uint32_t seq = 0, seg = 0, q_loads = 0;
+      uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
+      bool ok = true;
+      Seg nx;
+      auto take = [&](uint32_t i) {  // segment i into nx
+        if (!thread_wait(seg_full(i % kSegRing), (i / kSegRing) & 1, abort_flag, p.status)) return false;
+        nx = s_seg[i % kSegRing];
+        mbar_arrive(seg_empty(i % kSegRing));
+        return !(nx.flags & kSegStop);
+      };
+      auto load_q = [&] {  // of nx
+        const bool two = nx.flags & kSegTwo, dup = nx.flags & kSegDup;
+        const int copies = two || dup ? 2 : 1;
+        const int node = nx.q0 + nx.row0 / p.G;
+        mbar_expect_tx(q_full, copies * C::kPanels * (dup ? half_rows : p.tile_rows) * 128);
+        for (int i = 0; i < copies; ++i)
+          for (int pn = 0; pn < C::kPanels; ++pn)
+            tma_load_3d(q_sa + (two ? i * C::kQ : i * 64 * 128) + pn * (kTcRows * 128), dup ? &qhalf : &qmap, q_full,
+                        pn * 64, nx.h * p.G, two ? node + i * tile_nodes : node);
+        ++q_loads;
+      };
+      bool have = take(0), late_q = false;
+      if (have) load_q();
+      while (ok && have) {
+        const int nt = nx.nt;
+        const bool two = nx.flags & kSegTwo, dup = nx.flags & kSegDup;
+        const int steps = two ? 2 * nt : nt;
+        if (late_q) {  // the last segment joined its groups in the second Q tile
+          ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+          if (!ok) break;
+          load_q();
+          late_q = false;
         }
-        if (ok && qk) ok = warp_wait(full(sk), (at_k / kNS) & 1, abort_flag, p.status);
-        if (ok && pv) ok = warp_wait(p_full(w), tiles[w]++ & 1, abort_flag, p.status);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
+        ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
+        for (int t = -2; ok && t < steps; ++t) {
+          const int w = t & 1;
+          const bool pv = t >= 0, qk = t + 2 < steps;
+          const uint32_t at_v = seq + v_pos(two ? t >> 1 : t, nt, two);
+          const uint32_t at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
+          const int sv = static_cast<int>(at_v % kNS), sk = static_cast<int>(at_k % kNS);
+          if (t == 0 && seg > 0) ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+          // usually all complete: one round of polls
+          const bool v_in = !pv || mbar_try_wait(full(sv), (at_v / kNS) & 1);
+          const bool k_in = !qk || mbar_try_wait(full(sk), (at_k / kNS) & 1);
+          const bool p_in = !pv || mbar_try_wait(p_full(w), tiles[w] & 1);
+          if (ok && !v_in) ok = thread_wait(full(sv), (at_v / kNS) & 1, abort_flag, p.status);
+          if (ok && !k_in) ok = thread_wait(full(sk), (at_k / kNS) & 1, abort_flag, p.status);
+          if (ok && !p_in) ok = thread_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
+          if (!ok) break;
+          if (pv) ++tiles[w];
+          tc_fence_after();
           if (pv) {
             const uint32_t v = ring + sv * C::kSlot;
 #pragma unroll
@@ -913,51 +1019,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
             mma_commit(s_full(w));
           }
-          if (t == steps - 1) {
-            mma_commit(o_full);
-            if (have) load_q();  // the last P is there, so every QK of this segment is done with Q
-          }
         }
-        __syncwarp();
+        if (!ok) break;
+        mma_commit(o_full);
+        seq += 2 * nt;
+        ++seg;
+        // the last P was there, so every QK of this segment is done with Q
+        have = take(seg);
+        if (have) {
+          late_q = dup && (nx.flags & kSegTwo);
+          if (!late_q) load_q();
+        }
       }
-      seq += 2 * nt;
-      ++seg;
+      if (*abort_flag) {
+        mma_commit(drained);
+        drain_wait(drained, 0);
+        if (q_loads) drain_wait(q_full, (q_loads - 1) & 1);
+      }
     }
-    if (!ok) {
-      if (lane == 0) mma_commit(drained);
-      drain_wait(drained, 0);
-      drain_wait(q_full, seg & 1);
-    }
-  } else if (warp >= 4) {
+    __syncwarp();
+  } else {
     // ----------------------------------------------------------- softmax --
     const int w = (warp - 4) >> 2;
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // this thread's row of the tile (its TMEM lane)
+    const int r = quarter * 32 + lane;  // this thread's TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + w * 128 + lane_off;
-    uint32_t seq = 0, seg = 0, cnt = 0, joined = 0;
+    const int node_a = r / p.G, head_a = r - node_a * p.G;                // of tile row r
+    const int node_b = (r & 63) / p.G, head_b = (r & 63) - node_b * p.G;  // of a doubled tile's
+    uint32_t seq = 0, cnt = 0, joined = 0;
     bool ok = true;
-    bool have = sg.next(p);
-    if (threadIdx.x == 128 && !(have && sg.tile0 > 0)) p.parts[blockIdx.x].c0 = -1;
-    while (ok && have) {
-      const int nt = sg.tile1 - sg.tile0;
-      const int n = sg.s.n, start = sg.s.start, ctx = start + n;
-      const bool two = sg.rows(p) > p.tile_rows;
+    Seg sg;
+    for (uint32_t seg = 0; ok && read_seg(seg, sg); ++seg) {
+      const int nt = sg.nt;
+      const int n = sg.n, start = sg.start, ctx = start + n;
+      const bool two = sg.flags & kSegTwo, dup = sg.flags & kSegDup;
       const int steps = two ? 2 * nt : nt;
-      const int lr = two ? w * p.tile_rows + r : r;  // row within the group
-      const int row = sg.row0 + lr;
-      const int rows = two ? min(p.tile_rows, sg.rows(p) - w * p.tile_rows) : sg.rows(p);
-      const bool row_on = r < rows;
-      const bool warp_on = quarter * 32 < rows;
-      const int node = row_on ? row / p.G : 0;
+      const int lr = two ? w * p.tile_rows + r : (dup ? r - 64 * w : r);  // row within the segment's
+      const int rows = two ? min(sg.rows, (w + 1) * p.tile_rows) : sg.rows;
+      const bool row_on = r < kTcRows && lr >= 0 && lr < rows && (!two || r < p.tile_rows);
+      const bool warp_on = __any_sync(0xffffffffu, row_on);
+      const int node = sg.row0 / p.G + (two ? w * tile_nodes : 0) + (row_on ? (dup ? node_b : node_a) : 0);
+      const int head = sg.h * p.G + (dup ? head_b : head_a);
       // one thread of a group gives back the ring slots that its steps were the last to read
       const bool gives = quarter == 0 && lane == 0 && (!two || w == 1);
       auto give = [&](uint32_t at) { mbar_arrive(empty(static_cast<int>(at % kNS))); };
       // s_odd of the next segment: last read two segments ago, next written after this segment's PVs
       if (threadIdx.x == 128) s_odd[(seg + 1) % 3] = 0;
-      const unsigned long long* mrow = p.mask + static_cast<long long>(sg.s.q0 + node) * p.words;
+      const unsigned long long* mrow = p.mask + static_cast<long long>(sg.q0 + (row_on ? node : 0)) * p.words;
       // a row of one mask word is fetched before it is needed
-      const bool in_tree = sg.tile1 * kTcKeys > start;
+      const bool in_tree = (sg.tile0 + nt) * kTcKeys > start;
       const unsigned long long mword = in_tree && row_on ? mrow[0] : 0ull;
       float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
       for (int t = w; t < steps; t += 2) {
@@ -1120,54 +1231,82 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       if (!ok) break;
       tc_fence_after();
       if (gives && w < steps) give(seq + v_pos(two ? nt - 1 : ((steps - 1 - w) & ~1) + w, nt, two));
-      const bool whole = sg.whole();
-      float m = m_ref, lt = l, a0 = 1.f, a1 = 0.f;
+      const bool whole = sg.flags & kSegWhole;
+      // one row tile: group w stores the columns [w D/2, (w + 1) D/2) of both
+      // groups' joined O (of one key tile: group 0 all of its own); two: its own
       const bool merge = !two && nt > 1;
+      const int col0 = merge ? w * (D / 2) : 0, cols = merge ? D / 2 : D;
+      const uint32_t t_own = tmem + 256 + (two || dup ? w * 128 : 0) + lane_off;
+      float m = m_ref, lt = l, a0 = 1.f, a1 = 0.f;  // a0: factor of the O at t_own, a1: of the other
+      // [2 groups][D / 8 chunks of 4 columns][64 rows]: what a group of a doubled tile hands to the other
+      float4* hand = reinterpret_cast<float4*>(gbase + C::kQ);
       if (merge) {
-        s_ml[w * 128 + r] = make_float2(m_ref, l);
+        const int mr = dup ? lr & 127 : r;
+        s_ml[w * 128 + mr] = make_float2(m_ref, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(ml_full);
         ok = warp_wait(ml_full, joined++ & 1, abort_flag, p.status);
         if (!ok) break;
-        const float2 ml0 = s_ml[r], ml1 = s_ml[128 + r];
+        const float2 ml0 = s_ml[mr], ml1 = s_ml[128 + mr];
         m = fmaxf(ml0.x, ml1.x);
         a0 = ex2_approx(ml0.x - m);
         a1 = ex2_approx(ml1.x - m);
         lt = ml0.y * a0 + ml1.y * a1;
+        if (dup && w == 1) a0 = a1;
       }
-      // one row tile: group w stores the columns [w D/2, (w + 1) D/2) of both
-      // groups' joined O (of one key tile: group 0 all of its own); two: its own
-      if (warp_on && (merge || two || w == 0)) {
-        if (whole) {
-          const float inv = lt == 0.f ? 0.f : 1.f / lt;
-          a0 *= inv;
-          a1 *= inv;
+      if (whole) {
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        a0 *= inv;
+        a1 *= inv;
+      }
+      if (merge && dup) {
+        // the groups' rows are in different TMEM lanes: the other group's half goes through shared memory
+        if (warp_on) {
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            float o[32];
+            tmem_ld32(t_own + (D / 2 - col0) + c * 32, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              hand[(w * (D / 8) + c * 8 + i) * 64 + (lr & 63)] =
+                  make_float4(o[4 * i] * a0, o[4 * i + 1] * a0, o[4 * i + 2] * a0, o[4 * i + 3] * a0);
+          }
         }
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + sg.slot()) * p.group_rows + lr;
-        if (threadIdx.x == 128 && sg.tile0 > 0) p.parts[blockIdx.x] = sg.part(p, s_share->per);
-        const int col0 = merge ? w * (D / 2) : 0, cols = merge ? D / 2 : D;
-        T* dst = static_cast<T*>(p.out) +
-                 (static_cast<long long>(sg.s.q0 + node) * p.Hq + sg.h * p.G + row % p.G) * D + col0;
-        float* pdst = p.part + pr * D + col0;
-        const uint32_t t_own = tmem + 256 + (two ? w * 128 : 0) + lane_off + col0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ml_full);
+        ok = warp_wait(ml_full, joined++ & 1, abort_flag, p.status);
+        if (!ok) break;
+      }
+      if (warp_on && (merge || two || w == 0)) {
+        T* dst = static_cast<T*>(p.out) + (static_cast<long long>(sg.q0 + node) * p.Hq + head) * D + col0;
+        const int slot = sg.tile0 > 0 ? 0 : 1;
 #pragma unroll 1
         for (int c = 0; c < cols / 32; ++c) {
           float o0[32], o1[32];
-          tmem_ld32_issue(t_own + c * 32, o0);
-          if (merge) tmem_ld32_issue(t_own + 128 + c * 32, o1);
+          tmem_ld32_issue(t_own + col0 + c * 32, o0);
+          if (merge && !dup) {
+            tmem_ld32_issue(t_own + col0 + 128 + c * 32, o1);
+          } else if (merge) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(o1 + 4 * i) = hand[((w ^ 1) * (D / 8) + c * 8 + i) * 64 + (lr & 63)];
+          }
           tmem_wait_ld();
           tmem_ready(o0);
-          if (merge) tmem_ready(o1);
+          if (merge && !dup) tmem_ready(o1);
+          const float f1 = dup ? 1.f : a1;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             o0[i] *= a0;
-            if (merge) o0[i] = fmaf(o1[i], a1, o0[i]);
+            if (merge) o0[i] = fmaf(o1[i], f1, o0[i]);
           }
           if (row_on) {
-            // a store of a warp touches 32 rows, one line each: the wider the better
+            // a store of a warp's 32 rows to out touches a line each: the wider the better
             if (!whole) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) st_global_32(pdst + c * 32 + i, reinterpret_cast<const uint32_t*>(o0 + i));
+              for (int i = 0; i < 4; ++i)
+                st_global_32(part_o(p, blockIdx.x, slot, lr, (col0 >> 3) + c * 4 + i, D),
+                             reinterpret_cast<const uint32_t*>(o0 + 8 * i));
             } else if (p.out32) {
 #pragma unroll
               for (int i = 0; i < 32; i += 16) {
@@ -1182,11 +1321,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             }
           }
         }
-        if (!whole && row_on && col0 == 0) *reinterpret_cast<float2*>(p.part_ml + pr * 2) = make_float2(m, lt);
+        if (!whole && row_on && col0 == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
         if (s_odd[seg % 3] != 0 && row_on) {
           // the cleared values, added to what this thread has stored for a row that sees them
           const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-          const int k1 = min(sg.tile1 * kTcKeys, ctx);
+          const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
 #pragma unroll 1
           for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
             const int jn = key - start;
@@ -1201,17 +1340,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               const T x = vr[i];
               if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
               if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
-              else pdst[i] += to_f32(x);
+              else part_o(p, blockIdx.x, slot, lr, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
             }
           }
         }
       }
+      if (dup) fence_proxy_async();  // the next user of `hand` may be a TMA load
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
       seq += 2 * nt;
-      ++seg;
-      have = sg.next(p);
     }
   }
   tc_fence_before();
@@ -1246,7 +1384,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
   const int unit = (c - pt.c0 - 1) * kJoinY + blockIdx.y;
   const int r_begin = pt.rows * unit / units, r_end = pt.rows * (unit + 1) / units;
   const bool deal = parts > kJoinWarps;  // deal a row's parts to the warps
-  auto base_of = [&](int k, int r) { return (static_cast<long long>(pt.c0 + k) * 2 + (k == 0)) * p.group_rows + r; };
   for (int r0 = r_begin; r0 < r_end; r0 += deal ? 1 : kJoinWarps) {
     const int r = deal ? r0 : r0 + warp;
     const bool on = r < r_end;
@@ -1272,9 +1409,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
         for (int j = 0; j < kAhead; ++j) {
           const int k = k0 + j * step;
           if (k < parts) {
-            const long long pr = base_of(k, r);
-            ml[j] = *reinterpret_cast<const float2*>(p.part_ml + pr * 2);
-            const float* src = p.part + pr * D + lane * DPL;
+            ml[j] = *part_ml(p, pt.c0 + k, k == 0, r);
+            const float* src = part_o(p, pt.c0 + k, k == 0, r, lane * DPL / 8, D) + lane * DPL % 8;
             if (DPL == 4) {
               *reinterpret_cast<float4*>(o[j]) = *reinterpret_cast<const float4*>(src);
             } else {
@@ -1382,13 +1518,18 @@ bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, long long rows
 
 template <typename T, int D>
 int launch_tc(TreeParams& p, cudaStream_t s) {
-  CUtensorMap qm, km, vm;
+  CUtensorMap qm, qh, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const long long rows = static_cast<long long>(p.num_blocks) * p.block_size;
   p.box_shift = 4;  // the largest power of two of keys that lie together in a block, at most a tile
   while (p.box_shift < 7 && p.block_size % (2 << p.box_shift) == 0) ++p.box_shift;
+  p.block_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.block_size == 1 << i) p.block_shift = i;
+  p.half_rows = 64 / p.G * p.G;
   p.out32 = ps_host::aligned(p.out, 32);
   if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
+      !make_rows_map(&qh, p.q, bf16, p.total_q, p.Hq, D, p.G, p.half_rows ? p.half_rows / p.G : 1) ||
       !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift) ||
       !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift)) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
@@ -1400,7 +1541,7 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
     ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
     return PS_ERR_CUDA;
   }
-  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, km, vm, p);
+  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, qh, km, vm, p);
   ps_host::count_launch();
   const int rc = ps_host::check_launch("tree_attention");
   return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
