@@ -733,6 +733,75 @@ PS_DEVICE void scale_p(uint32_t t_p, int n, float alpha) {
   tmem_wait_st();
 }
 
+// A row's 128 scores become P, 32 at a time (16-bit columns 16 c .. of P lie
+// below the scores still to be read), against the row's reference max m_ref; the
+// sum of P is returned. A row whose scores pass the reference by more than kSlack
+// takes their max, rounded up, as the new one: the factor for what was computed
+// against the old one is a power of two, so scaling is exact; `alpha` collects it
+// for O and the old sum, and the P columns already stored are scaled here.
+// Infinite or NaN scores make the reference NaN and with it the row, as the
+// formula does. TAIL: `vis` says which keys the row sees. The loop stays rolled
+// and its body short: longer bodies ran slower, from beyond the first-level
+// instruction cache (64 scores at a time: 440 us for the largest case against 395).
+template <typename T, bool TAIL>
+PS_DEVICE f32x2 softmax_tile(uint32_t t_s, const uint4& vis, bool row_on, float scale, float& m_ref, float& alpha) {
+  float sv[32];
+  f32x2 sum = 0;
+  tmem_ld32_issue(t_s, sv);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t vc = TAIL ? pick(vis, c) : 0u;
+    auto seen = [&](int i) { return !TAIL || ((vc >> i) & 1); };
+    tmem_wait_ld();
+    tmem_ready(sv);
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+      mx[(i >> 1) & 3] =
+          max3_nan(mx[(i >> 1) & 3], seen(i) ? sv[i] : -INFINITY, seen(i + 1) ? sv[i + 1] : -INFINITY);
+    const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
+    const bool moved = row_on && !(top <= m_ref + kSlack);
+    if (__any_sync(0xffffffffu, moved)) {
+      const float m_new = !moved ? m_ref : (top <= FLT_MAX ? ceilf(top) : NAN);
+      const float up = m_new - m_ref;
+      const float a = up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
+      if (__any_sync(0xffffffffu, c > 0 && moved && m_ref != -FLT_MAX)) scale_p<T>(t_s, c, a);
+      sum = mul2(sum, pack_f2(a, a));
+      alpha *= a;
+      m_ref = m_new;
+    }
+    const f32x2 scale2 = pack_f2(scale, scale), neg_m = pack_f2(-m_ref, -m_ref);
+    f32x2 x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fma2(pack_f2(sv[2 * i], sv[2 * i + 1]), scale2, neg_m);
+    if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv);  // under this group's exponentials
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float p0, p1;
+      if (i % 8 == 1 || i % 8 == 4 || i % 8 == 7) {
+        // 3 of 8 on the FMA pipe: the special-function unit's 16 results a clock would bound the step
+        unpack_f2(ex2_poly2(x[i]), p0, p1);
+      } else {
+        float x0, x1;
+        unpack_f2(x[i], x0, x1);
+        p0 = ex2_approx(x0);
+        p1 = ex2_approx(x1);
+      }
+      if (TAIL) {
+        p0 = seen(2 * i) ? p0 : 0.f;
+        p1 = seen(2 * i + 1) ? p1 : 0.f;
+      }
+      sum = add2(sum, pack_f2(p0, p1));
+      // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12 (f16) of a
+      // term, as the output's own rounding
+      pk[i] = pack2<T>(p0, p1);
+    }
+    tmem_st16(t_s + c * 16, pk);
+  }
+  return sum;
+}
+
 // After a wait gave up: let the copies or MMAs in flight end (bounded too).
 PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
   const long long t0 = clock64();
@@ -986,16 +1055,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           late_q = false;
         }
         ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
+        // ring positions of step t's V and step t + 2's K, and whether they are in:
+        // asked for between the two products of the step before, under its MMAs
+        uint32_t at_v, at_k;
+        int sv, sk;
+        bool v_in, k_in;
+        auto ask = [&](int t) {
+          at_v = seq + v_pos(two ? t >> 1 : t, nt, two);
+          at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
+          sv = static_cast<int>(at_v % kNS);
+          sk = static_cast<int>(at_k % kNS);
+          v_in = t < 0 || t >= steps || mbar_try_wait(full(sv), (at_v / kNS) & 1);
+          k_in = t + 2 >= steps || mbar_try_wait(full(sk), (at_k / kNS) & 1);
+        };
+        ask(-2);
         for (int t = -2; ok && t < steps; ++t) {
           const int w = t & 1;
           const bool pv = t >= 0, qk = t + 2 < steps;
-          const uint32_t at_v = seq + v_pos(two ? t >> 1 : t, nt, two);
-          const uint32_t at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
-          const int sv = static_cast<int>(at_v % kNS), sk = static_cast<int>(at_k % kNS);
           if (t == 0 && seg > 0) ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-          // usually all complete: one round of polls
-          const bool v_in = !pv || mbar_try_wait(full(sv), (at_v / kNS) & 1);
-          const bool k_in = !qk || mbar_try_wait(full(sk), (at_k / kNS) & 1);
           const bool p_in = !pv || mbar_try_wait(p_full(w), tiles[w] & 1);
           if (ok && !v_in) ok = thread_wait(full(sv), (at_v / kNS) & 1, abort_flag, p.status);
           if (ok && !k_in) ok = thread_wait(full(sk), (at_k / kNS) & 1, abort_flag, p.status);
@@ -1010,8 +1087,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
                      (t > 1 || kk > 0) ? 1u : 0u);
           }
+          const uint32_t k = ring + sk * C::kSlot;
+          ask(t + 1);
           if (qk) {
-            const uint32_t q = q_sa + (two ? w * C::kQ : 0), k = ring + sk * C::kSlot;
+            const uint32_t q = q_sa + (two ? w * C::kQ : 0);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
@@ -1111,115 +1190,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         tc_fence_after();
         if (warp_on) {
           const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
-          float sv[32];
-          f32x2 sum = 0;
-          // the loops over 32-key groups stay rolled: unrolled, the kernel's code
-          // (168 KB) ran from beyond the instruction caches
-          if (tail || t < 2) {
-            // a group's first tile, and tiles with masked keys: the max, then the
-            // exponentials, in two passes over the scores
-            const uint4 vis = tail ? seen128(row_on, p.words == 1 ? &mword : mrow, p.words, key0 - start, n)
-                                   : make_uint4(~0u, ~0u, ~0u, ~0u);
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              tmem_ld32_issue(t_s + c * 32, sv);
-              const uint32_t vc = pick(vis, c);
-              tmem_wait_ld();
-              tmem_ready(sv);
-#pragma unroll
-              for (int i = 0; i < 32; i += 2)
-                mx = max3_nan(mx, (vc >> i) & 1 ? sv[i] : -INFINITY, (vc >> (i + 1)) & 1 ? sv[i + 1] : -INFINITY);
-            }
-            mx *= p.scale_log2;
-            float alpha = 1.f;
-            const bool moved = row_on && !(mx <= m_ref + kSlack);
-            if (moved) {
-              // an infinite or NaN score makes the row NaN, as the formula does
-              if (!(mx <= FLT_MAX)) mx = NAN;
-              alpha = m_ref == -FLT_MAX ? 0.f : ex2_approx(m_ref - mx);
-              m_ref = mx;
-            }
-            if (t >= 2 && __any_sync(0xffffffffu, moved)) scale_o<D>(t_o, alpha);
-            l *= alpha;
-            // P's 16-bit columns c * 16 .. lie below the scores still to be read
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              tmem_ld32_issue(t_s + c * 32, sv);
-              const uint32_t vc = pick(vis, c);
-              tmem_wait_ld();
-              tmem_ready(sv);
-              uint32_t pk[16];
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float p0 = ex2_approx((vc >> i) & 1 ? fmaf(sv[i], p.scale_log2, -m_ref) : -INFINITY);
-                const float p1 = ex2_approx((vc >> (i + 1)) & 1 ? fmaf(sv[i + 1], p.scale_log2, -m_ref) : -INFINITY);
-                sum = add2(sum, pack_f2(p0, p1));
-                // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12
-                // (f16) of a term, as the output's own rounding
-                pk[i / 2] = pack2<T>(p0, p1);
-              }
-              tmem_st16(t_s + c * 16, pk);
-            }
-          } else {
-            // one pass against the max so far: a row whose scores have grown by
-            // more than 2^kSlack since (rare) rescales O, the sum and the P
-            // columns already stored by an exact power of two
-            const f32x2 scale2 = pack_f2(p.scale_log2, p.scale_log2);
-            tmem_ld32_issue(t_s, sv);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              tmem_wait_ld();
-              tmem_ready(sv);
-              f32x2 x[16];
-              const f32x2 neg_m = pack_f2(-m_ref, -m_ref);
-              float mx = -INFINITY, my = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                x[i] = fma2(pack_f2(sv[2 * i], sv[2 * i + 1]), scale2, neg_m);
-                float x0, x1;
-                unpack_f2(x[i], x0, x1);
-                if (i & 1) mx = max3_nan(mx, x0, x1);
-                else my = max3_nan(my, x0, x1);
-              }
-              if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv);  // under this group's exponentials
-              mx = max3_nan(mx, my, my);
-              const bool moved = row_on && !(mx <= kSlack);
-              if (__any_sync(0xffffffffu, moved)) {
-                const float up = !moved ? 0.f : (mx <= FLT_MAX ? ceilf(mx) : NAN);
-                const float alpha =
-                    up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
-                scale_o<D>(t_o, alpha);
-                scale_p<T>(t_s, c, alpha);
-                l *= alpha;
-                sum = mul2(sum, pack_f2(alpha, alpha));
-                m_ref += up;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = add2(x[i], pack_f2(-up, -up));
-              }
-              uint32_t pk[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float p0, p1;
-                if (i % 8 == 1 || i % 8 == 4 || i % 8 == 7) {
-                  // 3 of 8 on the FMA pipe: the special-function unit's 16
-                  // results a clock would bound the tile
-                  unpack_f2(ex2_poly2(x[i]), p0, p1);
-                } else {
-                  float x0, x1;
-                  unpack_f2(x[i], x0, x1);
-                  p0 = ex2_approx(x0);
-                  p1 = ex2_approx(x1);
-                }
-                sum = add2(sum, pack_f2(p0, p1));
-                pk[i] = pack2<T>(p0, p1);
-              }
-              tmem_st16(t_s + c * 16, pk);
-            }
-          }
+          float alpha = 1.f;  // what O and the old sum have to be scaled by
+          f32x2 sum;
+          if (tail)
+            sum = softmax_tile<T, true>(t_s, seen128(row_on, p.words == 1 ? &mword : mrow, p.words, key0 - start, n),
+                                        row_on, p.scale_log2, m_ref, alpha);
+          else
+            sum = softmax_tile<T, false>(t_s, make_uint4(0, 0, 0, 0), row_on, p.scale_log2, m_ref, alpha);
+          if (t >= 2 && __any_sync(0xffffffffu, alpha != 1.f)) scale_o<D>(t_o, alpha);
           float s0, s1;
           unpack_f2(sum, s0, s1);
-          l += s0 + s1;
+          l = l * alpha + (s0 + s1);
           tmem_wait_st();
         }
         tc_fence_before();
