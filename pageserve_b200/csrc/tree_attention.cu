@@ -62,7 +62,6 @@ struct TreeParams {
   int tile_rows;   // query rows per tile
   int group_rows;  // query rows per work item: one tile or two
   uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
-  int half_rows;   // rows of a Q tile that holds each row twice
   int box_shift;   // log2 of the keys per TMA box
   int block_shift; // log2 of the block size, or -1
   int out32;       // out is 32-byte aligned
@@ -264,14 +263,6 @@ PS_DEVICE unsigned long long seen64(const unsigned long long* row, int words, in
   if (keep < 64) v &= (1ull << keep) - 1;
   return v;
 }
-
-// Bits of the 128 keys from tree index `off` on; none for a row that is not used.
-PS_DEVICE uint4 seen128(bool on, const unsigned long long* row, int words, int off, int n) {
-  const unsigned long long a = on ? seen64(row, words, off, n) : 0ull, b = on ? seen64(row, words, off + 64, n) : 0ull;
-  return make_uint4(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
-                    static_cast<uint32_t>(b >> 32));
-}
-PS_DEVICE uint32_t pick(const uint4& v, int c) { return c < 2 ? (c ? v.y : v.x) : (c == 2 ? v.z : v.w); }
 
 template <typename T>
 PS_DEVICE bool finite16(uint16_t x) {
@@ -569,23 +560,21 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 //              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
 //              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major), all
 //              by one thread
-//   warps 4-11 two softmax groups of 4 warps, one row per thread, each with its
-//              own S, O, max and sum. Of one row tile (up to 128 rows) group w
-//              takes the key tiles w, w + 2, ... and the two states are joined at
-//              the end of the row tile, each group storing half of the columns;
-//              of two row tiles group w takes tile w, and every key tile is
-//              loaded once for both. Of at most 64 rows the Q tile holds each row
-//              twice and group 1 works on the upper copies: a softmax step is
-//              bound by its SM sub-partition (TMEM lanes are fixed to warps), and
-//              this puts the groups on different ones
-// One group's exponentials run under the other's MMAs: step t (a key tile of
-// group t & 1) is QK(t), softmax, PV(t), and the MMA warp issues PV(t) QK(t + 2)
-// together, with one commit: what a commit costs the pipe is about one MMA, so
-// ring slots are given back by the softmax groups, for which S(t) complete says
-// that K of step t and V of step t - 2 have been read (MMAs complete in order).
-// A softmax thread reads its scores from TMEM 32 at a time: holding 128 would
+//   warps 4-11 softmax, two threads per row: warps 4-7 the first 64 keys of a
+//              tile, warps 8-11 the others; a pair of warps exchanges its rows'
+//              maxima, so that both halves of P refer to the same one
+// Step t is a key tile (of one row tile, up to 128 rows) or a key tile and one of
+// two row tiles in turn, which then share every loaded tile: QK(t), softmax(t),
+// PV(t). The MMA thread issues PV(t) QK(t + 2) under softmax(t + 1), with one
+// commit: what a commit costs the pipe is about one MMA, so ring slots are given
+// back by a softmax thread, for which S(t) complete says that K of step t and V of
+// step t - 2 have been read (MMAs complete in order). With two groups of warps on
+// alternate steps instead, each step's softmax (1900 clocks, bound by latency)
+// and MMAs (1460) followed one another: 2500 clocks a step.
+// A softmax thread reads its scores from TMEM 32 at a time: holding them would
 // need more than the 168 registers that 12 warps leave a thread.
-// TMEM: S0 | S1 | O0 | O1, 128 columns each; P_w overwrites S_w.
+// TMEM: S0 | S1 | O0 | O1 (the second row tile's), 128 columns each; the halves
+// of P overwrite the first 32 columns of the halves of S.
 // The ring and the barriers run on over the segments of a CTA's share: the next
 // segment's tiles load while the last one's output is stored.
 constexpr int kTcRows = 128;
@@ -696,13 +685,13 @@ PS_DEVICE f32x2 ex2_poly2(f32x2 x) {
                  __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
 }
 // The max that P, O and the sum refer to stays until a row's scores pass it by
-// 2^kSlack: P <= 2^8 is well inside the 16-bit types.
+// more than kSlack (log2): P <= 2^8 is well inside the 16-bit types. The new one
+// is rounded up, so that O and the sum are scaled by a power of two, exactly.
 constexpr float kSlack = 8.f;
-// This thread's O row times alpha.
-template <int D>
-PS_DEVICE void scale_o(uint32_t t_o, float alpha) {
+// n x 32 columns of this thread's O row times alpha.
+PS_DEVICE void scale_o(uint32_t t_o, int n, float alpha) {
 #pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < n; ++c) {
     float v[32];
     tmem_ld32(t_o + c * 32, v);
 #pragma unroll
@@ -712,69 +701,45 @@ PS_DEVICE void scale_o(uint32_t t_o, float alpha) {
   }
   tmem_wait_st();
 }
-// The first n 16-column groups of this thread's P row times alpha (a power of
-// two: exact).
-template <typename T>
-PS_DEVICE void scale_p(uint32_t t_p, int n, float alpha) {
-  tmem_wait_st();
-#pragma unroll 1
-  for (int c = 0; c < n; ++c) {
-    float v[16];
-    tmem_ld16(t_p + c * 16, v);
-    uint32_t u[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t in = __float_as_uint(v[i]);
-      const T* h = reinterpret_cast<const T*>(&in);
-      u[i] = pack2<T>(to_f32(h[0]) * alpha, to_f32(h[1]) * alpha);
-    }
-    tmem_st16(t_p + c * 16, u);
-  }
-  tmem_wait_st();
-}
 
-// A row's 128 scores become P, 32 at a time (16-bit columns 16 c .. of P lie
-// below the scores still to be read), against the row's reference max m_ref; the
-// sum of P is returned. A row whose scores pass the reference by more than kSlack
-// takes their max, rounded up, as the new one: the factor for what was computed
-// against the old one is a power of two, so scaling is exact; `alpha` collects it
-// for O and the old sum, and the P columns already stored are scaled here.
-// Infinite or NaN scores make the reference NaN and with it the row, as the
-// formula does. TAIL: `vis` says which keys the row sees. The loop stays rolled
-// and its body short: longer bodies ran slower, from beyond the first-level
-// instruction cache (64 scores at a time: 440 us for the largest case against 395).
+// The largest of this thread's 64 scores (in the log2 domain; NaN if one is).
+// TAIL: bit i of v1:v0 says that the row sees key i.
+template <bool TAIL>
+PS_DEVICE float top_score(uint32_t t_s, uint32_t v0, uint32_t v1, float scale) {
+  float sv[64];
+  tmem_ld32_issue(t_s, sv);
+  tmem_ld32_issue(t_s + 32, sv + 32);
+  tmem_wait_ld();
+  tmem_ready(sv);
+  tmem_ready(sv + 32);
+  auto seen = [&](int i) { return !TAIL || (((i < 32 ? v0 : v1) >> (i & 31)) & 1); };
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 64; i += 2)
+    mx[(i >> 1) & 3] =
+        max3_nan(mx[(i >> 1) & 3], seen(i) ? sv[i] : -INFINITY, seen(i + 1) ? sv[i + 1] : -INFINITY);
+  return max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
+}
+// This thread's 64 scores become P against the row's reference max, 32 at a time
+// (16-bit columns 16 c .. lie below the scores still to be read); returns the sum
+// of P. The loop stays rolled: longer bodies ran slower, from beyond the
+// first-level instruction cache.
 template <typename T, bool TAIL>
-PS_DEVICE f32x2 softmax_tile(uint32_t t_s, const uint4& vis, bool row_on, float scale, float& m_ref, float& alpha) {
+PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale, float m_ref) {
   float sv[32];
   f32x2 sum = 0;
+  const f32x2 scale2 = pack_f2(scale, scale), neg_m = pack_f2(-m_ref, -m_ref);
   tmem_ld32_issue(t_s, sv);
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    const uint32_t vc = TAIL ? pick(vis, c) : 0u;
+  for (int c = 0; c < 2; ++c) {
+    const uint32_t vc = c ? v1 : v0;
     auto seen = [&](int i) { return !TAIL || ((vc >> i) & 1); };
     tmem_wait_ld();
     tmem_ready(sv);
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 32; i += 2)
-      mx[(i >> 1) & 3] =
-          max3_nan(mx[(i >> 1) & 3], seen(i) ? sv[i] : -INFINITY, seen(i + 1) ? sv[i + 1] : -INFINITY);
-    const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
-    const bool moved = row_on && !(top <= m_ref + kSlack);
-    if (__any_sync(0xffffffffu, moved)) {
-      const float m_new = !moved ? m_ref : (top <= FLT_MAX ? ceilf(top) : NAN);
-      const float up = m_new - m_ref;
-      const float a = up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
-      if (__any_sync(0xffffffffu, c > 0 && moved && m_ref != -FLT_MAX)) scale_p<T>(t_s, c, a);
-      sum = mul2(sum, pack_f2(a, a));
-      alpha *= a;
-      m_ref = m_new;
-    }
-    const f32x2 scale2 = pack_f2(scale, scale), neg_m = pack_f2(-m_ref, -m_ref);
     f32x2 x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = fma2(pack_f2(sv[2 * i], sv[2 * i + 1]), scale2, neg_m);
-    if (c < 3) tmem_ld32_issue(t_s + (c + 1) * 32, sv);  // under this group's exponentials
+    if (c == 0) tmem_ld32_issue(t_s + 32, sv);  // under this group's exponentials
     uint32_t pk[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -799,7 +764,9 @@ PS_DEVICE f32x2 softmax_tile(uint32_t t_s, const uint4& vis, bool row_on, float 
     }
     tmem_st16(t_s + c * 16, pk);
   }
-  return sum;
+  float s0, s1;
+  unpack_f2(sum, s0, s1);
+  return s0 + s1;
 }
 
 // After a wait gave up: let the copies or MMAs in flight end (bounded too).
@@ -819,7 +786,7 @@ struct Seg {
   int b, q0, n, start, h, row0, rows, tile0, nt;
   int flags;
 };
-enum SegFlags : int { kSegStop = 1, kSegWhole = 2, kSegTwo = 4, kSegDup = 8 };
+enum SegFlags : int { kSegStop = 1, kSegWhole = 2, kSegTwo = 4 };
 constexpr int kSegRing = 4;
 constexpr int kSegReaders = 11;  // two producers, the MMA thread, eight softmax warps
 
@@ -840,7 +807,6 @@ PS_DEVICE bool thread_wait(uint32_t bar, uint32_t parity, volatile int* abort_fl
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap qmap,
-                                                                const __grid_constant__ CUtensorMap qhalf,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
                                                                 const TreeParams p) {
@@ -863,14 +829,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   auto s_full = [&](int w) { return bars + 8 * (2 * kNS + w); };
   auto p_full = [&](int w) { return bars + 8 * (2 * kNS + 2 + w); };
   const uint32_t q_full = bars + 8 * (2 * kNS + 4);
-  const uint32_t o_full = bars + 8 * (2 * kNS + 5);
-  const uint32_t o_free = bars + 8 * (2 * kNS + 6);
-  const uint32_t ml_full = bars + 8 * (2 * kNS + 7);
-  const uint32_t drained = bars + 8 * (2 * kNS + 8);
-  auto seg_full = [&](int i) { return bars + 8 * (2 * kNS + 9 + i); };
-  auto seg_empty = [&](int i) { return bars + 8 * (2 * kNS + 9 + kSegRing + i); };
-  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 10 + 2 * kSegRing);
-  float2* s_ml = reinterpret_cast<float2*>(misc);  // [2 groups][128 rows]
+  const uint32_t o_free = bars + 8 * (2 * kNS + 5);
+  const uint32_t drained = bars + 8 * (2 * kNS + 6);
+  auto pair = [&](int quarter) { return bars + 8 * (2 * kNS + 7 + quarter); };
+  auto seg_full = [&](int i) { return bars + 8 * (2 * kNS + 11 + i); };
+  auto seg_empty = [&](int i) { return bars + 8 * (2 * kNS + 11 + kSegRing + i); };
+  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 12 + 2 * kSegRing);
+  float* s_swap = reinterpret_cast<float*>(misc);  // [2][2 halves][128 rows]
   Seg* s_seg = reinterpret_cast<Seg*>(misc + 2 * 128 * 8);  // [kSegRing]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_seg + kSegRing);
   volatile int* s_odd = abort_flag + 1;  // [3], by segment mod 3
@@ -892,12 +857,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full(w), 1);
-      mbar_init(p_full(w), 4);
+      mbar_init(p_full(w), 8);
     }
     mbar_init(q_full, 1);
-    mbar_init(o_full, 1);
     mbar_init(o_free, 8);
-    mbar_init(ml_full, 8);
+    for (int i = 0; i < 4; ++i) mbar_init(pair(i), 2);
     mbar_init(drained, 1);
     for (int i = 0; i < kSegRing; ++i) {
       mbar_init(seg_full(i), 1);
@@ -908,7 +872,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qhalf)) : "memory");
   }
   Share<kTcKeys> share;
   if (warp == 2) share.find(p, lane);
@@ -916,7 +879,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int tile_nodes = p.tile_rows / p.G, half_rows = p.half_rows;
+  const int tile_nodes = p.tile_rows / p.G;
 
   // segment i for a reading warp; false: there is none, or a wait gave up
   auto read_seg = [&](uint32_t i, Seg& sg) {
@@ -942,7 +905,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           sg = Seg{c.b, c.q0, c.n, c.start, c.h, c.row0, c.rows, c.tile0, c.nt, 0};
           if (c.whole) sg.flags |= kSegWhole;
           if (c.rows > p.tile_rows) sg.flags |= kSegTwo;
-          else if (c.rows <= half_rows && c.nt > 1) sg.flags |= kSegDup;
           if (c.tile0 > 0) p.parts[blockIdx.x] = share.part(c);
         }
         s_seg[i % kSegRing] = sg;
@@ -1032,28 +994,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         return !(nx.flags & kSegStop);
       };
       auto load_q = [&] {  // of nx
-        const bool two = nx.flags & kSegTwo, dup = nx.flags & kSegDup;
-        const int copies = two || dup ? 2 : 1;
+        const int copies = nx.flags & kSegTwo ? 2 : 1;
         const int node = nx.q0 + nx.row0 / p.G;
-        mbar_expect_tx(q_full, copies * C::kPanels * (dup ? half_rows : p.tile_rows) * 128);
+        mbar_expect_tx(q_full, copies * C::kPanels * p.tile_rows * 128);
         for (int i = 0; i < copies; ++i)
           for (int pn = 0; pn < C::kPanels; ++pn)
-            tma_load_3d(q_sa + (two ? i * C::kQ : i * 64 * 128) + pn * (kTcRows * 128), dup ? &qhalf : &qmap, q_full,
-                        pn * 64, nx.h * p.G, two ? node + i * tile_nodes : node);
+            tma_load_3d(q_sa + i * C::kQ + pn * (kTcRows * 128), &qmap, q_full, pn * 64, nx.h * p.G,
+                        node + i * tile_nodes);
         ++q_loads;
       };
-      bool have = take(0), late_q = false;
+      bool have = take(0);
       if (have) load_q();
       while (ok && have) {
         const int nt = nx.nt;
-        const bool two = nx.flags & kSegTwo, dup = nx.flags & kSegDup;
+        const bool two = nx.flags & kSegTwo;
         const int steps = two ? 2 * nt : nt;
-        if (late_q) {  // the last segment joined its groups in the second Q tile
-          ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-          if (!ok) break;
-          load_q();
-          late_q = false;
-        }
         ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
         // ring positions of step t's V and step t + 2's K, and whether they are in:
         // asked for between the two products of the step before, under its MMAs
@@ -1081,11 +1036,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           if (pv) ++tiles[w];
           tc_fence_after();
           if (pv) {
-            const uint32_t v = ring + sv * C::kSlot;
+            const uint32_t v = ring + sv * C::kSlot, o = tmem + 256 + (two ? w * 128 : 0);
+            const bool first = t < (two ? 2 : 1);
 #pragma unroll
             for (int kk = 0; kk < kTcKeys / 16; ++kk)
-              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
-                     (t > 1 || kk > 0) ? 1u : 0u);
+              mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
+                     (!first || kk > 0) ? 1u : 0u);
           }
           const uint32_t k = ring + sk * C::kSlot;
           ask(t + 1);
@@ -1096,19 +1052,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
               mma_f16(tmem + w * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), id_qk, kk > 0 ? 1u : 0u);
             }
-            mma_commit(s_full(w));
           }
+          mma_commit(s_full(w));  // S(t + 2), and in any case: PV(t) is done
         }
         if (!ok) break;
-        mma_commit(o_full);
         seq += 2 * nt;
         ++seg;
         // the last P was there, so every QK of this segment is done with Q
         have = take(seg);
-        if (have) {
-          late_q = dup && (nx.flags & kSegTwo);
-          if (!late_q) load_q();
-        }
+        if (have) load_q();
       }
       if (*abort_flag) {
         mma_commit(drained);
@@ -1119,49 +1071,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax --
-    const int w = (warp - 4) >> 2;
+    const int half = (warp - 4) >> 2;   // which 64 keys of a tile
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // this thread's TMEM lane
+    const int r = quarter * 32 + lane;  // this thread's row of a tile (its TMEM lane)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + w * 128 + lane_off;
-    const int node_a = r / p.G, head_a = r - node_a * p.G;                // of tile row r
-    const int node_b = (r & 63) / p.G, head_b = (r & 63) - node_b * p.G;  // of a doubled tile's
-    uint32_t seq = 0, cnt = 0, joined = 0;
+    const int r_node = r / p.G, r_head = r - r_node * p.G;
+    const bool gives = threadIdx.x == 128;  // gives back the ring slots
+    uint32_t seq = 0, swaps = 0;
+    uint32_t phase[2] = {0, 0};  // completed S waits of each buffer before this segment
     bool ok = true;
+    // the value of this row's other thread; both warps of a pair make the same calls
+    auto swap = [&](float v) {
+      float* at = s_swap + (swaps & 1) * 256;
+      at[half * 128 + r] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair(quarter));
+      ok = ok && warp_wait(pair(quarter), swaps & 1, abort_flag, p.status);
+      ++swaps;
+      return at[(half ^ 1) * 128 + r];
+    };
     Seg sg;
     for (uint32_t seg = 0; ok && read_seg(seg, sg); ++seg) {
       const int nt = sg.nt;
       const int n = sg.n, start = sg.start, ctx = start + n;
-      const bool two = sg.flags & kSegTwo, dup = sg.flags & kSegDup;
+      const bool two = sg.flags & kSegTwo;
       const int steps = two ? 2 * nt : nt;
-      const int lr = two ? w * p.tile_rows + r : (dup ? r - 64 * w : r);  // row within the segment's
-      const int rows = two ? min(sg.rows, (w + 1) * p.tile_rows) : sg.rows;
-      const bool row_on = r < kTcRows && lr >= 0 && lr < rows && (!two || r < p.tile_rows);
-      const bool warp_on = __any_sync(0xffffffffu, row_on);
-      const int node = sg.row0 / p.G + (two ? w * tile_nodes : 0) + (row_on ? (dup ? node_b : node_a) : 0);
-      const int head = sg.h * p.G + (dup ? head_b : head_a);
-      // one thread of a group gives back the ring slots that its steps were the last to read
-      const bool gives = quarter == 0 && lane == 0 && (!two || w == 1);
+      const int node0 = sg.row0 / p.G + r_node;  // of the first row tile
+      const int rows0 = min(sg.rows, p.tile_rows), rows1 = sg.rows - rows0;
       auto give = [&](uint32_t at) { mbar_arrive(empty(static_cast<int>(at % kNS))); };
+      // S(x) complete (x < steps + 2; from steps on: PV(x - 2) alone)
+      auto wait_s = [&](int x) {
+        return warp_wait(s_full(x & 1), (phase[x & 1] + (x >> 1)) & 1, abort_flag, p.status);
+      };
+      auto give_of = [&](int x) {  // what S(x) says has been read
+        if (!gives || (two && !(x & 1))) return;
+        const int j = two ? x >> 1 : x, back = two ? 1 : 2;
+        if (x < steps) give(seq + k_pos(j, two));
+        if (j >= back) give(seq + v_pos(j - back, nt, two));
+      };
       // s_odd of the next segment: last read two segments ago, next written after this segment's PVs
-      if (threadIdx.x == 128) s_odd[(seg + 1) % 3] = 0;
-      const unsigned long long* mrow = p.mask + static_cast<long long>(sg.q0 + (row_on ? node : 0)) * p.words;
+      if (gives) s_odd[(seg + 1) % 3] = 0;
       // a row of one mask word is fetched before it is needed
       const bool in_tree = (sg.tile0 + nt) * kTcKeys > start;
-      const unsigned long long mword = in_tree && row_on ? mrow[0] : 0ull;
-      float m_ref = -FLT_MAX, l = 0.f;  // m_ref: the max that P and O refer to, in the log2 domain
-      for (int t = w; t < steps; t += 2) {
+      auto mask_row = [&](int node) { return p.mask + static_cast<long long>(sg.q0 + node) * p.words; };
+      unsigned long long mword = in_tree && r < rows0 ? mask_row(node0)[0] : 0ull;
+      unsigned long long mword_b = in_tree && r < rows1 ? mask_row(node0 + tile_nodes)[0] : 0ull;
+      // the reference max (log2 domain) and the sum of the row of the step's tile; _b: the other tile's
+      float m_ref = -FLT_MAX, l = 0.f, m_b = -FLT_MAX, l_b = 0.f;
+      for (int t = 0; t < steps; ++t) {
+        const int w = t & 1, tile = two ? w : 0;
         const int j = two ? t >> 1 : t;
         const int key0 = (sg.tile0 + j) * kTcKeys;
         const bool tail = key0 + kTcKeys > start;
-        ok = warp_wait(s_full(w), cnt & 1, abort_flag, p.status);
+        const bool row_on = r < (tile ? rows1 : rows0);
+        ok = wait_s(t);
         if (!ok) break;
-        ++cnt;
-        if (gives) {
-          give(seq + k_pos(j, two));
-          if (t >= 2) give(seq + v_pos(two ? j - 1 : j - 2, nt, two));
-        }
-        if (tail && (!two || w == 0)) {
+        give_of(t);
+        if (tail && tile == 0) {
           // V rows past the context hold anything, and a drafted row's values
           // that are not finite would reach rows that do not see it: clear them.
           // (S(t) is there, so the slot's last tile has been read and the wait
@@ -1174,10 +1140,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           if (key >= start) {
             bool bad = false;
             unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + r * 128;
+            constexpr int kChunks = 8 * C::kPanels / 2;  // 16-byte chunks for each of a row's threads
 #pragma unroll 1
-            for (int i = 0; i < 8 * C::kPanels; ++i) {
+            for (int k = 0; k < kChunks; ++k) {
               // the lanes' lines share their banks: each starts at another chunk
-              uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * (kTcKeys * 128) + (((i ^ r) & 7) << 4));
+              const int i = half * kChunks + ((k ^ r) & (kChunks < 8 ? kChunks - 1 : 7));
+              uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * (kTcKeys * 128) + ((i & 7) << 4));
               uint4 x = key < ctx ? *at16 : make_uint4(0, 0, 0, 0);
               const bool hit = clear_odd<T>(x);
               bad |= hit;
@@ -1188,145 +1156,135 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           fence_proxy_async();
         }
         tc_fence_after();
-        if (warp_on) {
-          const uint32_t t_o = tmem + 256 + w * 128 + lane_off;
-          float alpha = 1.f;  // what O and the old sum have to be scaled by
-          f32x2 sum;
-          if (tail)
-            sum = softmax_tile<T, true>(t_s, seen128(row_on, p.words == 1 ? &mword : mrow, p.words, key0 - start, n),
-                                        row_on, p.scale_log2, m_ref, alpha);
-          else
-            sum = softmax_tile<T, false>(t_s, make_uint4(0, 0, 0, 0), row_on, p.scale_log2, m_ref, alpha);
-          if (t >= 2 && __any_sync(0xffffffffu, alpha != 1.f)) scale_o<D>(t_o, alpha);
-          float s0, s1;
-          unpack_f2(sum, s0, s1);
-          l = l * alpha + (s0 + s1);
+        if (quarter * 32 < (tile ? rows1 : rows0)) {
+          const uint32_t t_s = tmem + w * 128 + half * 64 + lane_off;
+          uint32_t v0 = 0, v1 = 0;
+          if (tail) {
+            const int off = key0 + half * 64 - start;
+            const unsigned long long v =
+                !row_on ? 0ull
+                        : (p.words == 1 ? seen64(&mword, 1, off, n)
+                                        : seen64(mask_row(node0 + (tile ? tile_nodes : 0)), p.words, off, n));
+            v0 = static_cast<uint32_t>(v);
+            v1 = static_cast<uint32_t>(v >> 32);
+          }
+          float top = tail ? top_score<true>(t_s, v0, v1, p.scale_log2) : top_score<false>(t_s, 0, 0, p.scale_log2);
+          top = max3_nan(top, swap(top), -INFINITY);
+          if (!ok) break;
+          const bool moved = row_on && !(top <= m_ref + kSlack);
+          if (__any_sync(0xffffffffu, moved)) {
+            // infinite or NaN scores make the reference NaN and with it the row, as the formula does
+            const float m_new = !moved ? m_ref : (top <= FLT_MAX ? ceilf(top) : NAN);
+            const float up = m_new - m_ref;
+            const float a =
+                up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
+            l *= a;
+            m_ref = m_new;
+            if (t >= (two ? 2 : 1)) {
+              // of one row tile, PV(t - 1) may still be adding to O: S(t + 1) comes after it
+              if (!two) ok = wait_s(t + 1);
+              if (!ok) break;
+              tc_fence_after();
+              scale_o(tmem + 256 + tile * 128 + half * (D / 2) + lane_off, D / 64, a);
+            }
+          }
+          l += tail ? softmax_half<T, true>(t_s, v0, v1, p.scale_log2, m_ref)
+                    : softmax_half<T, false>(t_s, 0, 0, p.scale_log2, m_ref);
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(w));
+        if (two) {  // the next step is the other tile's
+          const float m = m_ref, ll = l;
+          const unsigned long long mw = mword;
+          m_ref = m_b;
+          l = l_b;
+          mword = mword_b;
+          m_b = m;
+          l_b = ll;
+          mword_b = mw;
+        }
       }
       if (!ok) break;
-      ok = warp_wait(o_full, seg & 1, abort_flag, p.status);
+      ok = wait_s(steps);
       if (!ok) break;
+      give_of(steps);
+      ok = wait_s(steps + 1);
+      if (!ok) break;
+      give_of(steps + 1);
+      phase[0] += (steps + 3) >> 1;
+      phase[1] += (steps + 2) >> 1;
       tc_fence_after();
-      if (gives && w < steps) give(seq + v_pos(two ? nt - 1 : ((steps - 1 - w) & ~1) + w, nt, two));
       const bool whole = sg.flags & kSegWhole;
-      // one row tile: group w stores the columns [w D/2, (w + 1) D/2) of both
-      // groups' joined O (of one key tile: group 0 all of its own); two: its own
-      const bool merge = !two && nt > 1;
-      const int col0 = merge ? w * (D / 2) : 0, cols = merge ? D / 2 : D;
-      const uint32_t t_own = tmem + 256 + (two || dup ? w * 128 : 0) + lane_off;
-      float m = m_ref, lt = l, a0 = 1.f, a1 = 0.f;  // a0: factor of the O at t_own, a1: of the other
-      // [2 groups][D / 8 chunks of 4 columns][64 rows]: what a group of a doubled tile hands to the other
-      float4* hand = reinterpret_cast<float4*>(gbase + C::kQ);
-      if (merge) {
-        const int mr = dup ? lr & 127 : r;
-        s_ml[w * 128 + mr] = make_float2(m_ref, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ml_full);
-        ok = warp_wait(ml_full, joined++ & 1, abort_flag, p.status);
-        if (!ok) break;
-        const float2 ml0 = s_ml[mr], ml1 = s_ml[128 + mr];
-        m = fmaxf(ml0.x, ml1.x);
-        a0 = ex2_approx(ml0.x - m);
-        a1 = ex2_approx(ml1.x - m);
-        lt = ml0.y * a0 + ml1.y * a1;
-        if (dup && w == 1) a0 = a1;
-      }
-      if (whole) {
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        a0 *= inv;
-        a1 *= inv;
-      }
-      if (merge && dup) {
-        // the groups' rows are in different TMEM lanes: the other group's half goes through shared memory
-        if (warp_on) {
+      const int slot = sg.tile0 > 0 ? 0 : 1;
+      for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
+        const int rows = tile ? rows1 : rows0;
+        if (quarter * 32 < rows) {  // this thread's half of its row's columns
+          const float m = tile ? m_b : m_ref;
+          float lt = tile ? l_b : l;
+          lt += swap(lt);
+          if (!ok) break;
+          const float f = !whole ? 1.f : (lt == 0.f ? 0.f : 1.f / lt);
+          const bool row_on = r < rows;
+          const int lr = tile * p.tile_rows + r, node = node0 + tile * tile_nodes;
+          const int col0 = half * (D / 2);
+          T* dst = static_cast<T*>(p.out) +
+                   (static_cast<long long>(sg.q0 + node) * p.Hq + sg.h * p.G + r_head) * D + col0;
 #pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
             float o[32];
-            tmem_ld32(t_own + (D / 2 - col0) + c * 32, o);
+            tmem_ld32(tmem + 256 + tile * 128 + lane_off + col0 + c * 32, o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              hand[(w * (D / 8) + c * 8 + i) * 64 + (lr & 63)] =
-                  make_float4(o[4 * i] * a0, o[4 * i + 1] * a0, o[4 * i + 2] * a0, o[4 * i + 3] * a0);
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ml_full);
-        ok = warp_wait(ml_full, joined++ & 1, abort_flag, p.status);
-        if (!ok) break;
-      }
-      if (warp_on && (merge || two || w == 0)) {
-        T* dst = static_cast<T*>(p.out) + (static_cast<long long>(sg.q0 + node) * p.Hq + head) * D + col0;
-        const int slot = sg.tile0 > 0 ? 0 : 1;
-#pragma unroll 1
-        for (int c = 0; c < cols / 32; ++c) {
-          float o0[32], o1[32];
-          tmem_ld32_issue(t_own + col0 + c * 32, o0);
-          if (merge && !dup) {
-            tmem_ld32_issue(t_own + col0 + 128 + c * 32, o1);
-          } else if (merge) {
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            if (row_on) {
+              // a store of a warp's 32 rows to out touches a line each: the wider the better
+              if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4*>(o1 + 4 * i) = hand[((w ^ 1) * (D / 8) + c * 8 + i) * 64 + (lr & 63)];
-          }
-          tmem_wait_ld();
-          tmem_ready(o0);
-          if (merge && !dup) tmem_ready(o1);
-          const float f1 = dup ? 1.f : a1;
+                for (int i = 0; i < 4; ++i)
+                  st_global_32(part_o(p, blockIdx.x, slot, lr, (col0 >> 3) + c * 4 + i, D),
+                               reinterpret_cast<const uint32_t*>(o + 8 * i));
+              } else if (p.out32) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            o0[i] *= a0;
-            if (merge) o0[i] = fmaf(o1[i], f1, o0[i]);
-          }
-          if (row_on) {
-            // a store of a warp's 32 rows to out touches a line each: the wider the better
-            if (!whole) {
+                for (int i = 0; i < 32; i += 16) {
+                  uint32_t v[8];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                st_global_32(part_o(p, blockIdx.x, slot, lr, (col0 >> 3) + c * 4 + i, D),
-                             reinterpret_cast<const uint32_t*>(o0 + 8 * i));
-            } else if (p.out32) {
+                  for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
+                  st_global_32(dst + c * 32 + i, v);
+                }
+              } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 16) {
-                uint32_t v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o0[i + 2 * e], o0[i + 2 * e + 1]);
-                st_global_32(dst + c * 32 + i, v);
+                for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o + i);
               }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o0 + i);
             }
           }
-        }
-        if (!whole && row_on && col0 == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
-        if (s_odd[seg % 3] != 0 && row_on) {
-          // the cleared values, added to what this thread has stored for a row that sees them
-          const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-          const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
+          if (!whole && row_on && half == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
+          if (s_odd[seg % 3] != 0 && row_on) {
+            // the cleared values, added to what this thread has stored for a row that sees them
+            const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
+            const unsigned long long* mrow = mask_row(node);
+            const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
 #pragma unroll 1
-          for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
-            const int jn = key - start;
-            if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
-            const int phys = table[key / p.block_size];
-            if (phys < 0 || phys >= p.num_blocks) continue;
-            const T* vr = static_cast<const T*>(p.v_cache) +
-                          ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
-                          col0;
+            for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
+              const int jn = key - start;
+              if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
+              const int phys = table[key / p.block_size];
+              if (phys < 0 || phys >= p.num_blocks) continue;
+              const T* vr = static_cast<const T*>(p.v_cache) +
+                            ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
+                            col0;
 #pragma unroll 1
-            for (int i = 0; i < cols; ++i) {
-              const T x = vr[i];
-              if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
-              if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
-              else part_o(p, blockIdx.x, slot, lr, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
+              for (int i = 0; i < D / 2; ++i) {
+                const T x = vr[i];
+                if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
+                if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
+                else part_o(p, blockIdx.x, slot, lr, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
+              }
             }
           }
         }
       }
-      if (dup) fence_proxy_async();  // the next user of `hand` may be a TMA load
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
@@ -1499,7 +1457,7 @@ bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, long long rows
 
 template <typename T, int D>
 int launch_tc(TreeParams& p, cudaStream_t s) {
-  CUtensorMap qm, qh, km, vm;
+  CUtensorMap qm, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const long long rows = static_cast<long long>(p.num_blocks) * p.block_size;
   p.box_shift = 4;  // the largest power of two of keys that lie together in a block, at most a tile
@@ -1507,10 +1465,8 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   p.block_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p.block_size == 1 << i) p.block_shift = i;
-  p.half_rows = 64 / p.G * p.G;
   p.out32 = ps_host::aligned(p.out, 32);
   if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
-      !make_rows_map(&qh, p.q, bf16, p.total_q, p.Hq, D, p.G, p.half_rows ? p.half_rows / p.G : 1) ||
       !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift) ||
       !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift)) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
@@ -1522,7 +1478,7 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
     ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
     return PS_ERR_CUDA;
   }
-  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, qh, km, vm, p);
+  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, km, vm, p);
   ps_host::count_launch();
   const int rc = ps_host::check_launch("tree_attention");
   return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
