@@ -59,6 +59,7 @@ struct TreeParams {
   int num_seqs;
   int num_ctas;
   int min_share;   // fewest key tiles worth a CTA
+  int never_cut;   // by the call's bounds no row group is cut: there is nothing to join
   int tile_rows;   // query rows per tile
   int group_rows;  // query rows per work item: one tile or two
   uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
@@ -114,42 +115,33 @@ struct Share {
   int quota, unit, per, b, pair, tile0;  // quota: row groups (unit 1) or key tiles (unit 0) left
   Seq s;
 
-  // By one whole warp. The first 256 sequences' lengths are loaded at once and
-  // kept in registers between the sums and the search: one round of latency.
-  PS_DEVICE void find(const TreeParams& p, int lane) {
-    constexpr int kKeep = 8;
-    int q0[kKeep], q1[kKeep], st[kKeep], pairs[kKeep], tiles[kKeep];
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-      const int b0 = min(i * 32 + lane, p.num_seqs - 1);
-      const bool on = i * 32 < p.num_seqs;  // warp-uniform
-      q0[i] = on ? p.cu_q[b0] : 0;
-      q1[i] = on ? p.cu_q[b0 + 1] : 0;
-      st[i] = on ? p.start_pos[b0] : 0;
-    }
+  // By one whole warp; `kept` is shared memory for the sequences' sizes between
+  // the sums and the search (of the first `room`; the others are read again).
+  PS_DEVICE void find(const TreeParams& p, int lane, Seq* kept, int room) {
     int total = 0, groups = 0, longest = 0;
     bool any_bad = false;
-    auto count = [&](const Seq& q, bool bad) {
-      groups += p.Hkv * q.row_groups;
-      total += q.items(p.Hkv);
-      longest = max(longest, q.key_tiles);
-      any_bad |= bad;
-    };
+#pragma unroll 1
+    for (int b0 = lane; b0 < p.num_seqs; b0 += 128) {  // the loads of 128 sequences are out at once
+      int q0[4], q1[4], st[4];
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-      pairs[i] = tiles[i] = 0;
-      if (i * 32 + lane < p.num_seqs) {
-        bool bad;
-        const Seq q = make_seq<KEYS>(p, q0[i], q1[i], st[i], &bad);
-        pairs[i] = p.Hkv * q.row_groups;
-        tiles[i] = q.key_tiles;
-        count(q, bad);
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(b0 + 32 * u, p.num_seqs - 1);
+        q0[u] = p.cu_q[i];
+        q1[u] = p.cu_q[i + 1];
+        st[u] = p.start_pos[i];
       }
-    }
-    for (int i = kKeep * 32 + lane; i < p.num_seqs; i += 32) {
-      bool bad;
-      const Seq q = make_seq<KEYS>(p, p.cu_q[i], p.cu_q[i + 1], p.start_pos[i], &bad);
-      count(q, bad);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = b0 + 32 * u;
+        if (i >= p.num_seqs) break;
+        bool bad;
+        const Seq q = make_seq<KEYS>(p, q0[u], q1[u], st[u], &bad);
+        if (i < room) kept[i] = q;
+        groups += p.Hkv * q.row_groups;
+        total += q.items(p.Hkv);
+        longest = max(longest, q.key_tiles);
+        any_bad |= bad;
+      }
     }
     if (any_bad && blockIdx.x == 0) record_error(p.status, kErrShape);
     total = __reduce_add_sync(0xffffffffu, total);
@@ -163,8 +155,14 @@ struct Share {
     const int begin = static_cast<int>(lo < all ? lo : all);
     quota = min(unit ? whole : per, all - begin);
     if (quota <= 0) return;
+    __syncwarp();
     int run = 0;
-    auto look = [&](int b0, int n) {  // the lane whose sequence holds `begin`, or -1
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
+      const int i = b0 + lane;
+      Seq q{};
+      if (i < p.num_seqs) q = i < room ? kept[i] : seq_of<KEYS>(p, i);
+      const int n = unit ? p.Hkv * q.row_groups : q.items(p.Hkv);
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -173,29 +171,18 @@ struct Share {
       }
       const int first = run + incl - n;
       const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && begin >= first && begin < first + n);
-      run += __shfl_sync(0xffffffffu, incl, 31);
-      if (!hit) return -1;
-      const int src = __ffs(hit) - 1;
-      b = b0 + src;
-      pair = begin - __shfl_sync(0xffffffffu, first, src);  // items for now
-      return src;
-    };
-    bool found = false, bad;
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-      if (!found && i * 32 < p.num_seqs) {
-        const int src = look(i * 32, unit ? pairs[i] : pairs[i] * tiles[i]);
-        if (src >= 0) {
-          found = true;
-          s = make_seq<KEYS>(p, __shfl_sync(0xffffffffu, q0[i], src), __shfl_sync(0xffffffffu, q1[i], src),
-                             __shfl_sync(0xffffffffu, st[i], src), &bad);
-        }
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        b = b0 + src;
+        pair = begin - __shfl_sync(0xffffffffu, first, src);  // items for now
+        s.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+        s.n = __shfl_sync(0xffffffffu, q.n, src);
+        s.start = __shfl_sync(0xffffffffu, q.start, src);
+        s.row_groups = __shfl_sync(0xffffffffu, q.row_groups, src);
+        s.key_tiles = __shfl_sync(0xffffffffu, q.key_tiles, src);
+        break;
       }
-    }
-    for (int b0 = kKeep * 32; !found && b0 < p.num_seqs; b0 += 32) {
-      const Seq q = seq_of<KEYS>(p, min(b0 + lane, p.num_seqs - 1));
-      found = look(b0, b0 + lane < p.num_seqs ? (unit ? p.Hkv * q.row_groups : q.items(p.Hkv)) : 0) >= 0;
-      if (found) s = seq_of<KEYS>(p, b);
+      run += __shfl_sync(0xffffffffu, incl, 31);
     }
     tile0 = 0;
     if (!unit) {
@@ -333,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     Share<kKeys> sh;
-    sh.find(p, lane);
+    sh.find(p, lane, reinterpret_cast<Seq*>(smem), kStages * 2 * kTile / static_cast<int>(sizeof(Seq)));
     if (lane == 0) {
       s_share = sh;
       p.parts[blockIdx.x].c0 = -1;
@@ -651,43 +638,19 @@ PS_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-PS_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 PS_DEVICE float max3_nan(float a, float b, float c) {  // NaN if one is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two values by 2^round(x) * q(x - round(x)), q the least relative error
-// polynomial of degree 5 for 2^r on [-1/2, 1/2] (fitted by iteratively
-// reweighted least squares): 2^-22, as ex2.approx. x is kept above -125 (2^-125
-// is nothing beside a sum of at least 2^-kSlack); NaN becomes 2^-125.
-PS_DEVICE f32x2 ex2_poly2(f32x2 x) {
-  float x0, x1;
-  unpack_f2(x, x0, x1);
-  x = pack_f2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-  const f32x2 big = pack_f2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are round(x)
-  const f32x2 t = add2(x, big);
-  const f32x2 r = fma2(add2(t, pack_f2(-12582912.f, -12582912.f)), pack_f2(-1.f, -1.f), x);
-  f32x2 q = pack_f2(0.00132764725f, 0.00132764725f);
-  q = fma2(q, r, pack_f2(0.00967554189f, 0.00967554189f));
-  q = fma2(q, r, pack_f2(0.0555071309f, 0.0555071309f));
-  q = fma2(q, r, pack_f2(0.240221202f, 0.240221202f));
-  q = fma2(q, r, pack_f2(0.693146944f, 0.693146944f));
-  q = fma2(q, r, pack_f2(1.00000012f, 1.00000012f));
-  float q0, q1, t0, t1;
-  unpack_f2(q, q0, q1);
-  unpack_f2(t, t0, t1);
-  return pack_f2(__uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23)),
-                 __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
-}
 // The max that P, O and the sum refer to stays until a row's scores pass it by
 // more than kSlack (log2): P <= 2^8 is well inside the 16-bit types. The new one
 // is rounded up, so that O and the sum are scaled by a power of two, exactly.
 constexpr float kSlack = 8.f;
+// 2^-up for a whole number up >= 0 (0 when it is tiny, NaN when up is).
+PS_DEVICE float pow2_down(float up) {
+  return up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
+}
 // n x 32 columns of this thread's O row times alpha.
 PS_DEVICE void scale_o(uint32_t t_o, int n, float alpha) {
 #pragma unroll 1
@@ -723,11 +686,13 @@ PS_DEVICE float top_score(uint32_t t_s, uint32_t v0, uint32_t v1, float scale) {
 // This thread's 64 scores become P against the row's reference max, 32 at a time
 // (16-bit columns 16 c .. lie below the scores still to be read); returns the sum
 // of P. The loop stays rolled: longer bodies ran slower, from beyond the
-// first-level instruction cache.
+// first-level instruction cache. (Taking 3 of 8 exponentials to the FMA pipe by a
+// polynomial was no faster: the loop is bound by latency and issue, not by the
+// special-function unit.)
 template <typename T, bool TAIL>
 PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale, float m_ref) {
   float sv[32];
-  f32x2 sum = 0;
+  f32x2 sum[4] = {0, 0, 0, 0};
   const f32x2 scale2 = pack_f2(scale, scale), neg_m = pack_f2(-m_ref, -m_ref);
   tmem_ld32_issue(t_s, sv);
 #pragma unroll 1
@@ -743,21 +708,14 @@ PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale
     uint32_t pk[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float p0, p1;
-      if (i % 8 == 1 || i % 8 == 4 || i % 8 == 7) {
-        // 3 of 8 on the FMA pipe: the special-function unit's 16 results a clock would bound the step
-        unpack_f2(ex2_poly2(x[i]), p0, p1);
-      } else {
-        float x0, x1;
-        unpack_f2(x[i], x0, x1);
-        p0 = ex2_approx(x0);
-        p1 = ex2_approx(x1);
-      }
+      float x0, x1;
+      unpack_f2(x[i], x0, x1);
+      float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
       if (TAIL) {
         p0 = seen(2 * i) ? p0 : 0.f;
         p1 = seen(2 * i + 1) ? p1 : 0.f;
       }
-      sum = add2(sum, pack_f2(p0, p1));
+      sum[i & 3] = add2(sum[i & 3], pack_f2(p0, p1));  // four chains: one would bound the loop by its latency
       // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12 (f16) of a
       // term, as the output's own rounding
       pk[i] = pack2<T>(p0, p1);
@@ -765,9 +723,27 @@ PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale
     tmem_st16(t_s + c * 16, pk);
   }
   float s0, s1;
-  unpack_f2(sum, s0, s1);
+  unpack_f2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
   return s0 + s1;
 }
+
+// A position of a ring of N slots: slot and phase parity.
+template <int N>
+struct Slot {
+  int i;
+  uint32_t phase;
+  PS_DEVICE void advance(int n) {
+    i += n;
+    if (i >= 2 * N) {  // n may be a segment's whole length
+      const int turns = i / N;
+      i -= turns * N;
+      phase ^= turns & 1;
+    } else if (i >= N) {
+      i -= N;
+      phase ^= 1;
+    }
+  }
+};
 
 // After a wait gave up: let the copies or MMAs in flight end (bounded too).
 PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
@@ -790,6 +766,17 @@ enum SegFlags : int { kSegStop = 1, kSegWhole = 2, kSegTwo = 4 };
 constexpr int kSegRing = 4;
 constexpr int kSegReaders = 11;  // two producers, the MMA thread, eight softmax warps
 
+PS_DEVICE uint32_t mbar_test(uint32_t bar, uint32_t parity) {  // a try_wait may suspend the thread, this does not
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 // Bounded wait of one thread (see warp_wait).
 PS_DEVICE bool thread_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -810,7 +797,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
                                                                 const TreeParams p) {
-  pdl_wait();
   pdl_trigger();
   using C = Tc<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -819,6 +805,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   const uint32_t q_sa = smem_u32(smem_raw);
   unsigned char* gbase = smem_raw;
   if (q_sa & 1023) {  // the swizzle needs the declared alignment
+    pdl_wait();
     if (threadIdx.x == 0) record_error(p.status, kErrShape);
     return;
   }
@@ -873,8 +860,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
   }
+  pdl_wait();  // barriers, TMEM and descriptors are ready before the kernel ahead ends
   Share<kTcKeys> share;
-  if (warp == 2) share.find(p, lane);
+  if (warp == 2) {
+    share.find(p, lane, reinterpret_cast<Seq*>(gbase + 2 * C::kQ), kNS * C::kSlot / static_cast<int>(sizeof(Seq)));
+    fence_proxy_async();  // the ring is TMA's from here on
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -983,7 +974,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     if (lane == 0) {
       constexpr uint32_t id_qk = instr_desc(kBf16, 128, kTcKeys);
       constexpr uint32_t id_pv = idesc_bmn(kBf16, 128, D);
-      uint32_t seq = 0, seg = 0, q_loads = 0;
+      uint32_t seg = 0, q_loads = 0;
+      Slot<kNS> base{0, 0};  // the segment's first ring position
       uint32_t tiles[2] = {0, 0};  // P tiles consumed of each group
       bool ok = true;
       Seg nx;
@@ -1010,53 +1002,57 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         const bool two = nx.flags & kSegTwo;
         const int steps = two ? 2 * nt : nt;
         ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
-        // ring positions of step t's V and step t + 2's K, and whether they are in:
-        // asked for between the two products of the step before, under its MMAs
-        uint32_t at_v, at_k;
-        int sv, sk;
-        bool v_in, k_in;
-        auto ask = [&](int t) {
-          at_v = seq + v_pos(two ? t >> 1 : t, nt, two);
-          at_k = seq + k_pos(two ? (t + 2) >> 1 : t + 2, two);
-          sv = static_cast<int>(at_v % kNS);
-          sk = static_cast<int>(at_k % kNS);
-          v_in = t < 0 || t >= steps || mbar_try_wait(full(sv), (at_v / kNS) & 1);
-          k_in = t + 2 >= steps || mbar_try_wait(full(sk), (at_k / kNS) & 1);
+        // ring slots of the next K (0 1 3 5 .. of one row tile, 0 0 2 2 4 4 .. of two)
+        // and V (2 4 .., 1 apart at the end; 1 1 3 3 ..)
+        Slot<kNS> vs = base, ks = base;
+        vs.advance(v_pos(0, nt, two));
+        auto qk = [&](int w) {
+          const uint32_t q = q_sa + (two ? w * C::kQ : 0), k = ring + ks.i * C::kSlot;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
+            mma_f16(tmem + w * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), id_qk, kk > 0 ? 1u : 0u);
+          }
         };
-        ask(-2);
-        for (int t = -2; ok && t < steps; ++t) {
+        for (int t = 0; ok && t < 2; ++t) {
+          if (t < steps) {
+            ok = thread_wait(full(ks.i), ks.phase, abort_flag, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            qk(t);
+            ks.advance(two ? 2 * t : 1 + t);
+          }
+          mma_commit(s_full(t));
+        }
+        if (ok && seg > 0) ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+#pragma unroll 1
+        for (int t = 0; ok && t < steps; ++t) {
           const int w = t & 1;
-          const bool pv = t >= 0, qk = t + 2 < steps;
-          if (t == 0 && seg > 0) ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
-          const bool p_in = !pv || mbar_try_wait(p_full(w), tiles[w] & 1);
-          if (ok && !v_in) ok = thread_wait(full(sv), (at_v / kNS) & 1, abort_flag, p.status);
-          if (ok && !k_in) ok = thread_wait(full(sk), (at_k / kNS) & 1, abort_flag, p.status);
-          if (ok && !p_in) ok = thread_wait(p_full(w), tiles[w] & 1, abort_flag, p.status);
-          if (!ok) break;
-          if (pv) ++tiles[w];
+          const bool more = t + 2 < steps;
+          const uint32_t bv = full(vs.i), bk = more ? full(ks.i) : bv, bp = p_full(w), pp = tiles[w] & 1;
+          const uint32_t pk = more ? ks.phase : vs.phase;
+          // usually all are complete: one round of tests
+          if (!(mbar_test(bv, vs.phase) & mbar_test(bk, pk) & mbar_test(bp, pp))) {
+            ok = thread_wait(bv, vs.phase, abort_flag, p.status) && thread_wait(bk, pk, abort_flag, p.status) &&
+                 thread_wait(bp, pp, abort_flag, p.status);
+            if (!ok) break;
+          }
+          ++tiles[w];
           tc_fence_after();
-          if (pv) {
-            const uint32_t v = ring + sv * C::kSlot, o = tmem + 256 + (two ? w * 128 : 0);
-            const bool first = t < (two ? 2 : 1);
+          const uint32_t v = ring + vs.i * C::kSlot, o = tmem + 256 + (two ? w * 128 : 0);
+          const uint32_t acc = t < (two ? 2 : 1) ? 0u : 1u;
 #pragma unroll
-            for (int kk = 0; kk < kTcKeys / 16; ++kk)
-              mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
-                     (!first || kk > 0) ? 1u : 0u);
-          }
-          const uint32_t k = ring + sk * C::kSlot;
-          ask(t + 1);
-          if (qk) {
-            const uint32_t q = q_sa + (two ? w * C::kQ : 0);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
-              mma_f16(tmem + w * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), id_qk, kk > 0 ? 1u : 0u);
-            }
-          }
+          for (int kk = 0; kk < kTcKeys / 16; ++kk)
+            mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
+                   kk > 0 ? 1u : acc);
+          if (more) qk(w);
           mma_commit(s_full(w));  // S(t + 2), and in any case: PV(t) is done
+          const int n = two ? 2 * w : 2;
+          ks.advance(n);
+          vs.advance(two || t < nt - 2 ? n : 1);
         }
         if (!ok) break;
-        seq += 2 * nt;
+        base.advance(2 * nt);
         ++seg;
         // the last P was there, so every QK of this segment is done with Q
         have = take(seg);
@@ -1169,15 +1165,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             v1 = static_cast<uint32_t>(v >> 32);
           }
           float top = tail ? top_score<true>(t_s, v0, v1, p.scale_log2) : top_score<false>(t_s, 0, 0, p.scale_log2);
+          // (exchanging under the exponentials instead, with the rare correction
+          // after them, made the loop longer and slower)
           top = max3_nan(top, swap(top), -INFINITY);
           if (!ok) break;
           const bool moved = row_on && !(top <= m_ref + kSlack);
           if (__any_sync(0xffffffffu, moved)) {
             // infinite or NaN scores make the reference NaN and with it the row, as the formula does
             const float m_new = !moved ? m_ref : (top <= FLT_MAX ? ceilf(top) : NAN);
-            const float up = m_new - m_ref;
-            const float a =
-                up <= 126.f ? __uint_as_float(static_cast<uint32_t>(127.f - up) << 23) : (up != up ? NAN : 0.f);
+            const float a = pow2_down(m_new - m_ref);
             l *= a;
             m_ref = m_new;
             if (t >= (two ? 2 : 1)) {
@@ -1385,7 +1381,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
 
 // ------------------------------------------------------------------- host --
 struct Plan {
-  bool tc;
+  bool tc, never_cut;
   int tile_rows, group_rows, ctas, min_share;
   double items;  // bound of the call's work items
   size_t bytes;
@@ -1411,13 +1407,15 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   const double most = pl.items / pl.min_share + 1;
   const int ctas = tc ? kTcCtas : 2 * kTcCtas;
   pl.ctas = most < ctas ? static_cast<int>(most) : ctas;
+  // Share::find takes whole row groups if their longest are within kJoinCost of a share
+  pl.never_cut = static_cast<double>(num_seqs) * Hkv * row_groups <= pl.ctas && key_tiles <= pl.min_share + kJoinCost;
   pl.bytes = 256 + static_cast<size_t>(pl.ctas) * (2 * static_cast<size_t>(pl.group_rows) * (D + 2) * sizeof(float) + sizeof(Part));
   return pl;
 }
 
 template <typename T, int D>
 int launch_join(const TreeParams& p, cudaStream_t s) {
-  if (p.num_ctas == 1) return PS_OK;
+  if (p.num_ctas == 1 || p.never_cut) return PS_OK;
   ps_host::launch(tree_join_kernel<T, D>, dim3(p.num_ctas - 1, kJoinY), kJoinWarps * 32, 0, s, p);
   ps_host::count_launch();
   return ps_host::check_launch("tree_attention(join)");
@@ -1579,6 +1577,7 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.num_seqs = num_seqs;
   p.num_ctas = pl.ctas;
   p.min_share = pl.min_share;
+  p.never_cut = pl.never_cut;
   p.tile_rows = pl.tile_rows;
   p.group_rows = pl.group_rows;
   if (pl.tc) {
