@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
     else if (j < s.held + given) id = p.free_blocks[first + (j - s.held)];
     int slot = -1;
     if (id >= 0 && id < p.num_blocks) slot = id * p.block_size + static_cast<int>(at % p.block_size);
-    else record_error(p.status, j < s.held ? kErrBlockId : (j < s.need ? kErrNoBlocks : kErrShape));
+    else record_error(p.status, j < s.held + given ? kErrBlockId : (j < s.need ? kErrNoBlocks : kErrShape));
     p.slots[row0 + i] = slot;
     if (!p.parents) p.positions[row0 + i] = static_cast<int32_t>(at < INT32_MAX ? at : INT32_MAX);
   }

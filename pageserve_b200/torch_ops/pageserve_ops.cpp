@@ -265,9 +265,33 @@ int int_arg(int64_t v, const char* what) {
   return static_cast<int>(v);
 }
 
+// The outputs of one call, cut from one allocation: an allocation costs about
+// a microsecond of the host's time, as much as a small step's kernel takes, and
+// build_step_tables has seven outputs. They share a storage, not an element.
+class Outputs {
+ public:
+  Outputs(int64_t bytes, const at::TensorOptions& opt)
+      : base_(at::empty({bytes}, opt.dtype(at::kByte))) {}
+  static int64_t size(int64_t n, int64_t item) { return (n * item + 15) / 16 * 16; }
+  at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
+    const int64_t item = static_cast<int64_t>(c10::elementSize(type));
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(),
+                                                            c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(off_ / item);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    off_ += size(t.numel(), item);
+    return t;
+  }
+
+ private:
+  at::Tensor base_;
+  int64_t off_ = 0;
+};
+
 using StepOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
-StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
+// `out` undefined: the tables are an output too.
+StepOut step_tables_call(at::Tensor& out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
                               const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
                               int64_t num_blocks, int64_t block_size, int64_t total_tokens,
                               const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
@@ -278,13 +302,13 @@ StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const 
   metadata(block_tables, dev, what);
   metadata(held, dev, what);
   metadata(free_blocks, dev, what);
-  metadata(out, dev, what);
+  if (out.defined()) metadata(out, dev, what);
   const int64_t B = seq_lens.numel(), T = total_tokens;
   TORCH_CHECK_VALUE(B > 0, what, ": empty batch");
   TORCH_CHECK_VALUE(T >= 0, what, ": total_tokens below 0");
   TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.size(0) == B && q_lens.numel() == B && held.numel() == B,
                     what, ": q_lens, held and block_tables need one entry per request");
-  TORCH_CHECK_VALUE(out.sizes() == block_tables.sizes(), what, ": out must have block_tables' shape");
+  TORCH_CHECK_VALUE(!out.defined() || out.sizes() == block_tables.sizes(), what, ": out must have block_tables' shape");
   int64_t words = 0;
   if (parents.has_value()) {
     metadata(*parents, dev, what);
@@ -293,10 +317,14 @@ StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const 
     words = (std::max<int64_t>(*max_q_len, 0) + 63) / 64;
   }
   c10::cuda::CUDAGuard g(dev);
-  const auto i32 = seq_lens.options();
-  at::Tensor held_out = at::empty({B}, i32), cu_q = at::empty({B + 1}, i32), used = at::empty({1}, i32);
-  at::Tensor positions = at::empty({T}, i32), slots = at::empty({T}, i32);
-  at::Tensor mask = parents.has_value() ? at::empty({T, words}, i32.dtype(at::kLong)) : at::empty({0}, i32.dtype(at::kLong));
+  const int64_t mask_rows = parents.has_value() ? T : 0;
+  Outputs o(Outputs::size(mask_rows * words, 8) + 2 * Outputs::size(T, 4) + Outputs::size(B, 4) +
+                Outputs::size(B + 1, 4) + Outputs::size(1, 4) + (out.defined() ? 0 : Outputs::size(block_tables.numel(), 4)),
+            seq_lens.options());
+  at::Tensor mask = parents.has_value() ? o.take({T, words}, at::kLong) : o.take({0}, at::kLong);
+  at::Tensor positions = o.take({T}, at::kInt), slots = o.take({T}, at::kInt), held_out = o.take({B}, at::kInt);
+  at::Tensor cu_q = o.take({B + 1}, at::kInt), used = o.take({1}, at::kInt);
+  if (!out.defined()) out = o.take(block_tables.sizes(), at::kInt);
   check_v(ps_build_step_tables(out.data_ptr<int32_t>(), held_out.data_ptr<int32_t>(), cu_q.data_ptr<int32_t>(),
                                positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
                                parents.has_value() ? mask.data_ptr<int64_t>() : nullptr, used.data_ptr<int32_t>(),
@@ -311,12 +339,20 @@ StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const 
   return {held_out, cu_q, positions, slots, mask, used};
 }
 
+StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
+                              const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
+                              int64_t num_blocks, int64_t block_size, int64_t total_tokens,
+                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+  return step_tables_call(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size, total_tokens,
+                          parents, max_q_len);
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_step_tables(
     const at::Tensor& seq_lens, const at::Tensor& q_lens, const at::Tensor& block_tables, const at::Tensor& held,
     const at::Tensor& free_blocks, int64_t num_blocks, int64_t block_size, int64_t total_tokens,
     const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
-  at::Tensor out = at::empty(block_tables.sizes(), block_tables.options());
-  auto r = build_step_tables_out(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
+  at::Tensor out;
+  auto r = step_tables_call(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
                                  total_tokens, parents, max_q_len);
   return {out, std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r), std::get<5>(r)};
 }
@@ -409,9 +445,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> accept_trees(
     code = dtype_code(k);
   }
   c10::cuda::CUDAGuard g(dev);
-  const auto i32 = start_pos.options();
-  at::Tensor num = at::empty({B}, i32), start = at::empty({B}, i32);
-  at::Tensor nodes = at::empty({B, max_q_len}, i32), out = at::empty({B, max_q_len}, i32);
+  const int64_t wide = std::max<int64_t>(max_q_len, 0);  // the C call refuses 0 and below
+  Outputs o(2 * Outputs::size(B, 4) + 2 * Outputs::size(B * wide, 4), start_pos.options());
+  at::Tensor num = o.take({B}, at::kInt), start = o.take({B}, at::kInt);
+  at::Tensor nodes = o.take({B, wide}, at::kInt), out = o.take({B, wide}, at::kInt);
   check_v(ps_accept_trees(num.data_ptr<int32_t>(), nodes.data_ptr<int32_t>(), out.data_ptr<int32_t>(),
                           start.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), targets.data_ptr<int32_t>(),
                           tree_mask.data_ptr<int64_t>(), cu_q.data_ptr<int32_t>(), start_pos.data_ptr<int32_t>(),
