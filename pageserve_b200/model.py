@@ -5,7 +5,8 @@
 ``layers``, ``k_cache``, ``v_cache``, ``block_size``, ...), and adds
 ``forward_batch`` — one pass over a whole scheduler step (many decode
 sequences plus chunked-prefill chunks) from device-resident block tables —
-and ``capture_decode_graph`` for CUDA-graph replay of a decode step.
+and ``capture_decode_graph`` for CUDA-graph replay of a decode step. A step
+that verifies drafted token trees is ``verify_trees``.
 
 Per layer the step runs (engine/model.py:164-190):
   rmsnorm -> fused QKV W8A16 linear (+bias) -> RoPE + KV-slot write ->
@@ -19,6 +20,7 @@ from __future__ import annotations
 import os
 from dataclasses import dataclass
 from types import SimpleNamespace
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -27,6 +29,7 @@ from . import _lib
 from .batch import attention_runs, pack_metadata
 from .paged_attention import AttentionWorkspace, paged_attention
 from .quantization import LinearWorkspace, QuantizedWeight, RowView, linear16, linear_swiglu
+from .speculative import Accepted, StepTables, accept_trees, build_step_tables, tree_attention
 
 Weight = torch.Tensor | QuantizedWeight
 
@@ -196,6 +199,24 @@ class StepMeta:
         self.start_pos = start_pos
         self.q_lens = q_lens
         self.ctx_lens = ctx_lens
+
+
+class TreeMeta:
+    """Device-resident metadata of a step of drafted trees."""
+
+    def __init__(self, tables: StepTables, start_pos: torch.Tensor, max_q_len: int, max_ctx: int):
+        self.tables = tables
+        self.start_pos = start_pos
+        self.max_q_len = max_q_len
+        self.max_ctx = max_ctx
+
+
+class VerifiedTrees(NamedTuple):
+    """What ``PagedCausalLM.verify_trees`` returns (all on the device)."""
+    accepted: Accepted            # the kept path of every request; start_pos is the next step's seq_lens
+    tables: StepTables            # block_tables and held are the next step's; free_used blocks left the free list
+    targets: torch.Tensor         # (T,) int32 greedy next token of every row
+    logits: torch.Tensor | None   # (T, V), with return_logits
 
 
 class PagedCausalLM:
@@ -426,7 +447,7 @@ class PagedCausalLM:
         d = torch.from_numpy(buf).to(self.device, non_blocking=False)
         return StepMeta(d[2 * B + 1:].view(B, mb), d[:B + 1], d[B + 1:2 * B + 1], list(q_lens), ctx)
 
-    def _forward(self, ids: torch.Tensor, meta: StepMeta, logits_rows: torch.Tensor | None):
+    def _forward(self, ids: torch.Tensor, meta: StepMeta | TreeMeta, logits_rows: torch.Tensor | None):
         T = ids.shape[0]
         H, hq, hkv, d = self.hidden_size, self.heads_local, self.kv_heads_local, self.head_dim
         lead = self.tp is None or self.tp.rank == 0  # adds the residual exactly once
@@ -435,14 +456,17 @@ class PagedCausalLM:
         x = torch.empty((T, H), dtype=self.dtype, device=self.device)
         _lib.check(lib.ps_embedding(x.data_ptr(), ids.data_ptr(), self.embed_tokens.data_ptr(), T, H,
                                     self.vocab_size, _lib.dtype_code(self.dtype), stream), "embedding")
-        positions = torch.empty(T, dtype=torch.int32, device=self.device)
-        slots = torch.empty(T, dtype=torch.int32, device=self.device)
-        B = len(meta.q_lens)
-        _lib.check(lib.ps_build_slot_mapping(positions.data_ptr(), slots.data_ptr(), meta.block_tables.data_ptr(),
-                                             meta.block_tables.shape[1], meta.cu_q.data_ptr(),
-                                             meta.start_pos.data_ptr(), B, T, self.num_blocks, self.block_size,
-                                             stream), "build_slot_mapping")
-        runs = attention_runs(meta.q_lens, hq // hkv)
+        if isinstance(meta, TreeMeta):
+            positions, slots, runs = meta.tables.positions, meta.tables.slots, None
+        else:
+            positions = torch.empty(T, dtype=torch.int32, device=self.device)
+            slots = torch.empty(T, dtype=torch.int32, device=self.device)
+            B = len(meta.q_lens)
+            _lib.check(lib.ps_build_slot_mapping(positions.data_ptr(), slots.data_ptr(), meta.block_tables.data_ptr(),
+                                                 meta.block_tables.shape[1], meta.cu_q.data_ptr(),
+                                                 meta.start_pos.data_ptr(), B, T, self.num_blocks, self.block_size,
+                                                 stream), "build_slot_mapping")
+            runs = attention_runs(meta.q_lens, hq // hkv)
         q = torch.empty((T, hq, d), dtype=self.dtype, device=self.device)
         attn = torch.empty((T, hq, d), dtype=self.dtype, device=self.device)
         num_slots = self.num_blocks * self.block_size
@@ -531,7 +555,12 @@ class PagedCausalLM:
         """Paged attention of every run into its rows of ``attn``; with both
         kinds present, the prefill runs on the side stream (forked after the
         KV write, joined before o_proj), launched first so its CTAs start
-        before the decode grid fills the SMs."""
+        before the decode grid fills the SMs. A step of trees is one call; its
+        scratch comes from the allocator, so that a captured step owns it."""
+        if isinstance(meta, TreeMeta):
+            tree_attention(q, kc, vc, meta.tables.block_tables, meta.tables.cu_q, meta.start_pos, meta.tables.tree_mask,
+                           meta.max_q_len, meta.max_ctx, out=attn)
+            return
         def run(s, e, ws):
             paged_attention(q, kc, vc, meta.block_tables[s:e], meta.cu_q[s:e + 1], meta.start_pos[s:e],
                             max(meta.q_lens[s:e]), max(meta.ctx_lens[s:e]), out=attn, workspace=ws)
@@ -596,6 +625,49 @@ class PagedCausalLM:
             import torch.distributed as dist
             dist.broadcast(nxt, src=0, group=self.tp.group)
         return (full if return_logits else None), nxt
+
+    def verify_trees(self, tokens: torch.Tensor, parents: torch.Tensor, seq_lens: torch.Tensor, q_lens: torch.Tensor,
+                     block_tables: torch.Tensor, held: torch.Tensor, free_blocks: torch.Tensor, max_q_len: int,
+                     max_ctx: int | None = None, return_logits: bool = False) -> VerifiedTrees:
+        """One greedy decode step that verifies a tree of drafted tokens per
+        request (the reference decodes one token per request and step,
+        engine/runner.py:65-79, server.py:47-51).
+
+        tokens int64, parents int32 (T,): the requests' rows in order, each
+        request's first row its last confirmed token (not in the cache yet),
+        every other row a drafted token that follows its parent row. seq_lens
+        (cached tokens), q_lens (rows; 0 waits), held (blocks in its table row)
+        int32 (B,); block_tables int32 (B, max_blocks); free_blocks int32: the
+        blocks the step may take. max_q_len bounds q_lens (at most 256),
+        max_ctx seq_lens + q_lens (default: what a table row holds). Rows
+        behind the last request are padding (any token of the vocabulary).
+
+        The confirmed tokens of the step are ``accepted.tokens[b,
+        :accepted.num[b]]``, the same as that many single-token greedy steps
+        yield up to the kernels' rounding; the last of them is the next step's
+        root. The cache then holds ``accepted.start_pos`` tokens per request.
+        Nothing is read back to the host, so the call can be captured in a
+        CUDA graph after one call outside it. Device errors (a free list that is too
+        short, lengths past the bounds) are read by ``_lib.raise_on_device_error``."""
+        if self.k_cache is None:
+            raise RuntimeError("allocate_kv_cache() must run before verify_trees()")
+        _lib.require_cuda(tokens, parents, seq_lens, q_lens, block_tables, held, free_blocks)
+        T = tokens.numel()
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            raise TypeError("verify_trees: tokens must be contiguous int64")
+        if tokens.device != self.device:
+            raise ValueError(f"verify_trees: tokens on {tokens.device}, the model on {self.device}")
+        if T == 0:
+            raise ValueError("verify_trees: no rows")
+        tabs = build_step_tables(seq_lens, q_lens, block_tables, held, free_blocks, self.num_blocks, self.block_size,
+                                 T, parents=parents, max_q_len=max_q_len)
+        if max_ctx is None:
+            max_ctx = block_tables.shape[1] * self.block_size
+        logits = self._forward(tokens, TreeMeta(tabs, seq_lens, max_q_len, max_ctx), None)
+        targets = self.next_tokens(logits)
+        acc = accept_trees(tokens, targets, tabs.tree_mask, tabs.cu_q, seq_lens, max_q_len, self.k_cache, self.v_cache,
+                           tabs.block_tables)
+        return VerifiedTrees(acc, tabs, targets, self.gather_logits(logits) if return_logits else None)
 
     def gather_logits(self, logits: torch.Tensor) -> torch.Tensor:
         """Full-vocabulary logits (all-gathered over the vocab shards under TP)."""

@@ -209,8 +209,10 @@ def _run(c, dev, **kw):
 def _tolerance(c, ref, mag):
     """What the arithmetic may be off by. u: half a step of the type. The
     output's rounding u |o|; each weight's rounding u (its term of the sum of
-    w |v|) and, for f16 weights below 2^-14, half a subnormal step 2^-25 of a
-    sum that is at least 1; scores in 32 bits, D products whose magnitudes
+    w |v|) and, for f16 weights below 2^-14, half a subnormal step 2^-25; they
+    are powers 2^(s - r) with r the largest score rounded up to a whole number
+    (or a lower one), so the largest weight and with it the sum is at least
+    1/2, and the step counts 2^-24 after the division; scores in 32 bits, D products whose magnitudes
     sum to at most |q| |k|, each sum off by 2^-23 of it (the accumulator may
     truncate): a relative error of twice that in a weight, twice for weight and
     sum; the exponential and the join, 2^-20; sums over n keys, n 2^-23."""
@@ -223,7 +225,7 @@ def _tolerance(c, ref, mag):
     n = c["max_ctx"]
     delta = D * 2.0 ** -23 * qn * kn / np.sqrt(D)
     vmax = float(c["v"].double().abs().nan_to_num(0, 0, 0).max())
-    sub = n * 2.0 ** -25 * vmax if dt == torch.float16 else 0.0
+    sub = n * 2.0 ** -24 * vmax if dt == torch.float16 else 0.0
     return u * np.abs(ref) + (u + 4 * delta + 2.0 ** -20 + n * 2.0 ** -23) * 1.01 * mag + sub + 1e-30
 
 
@@ -456,6 +458,166 @@ def test_attention_cache_past_32_bits(dev):
     c["tab"] = np.where(c["tab"] >= 0, c["tab"] + nb - n, -1)
     c["k"], c["v"] = k, v
     assert torch.equal(_run(c, dev), small)
+    assert _status() == 0
+
+
+def _gpu_reference(c, dev):
+    """The oracle's definition (out, sum of weight times |v|) in 64 bits with
+    matrix products on the GPU, for sizes where numpy takes minutes."""
+    q, k, v = (c[x].to(dev) for x in "qkv")
+    hq, d = q.shape[1:]
+    hkv, bs = k.shape[2], c["bs"]
+    outs, mags = [], []
+    for b, n0 in enumerate(c["sp"]):
+        a, e = int(c["cu"][b]), int(c["cu"][b + 1])
+        n = e - a
+        pos = torch.arange(n0 + n, device=dev)
+        row = torch.as_tensor(c["tab"][b], device=dev)
+        kb, vb = (x[row[pos // bs], pos % bs].double().permute(1, 0, 2) for x in (k, v))  # hkv, keys, d
+        qb = q[a:e].double().reshape(n, hkv, hq // hkv, d).permute(1, 2, 0, 3)  # hkv, g, n, d
+        s = torch.einsum("hgnd,hkd->hgnk", qb, kb) / np.sqrt(d)
+        sees = torch.zeros(n, n, dtype=torch.bool)
+        for i, x in enumerate(c["sets"][a:e]):
+            sees[i, list(x)] = True
+        s[..., n0:].masked_fill_(~sees.to(dev), -float("inf"))
+        w = torch.softmax(s, -1)
+        outs.append(torch.einsum("hgnk,hkd->hgnd", w, vb).permute(2, 0, 1, 3).reshape(n, hq, d))
+        mags.append(torch.einsum("hgnk,hkd->hgnd", w, vb.abs()).permute(2, 0, 1, 3).reshape(n, hq, d))
+    return torch.cat(outs), torch.cat(mags)
+
+
+def _check_large(c, dev, out=None):
+    got = (_run(c, dev) if out is None else out).double()
+    ref, mag = _gpu_reference(c, dev)
+    err, tol = (got - ref).abs(), _tolerance(c, ref.cpu().numpy(), mag.cpu().numpy())
+    over = err.cpu().numpy() - tol
+    worst = np.unravel_index(np.argmax(over), over.shape)
+    assert (over <= 0).all(), (worst, err[worst].item(), tol[worst], ref[worst].item())
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("B,lo,hi,n,heads,dtype", [
+    (96, 1000, 1100, 16, (40, 8, 128), torch.bfloat16), (200, 300, 700, 5, (14, 2, 64), torch.float16),
+    (64, 130, 260, 8, (16, 2, 128), torch.bfloat16), (6, 700, 2100, 70, (16, 2, 128), torch.float16),
+    (40, 1, 500, 33, (8, 8, 128), torch.bfloat16)])
+def test_attention_rounds_of_the_ring(dev, B, lo, hi, n, heads, dtype):
+    """Enough tiles per CTA that every buffer is used many times, its last tile
+    cut anywhere; each row is right and the bits are the same every time."""
+    rng = np.random.default_rng(B)
+    ctxs = rng.integers(lo, hi + 1, B).tolist()
+    c = _case(20, ctxs, [n] * B if n < 30 else rng.integers(1, n + 1, B).tolist(), *heads, 16, dtype)
+    a = _run(c, dev)
+    for _ in range(6):
+        assert torch.equal(a, _run(c, dev))
+    _check_large(c, dev, a)
+
+
+@pytest.mark.parametrize("nodes", [[40, 64, 17, 33], [64] * 3, [128, 1, 100], [256, 16]])
+def test_attention_several_row_tiles(dev, nodes):
+    _check_large(_case(21, [300, 0, 1023, 64][:len(nodes)], nodes, 16, 2, 128, 16, torch.bfloat16), dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", ["rise", "fall", "spikes"])
+@pytest.mark.parametrize("Hq,Hkv,D,bs", [(16, 2, 128, 16), (14, 2, 64, 16), (16, 2, 128, 8)])
+def test_attention_scores_of_any_size(dev, shape, dtype, Hq, Hkv, D, bs):
+    """Scores whose largest rises (or falls, or jumps) by tens from tile to
+    tile, so that running sums are rescaled, weights vanish and shares with
+    very different maxima are joined."""
+    ctxs, nodes = [1500, 700, 130], [9, 20, 3]
+    c = _case(22, ctxs, nodes, Hq, Hkv, D, bs, dtype)
+    for b, n0 in enumerate(ctxs):
+        p = np.arange(n0 + nodes[b])
+        grow = {"rise": p / p.size * 20, "fall": (1 - p / p.size) * 20,
+                "spikes": np.where(p % 211 == 7, 30.0, 0.05)}[shape]
+        blk = torch.as_tensor(c["tab"][b][p // bs])
+        rows = c["k"][blk, torch.as_tensor(p % bs)].float() * torch.as_tensor(grow, dtype=torch.float32)[:, None, None]
+        c["k"][blk, torch.as_tensor(p % bs)] = rows.to(dtype)
+    _check_large(c, dev)
+
+
+def test_attention_row_that_is_not_finite(dev):
+    """A query row of infinities gives NaN, as the formula does, and no other
+    row notices."""
+    c = _case(23, [700, 60], [5, 3], 16, 2, 128, 16, torch.bfloat16)
+    clean = _run(c, dev)
+    c["q"][2] = float("inf")
+    got = _run(c, dev)
+    assert torch.isnan(got[2]).all()
+    keep = [0, 1, 3, 4, 5, 6, 7]
+    assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(160, 1, 64), (129, 1, 128)])
+def test_attention_wide_groups(dev, Hq, Hkv, D):
+    _check_large(_case(24, [50, 300], [3, 9], Hq, Hkv, D, 16, torch.bfloat16), dev)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_alignment_of_out(dev, D):
+    c = _case(25, [200, 40], [3, 9], 16, 2, D, 16, torch.bfloat16)
+    want = _run(c, dev)
+    buf = torch.full((want.numel() + 24,), 5.0, dtype=torch.bfloat16, device=dev)
+    out = buf[8:8 + want.numel()].view(want.shape)  # 16- but not 32-byte aligned
+    assert torch.equal(_run(c, dev, out=out), want)
+    assert (buf[:8] == 5).all() and (buf[8 + want.numel():] == 5).all()
+    with pytest.raises(ValueError):
+        _run(c, dev, out=buf[1:1 + want.numel()].view(want.shape))
+
+
+def test_two_graphs_own_their_scratch(dev):
+    """Calls captured without a workspace: two graphs, replayed at once on two
+    streams, with shared inputs."""
+    from pageserve_b200 import speculative as sp
+    c = _case(26, [3000, 1100, 64], [8, 30, 2], 16, 2, 128, 16, torch.bfloat16)
+    want = _run(c, dev)
+    q, k, v = (c[x].to(dev) for x in "qkv")
+    tab, cu, sp0 = _i32(c["tab"], dev), _i32(c["cu"], dev), _i32(c["sp"], dev)
+    mask = torch.from_numpy(tree.mask_words(c["sets"], 1)).to(dev)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(sp.tree_attention(q, k, v, tab, cu, sp0, mask, c["max_q"], c["max_ctx"]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    assert _status() == 0
+
+
+def test_tables_and_acceptance_in_a_graph(dev):
+    """A captured step's bookkeeping follows the lengths in its buffers."""
+    from pageserve_b200 import speculative as sp
+    seq, ql, held = _i32([5, 20], dev), _i32([3, 2], dev), _i32([1, 2], dev)
+    tab = _i32([[4, -1, -1], [2, 9, -1]], dev)
+    free = _i32([7, 1, 3], dev)
+    par = _i32([-1, 0, 0, -1, 0], dev)
+    tok = torch.tensor([5, 6, 7, 5, 6], device=dev)
+    tgt = _i32([7, 1, 2, 3, 4], dev)
+
+    def step():
+        t = sp.build_step_tables(seq, ql, tab, held, free, 10, 16, 5, parents=par, max_q_len=3)
+        return t, sp.accept_trees(tok, tgt, t.tree_mask, t.cu_q, seq, 3)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t, a = step()
+    for s in ([5, 20], [15, 31], [16, 32], [0, 0]):
+        seq.copy_(_i32(s, dev))
+        held.copy_(_i32([(x + 15) // 16 for x in s], dev))
+        g.replay()
+        t2, a2 = step()
+        for x, y in zip(t + a, t2 + a2):
+            assert torch.equal(x, y)
+        assert a.num.tolist() == [2, 1] and a.tokens.tolist() == [[7, 2, -1], [3, -1, -1]]
+        assert a.start_pos.tolist() == [s[0] + 2, s[1] + 1]
     assert _status() == 0
 
 

@@ -133,3 +133,25 @@ def test_cpu_tensors_raise():
         sp.tree_attention(x, c, c, i.view(1, 1), i, i, m, 1, 16)
     with pytest.raises(RuntimeError, match="CUDA"):
         sp.accept_trees(m.view(-1), i, m, i, i, 1)
+
+
+def test_torch_operators_have_meta_shapes():
+    """Fake-tensor tracing sees each operator's outputs."""
+    from pageserve_b200 import ops as torch_ops
+    if not torch_ops.LIB_PATH.exists():
+        pytest.skip("libpageserve_torch_ops.so is not built")
+    ns = torch_ops.load()
+    i = lambda *s: torch.empty(s, dtype=torch.int32, device="meta")  # noqa: E731
+    r = ns.build_step_tables(i(3), i(3), i(3, 7), i(3), i(9), 9, 16, 20, i(20), 70)
+    assert [tuple(x.shape) for x in r] == [(3, 7), (3,), (4,), (20,), (20,), (20, 2), (1,)]
+    assert [x.dtype for x in r] == [torch.int32] * 5 + [torch.int64, torch.int32]
+    r = ns.build_step_tables(i(3), i(3), i(3, 7), i(3), i(9), 9, 16, 20)
+    assert r[5].shape == (0,)
+    q = torch.empty(20, 4, 64, dtype=torch.bfloat16, device="meta")
+    kv = torch.empty(9, 16, 2, 64, dtype=torch.bfloat16, device="meta")
+    mask = torch.empty(20, 2, dtype=torch.int64, device="meta")
+    out = ns.tree_attention(q, kv, kv, i(3, 7), i(4), i(3), mask, 70, 112)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    tok = torch.empty(20, dtype=torch.int64, device="meta")
+    r = ns.accept_trees(tok, i(20), mask, i(4), i(3), 70)
+    assert [tuple(x.shape) for x in r] == [(3,), (3, 70), (3, 70), (3,)] and all(x.dtype == torch.int32 for x in r)
