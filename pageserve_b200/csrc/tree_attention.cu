@@ -573,18 +573,29 @@ constexpr int kMinShare = 4;
 template <int D>
 struct Tc {
   static constexpr int kPanels = D / 64;                // 64-column panels of 128 rows x 128 bytes
+  static constexpr int kGroup = kPanels * 1024;         // 8 keys of a K or V tile: panel after panel
   static constexpr int kSlot = kTcKeys * D * 2;         // one K or V tile
   static constexpr int kQ = kTcRows * D * 2;
   static constexpr int kSlots = (224 * 1024 - 2 * kQ) / kSlot;  // 5 (D = 128) or 12 (D = 64)
   static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 3072 /* barriers, (max, sum), flags */;
 };
 
-PS_DEVICE uint64_t desc_lbo(uint32_t addr, uint32_t lbo_bytes) {
-  return smem_desc_sw128(addr) | static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFF) << 16;
+// 128B-swizzled descriptor of a K or V tile: groups of 8 keys sbo bytes apart,
+// panels of 64 dims (read MN-major) lbo bytes.
+PS_DEVICE uint64_t tile_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>(lbo >> 4) << 16 |
+         static_cast<uint64_t>(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 // B read MN-major ([k][n] rows of the V tile)
 __host__ __device__ constexpr uint32_t idesc_bmn(bool bf16, int m, int n) { return instr_desc(bf16, m, n) | (1u << 16); }
 
+PS_DEVICE void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int group, int head) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4, %5}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(group), "r"(head)
+      : "memory");
+}
 PS_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -907,11 +918,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     // ---------------------------------------------------- K, V producers --
     const bool is_v = warp == 3;
     const CUtensorMap* map = is_v ? &vmap : &kmap;
-    const int groups = kTcKeys >> p.box_shift;  // boxes of a 64-dim panel
-    const int boxes = groups * C::kPanels;
-    const bool mine = lane < boxes;             // this lane's box of a tile
-    const int panel = lane / groups, grp = lane - panel * groups;
-    const uint32_t dst = ring + panel * (kTcKeys * 128) + (grp << p.box_shift) * 128;
+    const bool mine = lane < kTcKeys >> p.box_shift;  // this lane's box of a tile
+    const int grp = lane;
+    const uint32_t dst = ring + ((grp << p.box_shift) >> 3) * C::kGroup;
     const int past = p.num_blocks * p.block_size;  // a row behind the tensor: zeros
     uint32_t at = 0;  // position in the ring
     bool ok = true;
@@ -947,7 +956,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             s_at[s] = at;
           }
           __syncwarp();
-          if (mine) tma_load_3d(dst + s * C::kSlot, map, full(s), panel * 64, sg.h, row);
+          if (mine) tma_load_5d(dst + s * C::kSlot, map, full(s), row >> 3, sg.h);
         }
         ++at;
       };
@@ -1010,8 +1019,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           const uint32_t q = q_sa + (two ? w * C::kQ : 0), k = ring + ks.i * C::kSlot;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32;
-            mma_f16(tmem + w * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), id_qk, kk > 0 ? 1u : 0u);
+            mma_f16(tmem + w * 128, smem_desc_sw128(q + (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32),
+                    tile_desc(k + (kk >> 2) * 1024 + (kk & 3) * 32, 0, C::kGroup), id_qk, kk > 0 ? 1u : 0u);
           }
         };
         for (int t = 0; ok && t < 2; ++t) {
@@ -1043,8 +1052,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           const uint32_t acc = t < (two ? 2 : 1) ? 0u : 1u;
 #pragma unroll
           for (int kk = 0; kk < kTcKeys / 16; ++kk)
-            mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_lbo(v + kk * 16 * 128, kTcKeys * 128), id_pv,
-                   kk > 0 ? 1u : acc);
+            mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                   tile_desc(v + kk * 2 * C::kGroup, 1024, C::kGroup), id_pv, kk > 0 ? 1u : acc);
           if (more) qk(w);
           mma_commit(s_full(w));  // S(t + 2), and in any case: PV(t) is done
           const int n = two ? 2 * w : 2;
@@ -1135,13 +1144,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           const int key = key0 + r;
           if (key >= start) {
             bool bad = false;
-            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + r * 128;
+            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + (r >> 3) * C::kGroup + (r & 7) * 128;
             constexpr int kChunks = 8 * C::kPanels / 2;  // 16-byte chunks for each of a row's threads
 #pragma unroll 1
             for (int k = 0; k < kChunks; ++k) {
               // the lanes' lines share their banks: each starts at another chunk
               const int i = half * kChunks + ((k ^ r) & (kChunks < 8 ? kChunks - 1 : 7));
-              uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * (kTcKeys * 128) + ((i & 7) << 4));
+              uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * 1024 + ((i & 7) << 4));
               uint4 x = key < ctx ? *at16 : make_uint4(0, 0, 0, 0);
               const bool hit = clear_odd<T>(x);
               bad |= hit;
@@ -1453,6 +1462,23 @@ bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, long long rows
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// One layer's cache in boxes of box_keys keys of one head, as groups of 8 keys x
+// panels of 64 dims: one copy writes both panels, in the matrix unit's order.
+bool make_cache_map(CUtensorMap* map, const void* base, bool bf16, long long rows, int heads, int D, int box_keys) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t pitch = static_cast<cuuint64_t>(heads) * D * 2;
+  cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(D / 64), static_cast<cuuint64_t>(rows / 8),
+                        static_cast<cuuint64_t>(heads)};
+  cuuint64_t strides[4] = {pitch, 128, 8 * pitch, static_cast<cuuint64_t>(D) * 2};
+  cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(D / 64), static_cast<cuuint32_t>(box_keys / 8), 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 int launch_tc(TreeParams& p, cudaStream_t s) {
   CUtensorMap qm, km, vm;
@@ -1465,8 +1491,8 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
     if (p.block_size == 1 << i) p.block_shift = i;
   p.out32 = ps_host::aligned(p.out, 32);
   if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
-      !make_rows_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift) ||
-      !make_rows_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1, 1 << p.box_shift)) {
+      !make_cache_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1 << p.box_shift) ||
+      !make_cache_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1 << p.box_shift)) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
     return PS_ERR_CUDA;
   }
