@@ -101,7 +101,7 @@ PS_DEVICE Seq seq_of(const TreeParams& p, int b) {
 // shares cut row groups, which then have to be joined; where whole row groups,
 // an equal number per CTA, take at most kJoinCost key tiles longer, they are not
 // cut (64 sequences x 2 heads at equal contexts: 17 key tiles per CTA against 15
-// and a joining of about 6 us).
+// and a joining of about 6 us; a key tile takes 1.3 us).
 constexpr int kJoinCost = 4;
 
 struct Cut {  // one segment
@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
         o[i][2] *= corr[1];
         o[i][3] *= corr[1];
       }
-      // P is rounded to the cache's type for the matrix unit: relative 2^-9
-      // (bf16) or 2^-12 (f16) a term, below the rounding of the output
+      // P is rounded to the cache's type for the matrix unit: relative 2^-8
+      // (bf16) or 2^-11 (f16) a term, as the rounding of the output
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t pa[4];
@@ -536,12 +536,11 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // query rows, 128-key tiles:
 //   warps 0, 3 TMA producers of K and of V: tiles go through one ring of equal
 //              slots in the order that the MMAs read them (K0 K1 V0 K2 V1 ...),
-//              as boxes of up to 128 keys of one block x 64 dims, one lane a box;
-//              keys past the context or outside the pool are loads past the end
-//              of the tensor, which fill zeros. A warp issues boxes at a bounded
-//              rate: alone, 2 KB boxes (16-key blocks) streamed 4.9 TB/s from HBM
-//              with one warp, 5.95 with two, 6.3 with four. Dealing each tile to
-//              three warps was slower (445 against 423 us for the largest case)
+//              as boxes of up to 128 keys of one block, one lane a box; keys past
+//              the context or outside the pool are loads past the end of the tensor,
+//              which fill zeros. A warp issues boxes at a bounded rate (2 KB ones
+//              alone streamed 4.9 TB/s from HBM with one warp, 5.95 with two), so
+//              a box carries both 64-dim panels of its keys
 //   warp 2     walks the CTA's share and hands its segments to the other roles
 //   warp 1     TMEM, the Q tiles (128 / G nodes x the G heads of the group, one
 //              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
@@ -555,9 +554,13 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // PV(t). The MMA thread issues PV(t) QK(t + 2) under softmax(t + 1), with one
 // commit: what a commit costs the pipe is about one MMA, so ring slots are given
 // back by a softmax thread, for which S(t) complete says that K of step t and V of
-// step t - 2 have been read (MMAs complete in order). With two groups of warps on
-// alternate steps instead, each step's softmax (1900 clocks, bound by latency)
-// and MMAs (1460) followed one another: 2500 clocks a step.
+// step t - 2 have been read (MMAs complete in order).
+// A step lasts about 2300 clocks of the softmax warps (200 the largest scores, 200
+// their exchange, 1430 exponentials and P, of which the special-function unit
+// takes 1024), under which lie 1420 of the matrix unit. One thread per row and
+// two groups of warps on alternate steps took 2500; looking for step t + 1's
+// largest scores under step t's exponentials was no faster, for S(t + 1) is not
+// there yet (and a third S does not fit beside two O).
 // A softmax thread reads its scores from TMEM 32 at a time: holding them would
 // need more than the 168 registers that 12 warps leave a thread.
 // TMEM: S0 | S1 | O0 | O1 (the second row tile's), 128 columns each; the halves
@@ -587,7 +590,9 @@ PS_DEVICE uint64_t tile_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
          static_cast<uint64_t>(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 // B read MN-major ([k][n] rows of the V tile)
-__host__ __device__ constexpr uint32_t idesc_bmn(bool bf16, int m, int n) { return instr_desc(bf16, m, n) | (1u << 16); }
+__host__ __device__ constexpr uint32_t idesc_bmn(bool bf16, int m, int n) {
+  return instr_desc(bf16, m, n) | (1u << 16);
+}
 
 PS_DEVICE void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int group, int head) {
   asm volatile(
@@ -598,8 +603,8 @@ PS_DEVICE void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, i
 }
 PS_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-          dst),
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
@@ -727,7 +732,7 @@ PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale
         p1 = seen(2 * i + 1) ? p1 : 0.f;
       }
       sum[i & 3] = add2(sum[i & 3], pack_f2(p0, p1));  // four chains: one would bound the loop by its latency
-      // P rounded to 16 bits for the matrix unit: 2^-9 (bf16) or 2^-12 (f16) of a
+      // P rounded to 16 bits for the matrix unit: 2^-8 (bf16) or 2^-11 (f16) of a
       // term, as the output's own rounding
       pk[i] = pack2<T>(p0, p1);
     }
@@ -1379,8 +1384,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
     if (on && (!deal || warp == 0)) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int row = pt.row0 + r;
-      T* dst = static_cast<T*>(p.out) + (static_cast<long long>(pt.q0 + row / p.G) * p.Hq + pt.h * p.G + row % p.G) * D +
-               lane * DPL;
+      T* dst = static_cast<T*>(p.out) +
+               (static_cast<long long>(pt.q0 + row / p.G) * p.Hq + pt.h * p.G + row % p.G) * D + lane * DPL;
 #pragma unroll
       for (int i = 0; i < DPL; i += 2)
         *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
@@ -1418,7 +1423,8 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   pl.ctas = most < ctas ? static_cast<int>(most) : ctas;
   // Share::find takes whole row groups if their longest are within kJoinCost of a share
   pl.never_cut = static_cast<double>(num_seqs) * Hkv * row_groups <= pl.ctas && key_tiles <= pl.min_share + kJoinCost;
-  pl.bytes = 256 + static_cast<size_t>(pl.ctas) * (2 * static_cast<size_t>(pl.group_rows) * (D + 2) * sizeof(float) + sizeof(Part));
+  const size_t per_cta = 2 * static_cast<size_t>(pl.group_rows) * (D + 2) * sizeof(float) + sizeof(Part);
+  pl.bytes = 256 + static_cast<size_t>(pl.ctas) * per_cta;
   return pl;
 }
 
@@ -1550,6 +1556,12 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   if (total_q == 0) return PS_OK;
   if (!out || !q || !k_cache || !v_cache || !tables || !cu_q || !start_pos || !tree_mask) {
     ps_host::set_error("tree_attention: null pointer");
+    return PS_ERR_INVALID;
+  }
+  const uintptr_t q_at = reinterpret_cast<uintptr_t>(q), out_at = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t span = static_cast<uintptr_t>(total_q) * Hq * D * 2;
+  if (q_at < out_at + span && out_at < q_at + span) {
+    ps_host::set_error("tree_attention: out overlaps q, which other blocks may still read");
     return PS_ERR_INVALID;
   }
   if (!ps_host::aligned(k_cache, 16) || !ps_host::aligned(v_cache, 16) || !ps_host::aligned(q, 16) ||

@@ -565,6 +565,21 @@ def test_attention_alignment_of_out(dev, D):
         _run(c, dev, out=buf[1:1 + want.numel()].view(want.shape))
 
 
+def test_attention_refuses_an_output_that_overlaps_q(dev):
+    """Every head's rows of q are read by blocks that finish at any time."""
+    from pageserve_b200 import speculative as sp
+    c = _case(27, [40], [4], 4, 2, 64, 16, torch.bfloat16)
+    buf = torch.zeros(8, 4, 64, dtype=torch.bfloat16, device=dev)
+    buf[:4] = c["q"].to(dev)
+    k, v = c["k"].to(dev), c["v"].to(dev)
+    mask = torch.from_numpy(tree.mask_words(c["sets"], 1)).to(dev)
+    a = (k, v, _i32(c["tab"], dev), _i32(c["cu"], dev), _i32(c["sp"], dev), mask, 4, 44)
+    for lo in (0, 1, 3):
+        with pytest.raises(ValueError):
+            sp.tree_attention(buf[:4], *a, out=buf[lo:lo + 4])
+    assert torch.equal(sp.tree_attention(buf[:4], *a, out=buf[4:]), _run(c, dev))
+
+
 def test_two_graphs_own_their_scratch(dev):
     """Calls captured without a workspace: two graphs, replayed at once on two
     streams, with shared inputs."""
