@@ -1036,9 +1036,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             qk(t);
             ks.advance(two ? 2 * t : 1 + t);
           }
-          mma_commit(s_full(t));
+          if (seg == 0) mma_commit(s_full(t));
         }
-        if (ok && seg > 0) ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+        if (ok && seg > 0) {
+          // The softmax warps are done with the last segment's O and its two last S
+          // phases: a commit before that could put a warp two phases behind.
+          ok = thread_wait(o_free, (seg - 1) & 1, abort_flag, p.status);
+          if (!ok) break;
+          mma_commit(s_full(0));
+          mma_commit(s_full(1));
+        }
 #pragma unroll 1
         for (int t = 0; ok && t < steps; ++t) {
           const int w = t & 1;

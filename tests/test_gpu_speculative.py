@@ -565,6 +565,24 @@ def test_attention_alignment_of_out(dev, D):
         _run(c, dev, out=buf[1:1 + want.numel()].view(want.shape))
 
 
+def test_attention_many_calls_in_a_row(dev):
+    """Many segments per CTA, thousands of calls queued behind each other: no
+    wait runs out (an error is recorded for one that does) and the bits stay."""
+    from pageserve_b200 import speculative as sp
+    from pageserve_b200.paged_attention import AttentionWorkspace
+    rng = np.random.default_rng(28)
+    c = _case(28, rng.integers(0, 700, 60).tolist(), rng.integers(1, 20, 60).tolist(), 40, 8, 128, 16, torch.bfloat16)
+    want = _run(c, dev)
+    q, k, v = (c[x].to(dev) for x in "qkv")
+    a = (_i32(c["tab"], dev), _i32(c["cu"], dev), _i32(c["sp"], dev),
+         torch.from_numpy(tree.mask_words(c["sets"], 1)).to(dev), c["max_q"], c["max_ctx"])
+    out, ws = torch.zeros_like(q), AttentionWorkspace()
+    for _ in range(3000):
+        sp.tree_attention(q, k, v, *a, out=out, workspace=ws)
+    assert torch.equal(out, want)
+    assert _status() == 0
+
+
 def test_attention_refuses_an_output_that_overlaps_q(dev):
     """Every head's rows of q are read by blocks that finish at any time."""
     from pageserve_b200 import speculative as sp
