@@ -1565,12 +1565,6 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
     ps_host::set_error("tree_attention: null pointer");
     return PS_ERR_INVALID;
   }
-  const uintptr_t q_at = reinterpret_cast<uintptr_t>(q), out_at = reinterpret_cast<uintptr_t>(out);
-  const uintptr_t span = static_cast<uintptr_t>(total_q) * Hq * D * 2;
-  if (q_at < out_at + span && out_at < q_at + span) {
-    ps_host::set_error("tree_attention: out overlaps q, which other blocks may still read");
-    return PS_ERR_INVALID;
-  }
   if (!ps_host::aligned(k_cache, 16) || !ps_host::aligned(v_cache, 16) || !ps_host::aligned(q, 16) ||
       !ps_host::aligned(out, 16) || !ps_host::aligned(workspace, 16)) {
     ps_host::set_error("tree_attention: q, out, the caches and the workspace need 16-byte alignment");
@@ -1592,6 +1586,12 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   }
   if (!workspace || workspace_bytes < pl.bytes) {
     ps_host::set_error("tree_attention: workspace of %zu bytes needed, %zu given", pl.bytes, workspace_bytes);
+    return PS_ERR_INVALID;
+  }
+  const uintptr_t q_at = reinterpret_cast<uintptr_t>(q), out_at = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t span = static_cast<uintptr_t>(total_q) * Hq * D * 2;
+  if (q_at < out_at + span && out_at < q_at + span) {
+    ps_host::set_error("tree_attention: out overlaps q, which other blocks may still read");
     return PS_ERR_INVALID;
   }
   TreeParams p{};
