@@ -322,7 +322,8 @@ PS_API int ps_tree_attention(void* out_dev, const void* q_dev, const void* k_cac
  *   in both caches ([num_layers][num_blocks][block_size][num_kv_heads][head_dim],
  *   dtype PS_BF16 / PS_F16 / PS_F32; both NULL: no move) the rows at positions
  *   start + path[k] move to start + k. Rows behind start_out are left over.
- * num and start_out must not alias start_pos or cu_q. max_q_len <= 256. */
+ * num and start_out must not alias start_pos or cu_q, nor the caches each other.
+ * max_q_len <= 256. */
 PS_API int ps_accept_trees(int32_t* num_dev, int32_t* nodes_dev, int32_t* out_tokens_dev, int32_t* start_out_dev,
                            const int64_t* tokens_dev, const int32_t* targets_dev, const int64_t* tree_mask_dev,
                            const int32_t* cu_q_dev, const int32_t* start_pos_dev, int num_seqs, int total_tokens,

@@ -235,6 +235,12 @@ extern "C" int ps_accept_trees(int32_t* num, int32_t* nodes, int32_t* out_tokens
       ps_host::set_error("accept_trees: cache rows must be whole 16-byte units and the caches 16-byte aligned");
       return PS_ERR_INVALID;
     }
+    const uintptr_t k_at = reinterpret_cast<uintptr_t>(k_cache), v_at = reinterpret_cast<uintptr_t>(v_cache);
+    const uintptr_t span = static_cast<uintptr_t>(num_layers) * num_blocks * block_size * row_bytes;
+    if (k_at < v_at + span && v_at < k_at + span) {
+      ps_host::set_error("accept_trees: the caches overlap; their rows are moved at the same time");
+      return PS_ERR_INVALID;
+    }
     p.row_units = static_cast<int>(row_bytes / 16);
     p.layer_units = static_cast<long long>(num_blocks) * block_size * p.row_units;
     // One unit per thread, unless that is more than kCtas CTAs, whose finding of

@@ -583,6 +583,25 @@ def test_attention_many_calls_in_a_row(dev):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("bs", [48, 80, 96, 192, 384])
+@pytest.mark.parametrize("Hq,Hkv,D", [(14, 2, 64), (16, 2, 128)])
+def test_attention_blocks_of_several_boxes(dev, bs, Hq, Hkv, D):
+    """Block sizes that are whole 16-key groups but no power of two: keys are
+    loaded in the largest power of two that divides them."""
+    _check_large(_case(29, [bs - 1, 500, 3 * bs, 1], [7, 20, 1, 3], Hq, Hkv, D, bs, torch.bfloat16), dev)
+
+
+def test_attention_without_work(dev):
+    """Requests that all wait: nothing is written."""
+    from pageserve_b200 import speculative as sp
+    q = torch.ones(3, 16, 128, dtype=torch.bfloat16, device=dev)
+    kv = torch.zeros(4, 16, 2, 128, dtype=torch.bfloat16, device=dev)
+    out = torch.full_like(q, 3.0)
+    mask = torch.zeros(3, 1, dtype=torch.int64, device=dev)
+    sp.tree_attention(q, kv, kv, _i32([[0, 1], [2, 3]], dev), _i32([0, 0, 0], dev), _i32([9, 0], dev), mask, 3, 32, out=out)
+    assert (out == 3).all() and _status() == 0
+
+
 def test_attention_refuses_an_output_that_overlaps_q(dev):
     """Every head's rows of q are read by blocks that finish at any time."""
     from pageserve_b200 import speculative as sp

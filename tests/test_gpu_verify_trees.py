@@ -223,3 +223,17 @@ def test_verification_refusals(dev):
     m.k_cache = None
     with pytest.raises(RuntimeError):
         m.verify_trees(tok, par, i, one, tab, i, free, 1)
+
+
+def test_all_requests_wait(dev):
+    """A step of padding alone changes nothing."""
+    from pageserve_b200 import _lib
+    m = _model(torch.bfloat16, True, 16, 16)
+    s = _Requests(m, [np.arange(20), np.arange(5)], 4, range(16), dev)
+    before = m.k_cache.clone(), m.v_cache.clone()
+    zero = torch.zeros(2, dtype=torch.int32, device=dev)
+    r = m.verify_trees(torch.zeros(3, dtype=torch.int64, device=dev), torch.full((3,), -1, dtype=torch.int32, device=dev),
+                       s.cached, zero, s.tables, s.held, s.free, 8)
+    assert s.take(r) == [[], []] and s.cached.tolist() == [19, 4]
+    assert torch.equal(m.k_cache, before[0]) and torch.equal(m.v_cache, before[1])
+    assert _lib.device_status(clear=True) == 0

@@ -155,3 +155,14 @@ def test_torch_operators_have_meta_shapes():
     tok = torch.empty(20, dtype=torch.int64, device="meta")
     r = ns.accept_trees(tok, i(20), mask, i(4), i(3), 70)
     assert [tuple(x.shape) for x in r] == [(3,), (3, 70), (3, 70), (3,)] and all(x.dtype == torch.int32 for x in r)
+
+
+def test_accept_trees_refuses_overlapping_caches():
+    """K and V rows move at the same time: one cache as both, or two that
+    overlap, would lose rows."""
+    lib = _lib_or_skip()
+    size = 2 * 16 * 16 * 2 * 64 * 2  # bytes of a cache of _accept's sizes
+    for v in (P, P + 16, P + size - 16):
+        assert _accept(lib, v=v) == _lib.PS_ERR_INVALID
+        assert "overlap" in _lib.last_error()
+        assert _accept(lib, k=v, v=P) == _lib.PS_ERR_INVALID
