@@ -546,9 +546,9 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 //              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
 //              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major), all
 //              by one thread
-//   warps 4-11 softmax, two threads per row: warps 4-7 the first 64 keys of a
-//              tile, warps 8-11 the others; a pair of warps exchanges its rows'
-//              maxima, so that both halves of P refer to the same one
+//   warps 4-11 softmax, two threads per row (DUP: four): warps 4-7 the first 64
+//              keys of a tile, warps 8-11 the others; a pair of warps exchanges its
+//              rows' maxima, so that both halves of P refer to the same one
 // Step t is a key tile (of one row tile, up to 128 rows) or a key tile and one of
 // two row tiles in turn, which then share every loaded tile: QK(t), softmax(t),
 // PV(t). The MMA thread issues PV(t) QK(t + 2) under softmax(t + 1), with one
@@ -561,6 +561,13 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // two groups of warps on alternate steps took 2500; looking for step t + 1's
 // largest scores under step t's exponentials was no faster, for S(t + 1) is not
 // there yet (and a third S does not fit beside two O).
+// DUP: calls whose row groups have at most 64 rows by their bounds load them into
+// both halves of the tile, lanes r and r + 64. Of every 64 keys lane r's P has the
+// first 32 and zeros, lane r + 64's the others: four threads per row, each with a
+// quarter of its keys. The two lanes are two shares of the softmax with a maximum,
+// a sum and an O each, joined when the row group's keys are done. One node at
+// context 128: 9.0 -> 8.3 us, 5 requests x 7 nodes 10.6 -> 9.5, 64 x 8 nodes at 2048
+// 35.6 -> 33.6 (copies of K and V alone at this pattern and these CTAs: within 10%).
 // A softmax thread reads its scores from TMEM 32 at a time: holding them would
 // need more than the 168 registers that 12 warps leave a thread.
 // TMEM: S0 | S1 | O0 | O1 (the second row tile's), 128 columns each; the halves
@@ -681,38 +688,38 @@ PS_DEVICE void scale_o(uint32_t t_o, int n, float alpha) {
   tmem_wait_st();
 }
 
-// The largest of this thread's 64 scores (in the log2 domain; NaN if one is).
+// The largest of N of this thread's scores (in the log2 domain; NaN if one is).
 // TAIL: bit i of v1:v0 says that the row sees key i.
-template <bool TAIL>
+template <int N, bool TAIL>
 PS_DEVICE float top_score(uint32_t t_s, uint32_t v0, uint32_t v1, float scale) {
-  float sv[64];
-  tmem_ld32_issue(t_s, sv);
-  tmem_ld32_issue(t_s + 32, sv + 32);
+  float sv[N];
+#pragma unroll
+  for (int c = 0; c < N; c += 32) tmem_ld32_issue(t_s + c, sv + c);
   tmem_wait_ld();
-  tmem_ready(sv);
-  tmem_ready(sv + 32);
+#pragma unroll
+  for (int c = 0; c < N; c += 32) tmem_ready(sv + c);
   auto seen = [&](int i) { return !TAIL || (((i < 32 ? v0 : v1) >> (i & 31)) & 1); };
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < 64; i += 2)
+  for (int i = 0; i < N; i += 2)
     mx[(i >> 1) & 3] =
         max3_nan(mx[(i >> 1) & 3], seen(i) ? sv[i] : -INFINITY, seen(i + 1) ? sv[i + 1] : -INFINITY);
   return max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
 }
-// This thread's 64 scores become P against the row's reference max, 32 at a time
+// N of this thread's scores become P against the row's reference max, 32 at a time
 // (16-bit columns 16 c .. lie below the scores still to be read); returns the sum
 // of P. The loop stays rolled: longer bodies ran slower, from beyond the
 // first-level instruction cache. (Taking 3 of 8 exponentials to the FMA pipe by a
 // polynomial was no faster: the loop is bound by latency and issue, not by the
 // special-function unit.)
-template <typename T, bool TAIL>
-PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale, float m_ref) {
+template <typename T, int N, bool TAIL>
+PS_DEVICE float softmax_part(uint32_t t_s, uint32_t t_p, uint32_t v0, uint32_t v1, float scale, float m_ref) {
   float sv[32];
   f32x2 sum[4] = {0, 0, 0, 0};
   const f32x2 scale2 = pack_f2(scale, scale), neg_m = pack_f2(-m_ref, -m_ref);
   tmem_ld32_issue(t_s, sv);
 #pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < N / 32; ++c) {
     const uint32_t vc = c ? v1 : v0;
     auto seen = [&](int i) { return !TAIL || ((vc >> i) & 1); };
     tmem_wait_ld();
@@ -720,7 +727,7 @@ PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale
     f32x2 x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = fma2(pack_f2(sv[2 * i], sv[2 * i + 1]), scale2, neg_m);
-    if (c == 0) tmem_ld32_issue(t_s + 32, sv);  // under this group's exponentials
+    if (N > 32 && c == 0) tmem_ld32_issue(t_s + 32, sv);  // under this group's exponentials
     uint32_t pk[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -736,7 +743,7 @@ PS_DEVICE float softmax_half(uint32_t t_s, uint32_t v0, uint32_t v1, float scale
       // term, as the output's own rounding
       pk[i] = pack2<T>(p0, p1);
     }
-    tmem_st16(t_s + c * 16, pk);
+    tmem_st16(t_p + c * 16, pk);
   }
   float s0, s1;
   unpack_f2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
@@ -808,7 +815,7 @@ PS_DEVICE bool thread_wait(uint32_t bar, uint32_t parity, volatile int* abort_fl
   return true;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool DUP>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                 const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap,
@@ -837,7 +844,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   auto pair = [&](int quarter) { return bars + 8 * (2 * kNS + 7 + quarter); };
   auto seg_full = [&](int i) { return bars + 8 * (2 * kNS + 11 + i); };
   auto seg_empty = [&](int i) { return bars + 8 * (2 * kNS + 11 + kSegRing + i); };
-  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 12 + 2 * kSegRing);
+  auto cross = [&](int i) { return bars + 8 * (2 * kNS + 11 + 2 * kSegRing + i); };
+  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 14 + 2 * kSegRing);
   float* s_swap = reinterpret_cast<float*>(misc);  // [2][2 halves][128 rows]
   Seg* s_seg = reinterpret_cast<Seg*>(misc + 2 * 128 * 8);  // [kSegRing]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_seg + kSegRing);
@@ -865,6 +873,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     mbar_init(q_full, 1);
     mbar_init(o_free, 8);
     for (int i = 0; i < 4; ++i) mbar_init(pair(i), 2);
+    for (int i = 0; i < 2; ++i) mbar_init(cross(i), 4);
     mbar_init(drained, 1);
     for (int i = 0; i < kSegRing; ++i) {
       mbar_init(seg_full(i), 1);
@@ -932,7 +941,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     Seg sg;
     for (uint32_t i = 0; ok && read_seg(i, sg); ++i) {
       const int nt = sg.nt;
-      const bool two = sg.flags & kSegTwo;
+      const bool two = !DUP && (sg.flags & kSegTwo);
       const int ctx = sg.start + sg.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
       // row of this lane's box of tile j
@@ -1000,20 +1009,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         return !(nx.flags & kSegStop);
       };
       auto load_q = [&] {  // of nx
-        const int copies = nx.flags & kSegTwo ? 2 : 1;
+        const int copies = DUP || (nx.flags & kSegTwo) ? 2 : 1;
         const int node = nx.q0 + nx.row0 / p.G;
         mbar_expect_tx(q_full, copies * C::kPanels * p.tile_rows * 128);
         for (int i = 0; i < copies; ++i)
           for (int pn = 0; pn < C::kPanels; ++pn)
-            tma_load_3d(q_sa + i * C::kQ + pn * (kTcRows * 128), &qmap, q_full, pn * 64, nx.h * p.G,
-                        node + i * tile_nodes);
+            tma_load_3d(q_sa + i * (DUP ? 64 * 128 : C::kQ) + pn * (kTcRows * 128), &qmap, q_full, pn * 64, nx.h * p.G,
+                        node + (DUP ? 0 : i * tile_nodes));
         ++q_loads;
       };
       bool have = take(0);
       if (have) load_q();
       while (ok && have) {
         const int nt = nx.nt;
-        const bool two = nx.flags & kSegTwo;
+        const bool two = !DUP && (nx.flags & kSegTwo);
         const int steps = two ? 2 * nt : nt;
         ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
         // ring slots of the next K (0 1 3 5 .. of one row tile, 0 0 2 2 4 4 .. of two)
@@ -1090,28 +1099,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     // ----------------------------------------------------------- softmax --
     const int half = (warp - 4) >> 2;   // which 64 keys of a tile
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // this thread's row of a tile (its TMEM lane)
+    const int side = DUP ? quarter >> 1 : 0;
+    const int t_lane = quarter * 32 + lane;   // this thread's TMEM lane
+    const int r = DUP ? t_lane & 63 : t_lane;  // and the row of a tile in it
+    const int first_row = r - lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int r_node = r / p.G, r_head = r - r_node * p.G;
     const bool gives = threadIdx.x == 128;  // gives back the ring slots
-    uint32_t seq = 0, swaps = 0;
+    uint32_t seq = 0, swaps = 0, crosses = 0;
     uint32_t phase[2] = {0, 0};  // completed S waits of each buffer before this segment
     bool ok = true;
     // the value of this row's other thread; both warps of a pair make the same calls
     auto swap = [&](float v) {
       float* at = s_swap + (swaps & 1) * 256;
-      at[half * 128 + r] = v;
+      at[half * 128 + t_lane] = v;
       __syncwarp();
       if (lane == 0) mbar_arrive(pair(quarter));
       ok = ok && warp_wait(pair(quarter), swaps & 1, abort_flag, p.status);
       ++swaps;
-      return at[(half ^ 1) * 128 + r];
+      return at[(half ^ 1) * 128 + t_lane];
     };
     Seg sg;
     for (uint32_t seg = 0; ok && read_seg(seg, sg); ++seg) {
       const int nt = sg.nt;
       const int n = sg.n, start = sg.start, ctx = start + n;
-      const bool two = sg.flags & kSegTwo;
+      const bool two = !DUP && (sg.flags & kSegTwo);
       const int steps = two ? 2 * nt : nt;
       const int node0 = sg.row0 / p.G + r_node;  // of the first row tile
       const int rows0 = min(sg.rows, p.tile_rows), rows1 = sg.rows - rows0;
@@ -1153,15 +1165,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           const int s = static_cast<int>(at % kNS);
           ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status);
           if (!ok) break;
-          const int key = key0 + r;
+          const int row = t_lane, key = key0 + row;
           if (key >= start) {
             bool bad = false;
-            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + (r >> 3) * C::kGroup + (r & 7) * 128;
+            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + (row >> 3) * C::kGroup + (row & 7) * 128;
             constexpr int kChunks = 8 * C::kPanels / 2;  // 16-byte chunks for each of a row's threads
 #pragma unroll 1
             for (int k = 0; k < kChunks; ++k) {
               // the lanes' lines share their banks: each starts at another chunk
-              const int i = half * kChunks + ((k ^ r) & (kChunks < 8 ? kChunks - 1 : 7));
+              const int i = half * kChunks + ((k ^ row) & (kChunks < 8 ? kChunks - 1 : 7));
               uint4* at16 = reinterpret_cast<uint4*>(line + (i >> 3) * 1024 + ((i & 7) << 4));
               uint4 x = key < ctx ? *at16 : make_uint4(0, 0, 0, 0);
               const bool hit = clear_odd<T>(x);
@@ -1173,7 +1185,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           fence_proxy_async();
         }
         tc_fence_after();
-        if (quarter * 32 < (tile ? rows1 : rows0)) {
+        if (first_row < (tile ? rows1 : rows0)) {
           const uint32_t t_s = tmem + w * 128 + half * 64 + lane_off;
           uint32_t v0 = 0, v1 = 0;
           if (tail) {
@@ -1185,7 +1197,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             v0 = static_cast<uint32_t>(v);
             v1 = static_cast<uint32_t>(v >> 32);
           }
-          float top = tail ? top_score<true>(t_s, v0, v1, p.scale_log2) : top_score<false>(t_s, 0, 0, p.scale_log2);
+          // DUP: the 32 keys of this side, and zeros in P for the other's
+          constexpr int kN = DUP ? 32 : 64;
+          const uint32_t t_n = t_s + side * 32, t_p = t_s + side * 16;
+          if (DUP && side) v0 = v1;
+          float top = tail ? top_score<kN, true>(t_n, v0, v1, p.scale_log2)
+                           : top_score<kN, false>(t_n, 0, 0, p.scale_log2);
           // (exchanging under the exponentials instead, with the rare correction
           // after them, made the loop longer and slower)
           top = max3_nan(top, swap(top), -INFINITY);
@@ -1205,8 +1222,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
               scale_o(tmem + 256 + tile * 128 + half * (D / 2) + lane_off, D / 64, a);
             }
           }
-          l += tail ? softmax_half<T, true>(t_s, v0, v1, p.scale_log2, m_ref)
-                    : softmax_half<T, false>(t_s, 0, 0, p.scale_log2, m_ref);
+          l += tail ? softmax_part<T, kN, true>(t_n, t_p, v0, v1, p.scale_log2, m_ref)
+                    : softmax_part<T, kN, false>(t_n, t_p, 0, 0, p.scale_log2, m_ref);
+          if (DUP) {
+            const uint32_t zero[16] = {};
+            tmem_st16(t_s + (side ^ 1) * 16, zero);
+          }
           tmem_wait_st();
         }
         tc_fence_before();
@@ -1237,33 +1258,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
       const int slot = sg.tile0 > 0 ? 0 : 1;
       for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
         const int rows = tile ? rows1 : rows0;
-        if (quarter * 32 < rows) {  // this thread's half of its row's columns
-          const float m = tile ? m_b : m_ref;
+        if (first_row < rows) {  // this thread's half (DUP: quarter) of its row's columns
+          float m = tile ? m_b : m_ref;
           float lt = tile ? l_b : l;
           lt += swap(lt);
           if (!ok) break;
-          const float f = !whole ? 1.f : (lt == 0.f ? 0.f : 1.f / lt);
           const bool row_on = r < rows;
           const int lr = tile * p.tile_rows + r, node = node0 + tile * tile_nodes;
-          const int col0 = half * (D / 2);
+          constexpr int kCols = DUP ? D / 4 : D / 2;  // it stores, kChunk at a time
+          constexpr int kChunk = kCols < 32 ? kCols : 32;
+          const int col0 = half * (D / 2) + side * (D / 4);
+          const uint32_t t_o = tmem + 256 + tile * 128 + lane_off;
+          float o[32], f = 1.f;
+          if (DUP) {
+            // Both sides' sums and half of each side's O change hands through the
+            // unused second Q tile; the next segment's S comes after everyone's o_free.
+            float* x = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + side) * kCols) * 64 + r;
+            tmem_ld32(t_o + half * (D / 2) + (D == 128 ? (side ^ 1) * 32 : 0), o);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) x[i * 64] = D == 128 ? o[i] : (side ? o[i] : o[i + 32 - kCols]);
+            float* at = s_swap + (swaps & 1) * 256 + t_lane;  // (the pair's next buffer)
+            at[half * 128] = half ? lt : m;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(cross(quarter & 1));
+            ok = warp_wait(cross(quarter & 1), crosses++ & 1, abort_flag, p.status);
+            if (!ok) break;
+            const float* other = s_swap + (swaps & 1) * 256 + (t_lane ^ 64);
+            const float m2 = other[0], l2 = other[128];
+            const float m1 = m;
+            m = fmaxf(m1, m2);
+            f = exp2f(m1 - m);  // NaN if a max is
+            const float f2 = exp2f(m2 - m);
+            lt = lt * f + l2 * f2;
+            if (D == 128) tmem_ld32(t_o + col0, o);
+            const float* y = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + (side ^ 1)) * kCols) * 64 + r;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i)
+              o[i] = (D == 128 ? o[i] : (side ? o[i + 32 - kCols] : o[i])) * f + y[i * 64] * f2;
+            f = 1.f;
+          }
+          if (whole) f = lt == 0.f ? 0.f : 1.f / lt;
           T* dst = static_cast<T*>(p.out) +
                    (static_cast<long long>(sg.q0 + node) * p.Hq + sg.h * p.G + r_head) * D + col0;
 #pragma unroll 1
-          for (int c = 0; c < D / 64; ++c) {
-            float o[32];
-            tmem_ld32(tmem + 256 + tile * 128 + lane_off + col0 + c * 32, o);
+          for (int c = 0; c < kCols / kChunk; ++c) {
+            if (!DUP) tmem_ld32(t_o + col0 + c * 32, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
+            for (int i = 0; i < kChunk; ++i) o[i] *= f;
             if (row_on) {
               // a store of a warp's 32 rows to out touches a line each: the wider the better
               if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < kChunk / 8; ++i)
                   st_global_32(part_o(p, blockIdx.x, slot, lr, (col0 >> 3) + c * 4 + i, D),
                                reinterpret_cast<const uint32_t*>(o + 8 * i));
               } else if (p.out32) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 16) {
+                for (int i = 0; i < kChunk; i += 16) {
                   uint32_t v[8];
 #pragma unroll
                   for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
@@ -1271,11 +1322,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                 }
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o + i);
+                for (int i = 0; i < kChunk; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o + i);
               }
             }
           }
-          if (!whole && row_on && half == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
+          if (!whole && row_on && half == 0 && side == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
           if (s_odd[seg % 3] != 0 && row_on) {
             // the cleared values, added to what this thread has stored for a row that sees them
             const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
@@ -1291,7 +1342,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                             ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
                             col0;
 #pragma unroll 1
-              for (int i = 0; i < D / 2; ++i) {
+              for (int i = 0; i < kCols; ++i) {
                 const T x = vr[i];
                 if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
                 if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
@@ -1402,7 +1453,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
 
 // ------------------------------------------------------------------- host --
 struct Plan {
-  bool tc, never_cut;
+  bool tc, dup, never_cut;
   int tile_rows, group_rows, ctas, min_share;
   double items;  // bound of the call's work items
   size_t bytes;
@@ -1418,8 +1469,9 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   Plan pl{};
   const int G = Hq / Hkv, keys = tc ? kTcKeys : kKeys;
   pl.tc = tc;
-  pl.tile_rows = tc ? kTcRows / G * G : kRows;
-  pl.group_rows = tc ? 2 * pl.tile_rows : kRows;
+  pl.dup = tc && static_cast<long long>(max_q_len) * G <= kTcRows / 2;
+  pl.tile_rows = tc ? (pl.dup ? kTcRows / 2 : kTcRows) / G * G : kRows;
+  pl.group_rows = tc ? (pl.dup ? 1 : 2) * pl.tile_rows : kRows;
   const int key_tiles = (max_ctx + keys - 1) / keys;
   // a share of fewer key tiles would pay more for its joining than it saves
   pl.min_share = key_tiles < kMinShare ? key_tiles : kMinShare;
@@ -1492,7 +1544,7 @@ bool make_cache_map(CUtensorMap* map, const void* base, bool bf16, long long row
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool DUP>
 int launch_tc(TreeParams& p, cudaStream_t s) {
   CUtensorMap qm, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -1509,7 +1561,7 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
     return PS_ERR_CUDA;
   }
-  auto kern = tree_tc_kernel<T, D>;
+  auto kern = tree_tc_kernel<T, D, DUP>;
   static std::atomic<uint64_t> done{0};
   if (!ps_host::reserve_smem(reinterpret_cast<const void*>(kern), Tc<D>::kSmem, &done)) {
     ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
@@ -1519,6 +1571,11 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   ps_host::count_launch();
   const int rc = ps_host::check_launch("tree_attention");
   return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
+}
+
+template <typename T, int D>
+int launch_tc(TreeParams& p, cudaStream_t s, bool dup) {
+  return dup ? launch_tc<T, D, true>(p, s) : launch_tc<T, D, false>(p, s);
 }
 
 }  // namespace
@@ -1642,8 +1699,8 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pl.tc) {
     if (dtype == PS_BF16)
-      return D == 128 ? launch_tc<__nv_bfloat16, 128>(p, s) : launch_tc<__nv_bfloat16, 64>(p, s);
-    return D == 128 ? launch_tc<__half, 128>(p, s) : launch_tc<__half, 64>(p, s);
+      return D == 128 ? launch_tc<__nv_bfloat16, 128>(p, s, pl.dup) : launch_tc<__nv_bfloat16, 64>(p, s, pl.dup);
+    return D == 128 ? launch_tc<__half, 128>(p, s, pl.dup) : launch_tc<__half, 64>(p, s, pl.dup);
   }
   if (dtype == PS_BF16)
     return D == 128 ? launch_mma<__nv_bfloat16, 128>(p, s) : launch_mma<__nv_bfloat16, 64>(p, s);

@@ -591,6 +591,18 @@ def test_attention_blocks_of_several_boxes(dev, bs, Hq, Hkv, D):
     _check_large(_case(29, [bs - 1, 500, 3 * bs, 1], [7, 20, 1, 3], Hq, Hkv, D, bs, torch.bfloat16), dev)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 1, 128), (14, 2, 64), (40, 8, 128), (64, 1, 64), (3, 1, 128), (33, 1, 64)])
+@pytest.mark.parametrize("rows", [64, 65])
+def test_attention_small_row_groups(dev, rows, Hq, Hkv, D):
+    """On both sides of the bound where rows are doubled, with requests of fewer
+    rows, of none and contexts that end anywhere in a tile or are cut."""
+    G = Hq // Hkv
+    n = max(1, rows // G) + (rows == 65)
+    ctxs = [2000, 0, 127, 128, 31, 32, 64, 5000, 96]
+    nodes = [n, n, max(1, n - 1), 1, n, 0, n, n, max(1, n // 2)]
+    _check_large(_case(30, ctxs, nodes, Hq, Hkv, D, 16, torch.bfloat16, kind="star"), dev)
+
+
 def test_attention_without_work(dev):
     """Requests that all wait: nothing is written."""
     from pageserve_b200 import speculative as sp
