@@ -60,8 +60,7 @@ struct TreeParams {
   int num_ctas;
   int min_share;   // fewest key tiles worth a CTA
   int never_cut;   // by the call's bounds no row group is cut: there is nothing to join
-  int tile_rows;   // query rows per tile
-  int group_rows;  // query rows per work item: one tile or two
+  int group_rows;  // query rows per work item
   uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
   int box_shift;   // log2 of the keys per TMA box
   int block_shift; // log2 of the block size, or -1
@@ -542,25 +541,27 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 //              alone streamed 4.9 TB/s from HBM with one warp, 5.95 with two), so
 //              a box carries both 64-dim panels of its keys
 //   warp 2     walks the CTA's share and hands its segments to the other roles
-//   warp 1     TMEM, the Q tiles (128 / G nodes x the G heads of the group, one
-//              box per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in
-//              shared memory), O_w += P_w V_j (P from TMEM, V read MN-major), all
-//              by one thread
+//   warp 1     TMEM, the Q tile (128 / G nodes x the G heads of the group, one box
+//              per 64 dims) and the MMAs: S_w = Q K_j^T (both operands in shared
+//              memory), O += P_w V_j (P from TMEM, V read MN-major), all by one thread
 //   warps 4-11 softmax, two threads per row (DUP: four): warps 4-7 the first 64
 //              keys of a tile, warps 8-11 the others; a pair of warps exchanges its
 //              rows' maxima, so that both halves of P refer to the same one
-// Step t is a key tile (of one row tile, up to 128 rows) or a key tile and one of
-// two row tiles in turn, which then share every loaded tile: QK(t), softmax(t),
-// PV(t). The MMA thread issues PV(t) QK(t + 2) under softmax(t + 1), with one
-// commit: what a commit costs the pipe is about one MMA, so ring slots are given
-// back by a softmax thread, for which S(t) complete says that K of step t and V of
-// step t - 2 have been read (MMAs complete in order).
+// Step t is a key tile: QK(t), softmax(t), PV(t). The MMA thread issues PV(t)
+// QK(t + 2) under softmax(t + 1), with one commit: what a commit costs the pipe is
+// about one MMA, so ring slots are given back by a softmax thread, for which S(t)
+// complete says that K of step t and V of step t - 2 have been read (MMAs complete
+// in order).
 // A step lasts about 2300 clocks of the softmax warps (200 the largest scores, 200
 // their exchange, 1430 exponentials and P, of which the special-function unit
 // takes 1024), under which lie 1420 of the matrix unit. One thread per row and
 // two groups of warps on alternate steps took 2500; looking for step t + 1's
 // largest scores under step t's exponentials was no faster, for S(t + 1) is not
-// there yet (and a third S does not fit beside two O).
+// there yet. Two row tiles that share each loaded key tile (128 x 2 rows, two O)
+// were slower wherever they applied, for the partials of cut row groups doubled:
+// 8 requests of up to 64 nodes 32.7 against 27.2 us, one of 33 nodes at context
+// 32717 63.1 against 58.4, 64 of up to 64 nodes at 4096 148 against 138; the
+// second reader of a key tile finds it in L2.
 // DUP: calls whose row groups have at most 64 rows by their bounds load them into
 // both halves of the tile, lanes r and r + 64. Of every 64 keys lane r's P has the
 // first 32 and zeros, lane r + 64's the others: four threads per row, each with a
@@ -570,8 +571,8 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 // 35.6 -> 33.6 (copies of K and V alone at this pattern and these CTAs: within 10%).
 // A softmax thread reads its scores from TMEM 32 at a time: holding them would
 // need more than the 168 registers that 12 warps leave a thread.
-// TMEM: S0 | S1 | O0 | O1 (the second row tile's), 128 columns each; the halves
-// of P overwrite the first 32 columns of the halves of S.
+// TMEM: S0 | S1 | O, 128 columns each; the halves of P overwrite the first 32
+// columns of the halves of S.
 // The ring and the barriers run on over the segments of a CTA's share: the next
 // segment's tiles load while the last one's output is stored.
 constexpr int kTcRows = 128;
@@ -580,14 +581,15 @@ constexpr int kTcThreads = 384;
 constexpr int kTcCtas = 148;
 constexpr int kMinShare = 4;
 
-template <int D>
+template <int D, bool DUP>
 struct Tc {
   static constexpr int kPanels = D / 64;                // 64-column panels of 128 rows x 128 bytes
   static constexpr int kGroup = kPanels * 1024;         // 8 keys of a K or V tile: panel after panel
   static constexpr int kSlot = kTcKeys * D * 2;         // one K or V tile
   static constexpr int kQ = kTcRows * D * 2;
-  static constexpr int kSlots = (224 * 1024 - 2 * kQ) / kSlot;  // 5 (D = 128) or 12 (D = 64)
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 3072 /* barriers, (max, sum), flags */;
+  static constexpr int kQs = DUP ? 2 * kQ : kQ;         // (and what DUP's lanes exchange)
+  static constexpr int kSlots = (224 * 1024 - kQs) / kSlot;  // 5 or 6 (D = 128), 12 or 13 (D = 64)
+  static constexpr int kSmem = kQs + kSlots * kSlot + 3072 /* barriers, (max, sum), flags */;
 };
 
 // 128B-swizzled descriptor of a K or V tile: groups of 8 keys sbo bytes apart,
@@ -777,15 +779,15 @@ PS_DEVICE void drain_wait(uint32_t bar, uint32_t parity) {
 
 // Order of a segment's loads, K_j and V_j among its 2 * nt tiles: as the MMAs
 // read them, QK two steps ahead of PV.
-PS_DEVICE int k_pos(int j, bool two) { return two ? 2 * j : (j < 2 ? j : 2 * j - 1); }
-PS_DEVICE int v_pos(int j, int nt, bool two) { return two ? 2 * j + 1 : min(nt, j + 2) + j; }
+PS_DEVICE int k_pos(int j) { return j < 2 ? j : 2 * j - 1; }
+PS_DEVICE int v_pos(int j, int nt) { return min(nt, j + 2) + j; }
 
 // A segment as the roles read it.
 struct Seg {
   int b, q0, n, start, h, row0, rows, tile0, nt;
   int flags;
 };
-enum SegFlags : int { kSegStop = 1, kSegWhole = 2, kSegTwo = 4 };
+enum SegFlags : int { kSegStop = 1, kSegWhole = 2 };
 constexpr int kSegRing = 4;
 constexpr int kSegReaders = 11;  // two producers, the MMA thread, eight softmax warps
 
@@ -821,7 +823,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
                                                                 const __grid_constant__ CUtensorMap vmap,
                                                                 const TreeParams p) {
   pdl_trigger();
-  using C = Tc<D>;
+  using C = Tc<D, DUP>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kNS = C::kSlots;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -832,7 +834,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     if (threadIdx.x == 0) record_error(p.status, kErrShape);
     return;
   }
-  const uint32_t ring = q_sa + 2 * C::kQ;
+  const uint32_t ring = q_sa + C::kQs;
   const uint32_t bars = ring + kNS * C::kSlot;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (kNS + s); };
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   auto seg_full = [&](int i) { return bars + 8 * (2 * kNS + 11 + i); };
   auto seg_empty = [&](int i) { return bars + 8 * (2 * kNS + 11 + kSegRing + i); };
   auto cross = [&](int i) { return bars + 8 * (2 * kNS + 11 + 2 * kSegRing + i); };
-  unsigned char* misc = gbase + 2 * C::kQ + kNS * C::kSlot + 8 * (2 * kNS + 14 + 2 * kSegRing);
+  unsigned char* misc = gbase + C::kQs + kNS * C::kSlot + 8 * (2 * kNS + 14 + 2 * kSegRing);
   float* s_swap = reinterpret_cast<float*>(misc);  // [2][2 halves][128 rows]
   Seg* s_seg = reinterpret_cast<Seg*>(misc + 2 * 128 * 8);  // [kSegRing]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_seg + kSegRing);
@@ -888,14 +890,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
   pdl_wait();  // barriers, TMEM and descriptors are ready before the kernel ahead ends
   Share<kTcKeys> share;
   if (warp == 2) {
-    share.find(p, lane, reinterpret_cast<Seq*>(gbase + 2 * C::kQ), kNS * C::kSlot / static_cast<int>(sizeof(Seq)));
+    share.find(p, lane, reinterpret_cast<Seq*>(gbase + C::kQs), kNS * C::kSlot / static_cast<int>(sizeof(Seq)));
     fence_proxy_async();  // the ring is TMA's from here on
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int tile_nodes = p.tile_rows / p.G;
 
   // segment i for a reading warp; false: there is none, or a wait gave up
   auto read_seg = [&](uint32_t i, Seg& sg) {
@@ -920,7 +921,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         if (more) {
           sg = Seg{c.b, c.q0, c.n, c.start, c.h, c.row0, c.rows, c.tile0, c.nt, 0};
           if (c.whole) sg.flags |= kSegWhole;
-          if (c.rows > p.tile_rows) sg.flags |= kSegTwo;
           if (c.tile0 > 0) p.parts[blockIdx.x] = share.part(c);
         }
         s_seg[i % kSegRing] = sg;
@@ -941,7 +941,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     Seg sg;
     for (uint32_t i = 0; ok && read_seg(i, sg); ++i) {
       const int nt = sg.nt;
-      const bool two = !DUP && (sg.flags & kSegTwo);
       const int ctx = sg.start + sg.n;
       const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
       // row of this lane's box of tile j
@@ -974,16 +973,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         }
         ++at;
       };
-      // K_0 [K_1] V_0 K_2 V_1 ... of one row tile, K_0 V_0 K_1 V_1 ... of two;
-      // rows are looked up about two tiles ahead of their loads
-      const int ahead = two ? 1 : 2;
+      // K_0 [K_1] V_0 K_2 V_1 ...; rows are looked up about two tiles ahead of their loads
       int row0 = row_of(0), row1 = row_of(1), row2 = row_of(2);  // of the tiles j, j + 1, j + 2
       turn(false, row0);
-      if (ok && !two && nt > 1) turn(false, row1);
+      if (ok && nt > 1) turn(false, row1);
       for (int j = 0; ok && j < nt; ++j) {
         const int next = row_of(j + 3);
         turn(true, row0);
-        if (ok && j + ahead < nt) turn(false, two ? row1 : row2);
+        if (ok && j + 2 < nt) turn(false, row2);
         row0 = row1;
         row1 = row2;
         row2 = next;
@@ -1009,41 +1006,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         return !(nx.flags & kSegStop);
       };
       auto load_q = [&] {  // of nx
-        const int copies = DUP || (nx.flags & kSegTwo) ? 2 : 1;
         const int node = nx.q0 + nx.row0 / p.G;
-        mbar_expect_tx(q_full, copies * C::kPanels * p.tile_rows * 128);
-        for (int i = 0; i < copies; ++i)
+        mbar_expect_tx(q_full, (DUP ? 2 : 1) * C::kPanels * p.group_rows * 128);
+        for (int i = 0; i < (DUP ? 2 : 1); ++i)
           for (int pn = 0; pn < C::kPanels; ++pn)
-            tma_load_3d(q_sa + i * (DUP ? 64 * 128 : C::kQ) + pn * (kTcRows * 128), &qmap, q_full, pn * 64, nx.h * p.G,
-                        node + (DUP ? 0 : i * tile_nodes));
+            tma_load_3d(q_sa + i * (64 * 128) + pn * (kTcRows * 128), &qmap, q_full, pn * 64, nx.h * p.G, node);
         ++q_loads;
       };
       bool have = take(0);
       if (have) load_q();
       while (ok && have) {
         const int nt = nx.nt;
-        const bool two = !DUP && (nx.flags & kSegTwo);
-        const int steps = two ? 2 * nt : nt;
         ok = thread_wait(q_full, seg & 1, abort_flag, p.status);
-        // ring slots of the next K (0 1 3 5 .. of one row tile, 0 0 2 2 4 4 .. of two)
-        // and V (2 4 .., 1 apart at the end; 1 1 3 3 ..)
+        // ring slots of the next K (0 1 3 5 ..) and V (2 4 .., 1 apart at the end)
         Slot<kNS> vs = base, ks = base;
-        vs.advance(v_pos(0, nt, two));
+        vs.advance(v_pos(0, nt));
         auto qk = [&](int w) {
-          const uint32_t q = q_sa + (two ? w * C::kQ : 0), k = ring + ks.i * C::kSlot;
+          const uint32_t k = ring + ks.i * C::kSlot;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            mma_f16(tmem + w * 128, smem_desc_sw128(q + (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32),
+            mma_f16(tmem + w * 128, smem_desc_sw128(q_sa + (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32),
                     tile_desc(k + (kk >> 2) * 1024 + (kk & 3) * 32, 0, C::kGroup), id_qk, kk > 0 ? 1u : 0u);
           }
         };
         for (int t = 0; ok && t < 2; ++t) {
-          if (t < steps) {
+          if (t < nt) {
             ok = thread_wait(full(ks.i), ks.phase, abort_flag, p.status);
             if (!ok) break;
             tc_fence_after();
             qk(t);
-            ks.advance(two ? 2 * t : 1 + t);
+            ks.advance(1 + t);
           }
           if (seg == 0) mma_commit(s_full(t));
         }
@@ -1056,9 +1048,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           mma_commit(s_full(1));
         }
 #pragma unroll 1
-        for (int t = 0; ok && t < steps; ++t) {
+        for (int t = 0; ok && t < nt; ++t) {
           const int w = t & 1;
-          const bool more = t + 2 < steps;
+          const bool more = t + 2 < nt;
           const uint32_t bv = full(vs.i), bk = more ? full(ks.i) : bv, bp = p_full(w), pp = tiles[w] & 1;
           const uint32_t pk = more ? ks.phase : vs.phase;
           // usually all are complete: one round of tests
@@ -1069,17 +1061,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           }
           ++tiles[w];
           tc_fence_after();
-          const uint32_t v = ring + vs.i * C::kSlot, o = tmem + 256 + (two ? w * 128 : 0);
-          const uint32_t acc = t < (two ? 2 : 1) ? 0u : 1u;
+          const uint32_t v = ring + vs.i * C::kSlot;
+          const uint32_t acc = t == 0 ? 0u : 1u;
 #pragma unroll
           for (int kk = 0; kk < kTcKeys / 16; ++kk)
-            mma_ts(o, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+            mma_ts(tmem + 256, tmem + w * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
                    tile_desc(v + kk * 2 * C::kGroup, 1024, C::kGroup), id_pv, kk > 0 ? 1u : acc);
           if (more) qk(w);
           mma_commit(s_full(w));  // S(t + 2), and in any case: PV(t) is done
-          const int n = two ? 2 * w : 2;
-          ks.advance(n);
-          vs.advance(two || t < nt - 2 ? n : 1);
+          ks.advance(2);
+          vs.advance(t < nt - 2 ? 2 : 1);
         }
         if (!ok) break;
         base.advance(2 * nt);
@@ -1123,52 +1114,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
     for (uint32_t seg = 0; ok && read_seg(seg, sg); ++seg) {
       const int nt = sg.nt;
       const int n = sg.n, start = sg.start, ctx = start + n;
-      const bool two = !DUP && (sg.flags & kSegTwo);
-      const int steps = two ? 2 * nt : nt;
-      const int node0 = sg.row0 / p.G + r_node;  // of the first row tile
-      const int rows0 = min(sg.rows, p.tile_rows), rows1 = sg.rows - rows0;
+      const int node = sg.row0 / p.G + r_node;
+      const bool row_on = r < sg.rows;
       auto give = [&](uint32_t at) { mbar_arrive(empty(static_cast<int>(at % kNS))); };
-      // S(x) complete (x < steps + 2; from steps on: PV(x - 2) alone)
+      // S(x) complete (x < nt + 2; from nt on: PV(x - 2) alone)
       auto wait_s = [&](int x) {
         return warp_wait(s_full(x & 1), (phase[x & 1] + (x >> 1)) & 1, abort_flag, p.status);
       };
       auto give_of = [&](int x) {  // what S(x) says has been read
-        if (!gives || (two && !(x & 1))) return;
-        const int j = two ? x >> 1 : x, back = two ? 1 : 2;
-        if (x < steps) give(seq + k_pos(j, two));
-        if (j >= back) give(seq + v_pos(j - back, nt, two));
+        if (!gives) return;
+        if (x < nt) give(seq + k_pos(x));
+        if (x >= 2) give(seq + v_pos(x - 2, nt));
       };
       // s_odd of the next segment: last read two segments ago, next written after this segment's PVs
       if (gives) s_odd[(seg + 1) % 3] = 0;
       // a row of one mask word is fetched before it is needed
       const bool in_tree = (sg.tile0 + nt) * kTcKeys > start;
       auto mask_row = [&](int node) { return p.mask + static_cast<long long>(sg.q0 + node) * p.words; };
-      unsigned long long mword = in_tree && r < rows0 ? mask_row(node0)[0] : 0ull;
-      unsigned long long mword_b = in_tree && r < rows1 ? mask_row(node0 + tile_nodes)[0] : 0ull;
-      // the reference max (log2 domain) and the sum of the row of the step's tile; _b: the other tile's
-      float m_ref = -FLT_MAX, l = 0.f, m_b = -FLT_MAX, l_b = 0.f;
-      for (int t = 0; t < steps; ++t) {
-        const int w = t & 1, tile = two ? w : 0;
-        const int j = two ? t >> 1 : t;
-        const int key0 = (sg.tile0 + j) * kTcKeys;
+      const unsigned long long mword = in_tree && row_on ? mask_row(node)[0] : 0ull;
+      float m_ref = -FLT_MAX, l = 0.f;  // the reference max (log2 domain) and the sum of this row
+      for (int t = 0; t < nt; ++t) {
+        const int w = t & 1;
+        const int key0 = (sg.tile0 + t) * kTcKeys;
         const bool tail = key0 + kTcKeys > start;
-        const bool row_on = r < (tile ? rows1 : rows0);
         ok = wait_s(t);
         if (!ok) break;
         give_of(t);
-        if (tail && tile == 0) {
+        if (tail) {
           // V rows past the context hold anything, and a drafted row's values
           // that are not finite would reach rows that do not see it: clear them.
           // (S(t) is there, so the slot's last tile has been read and the wait
           // below is for this V's phase and no earlier one.)
-          const uint32_t at = seq + v_pos(j, nt, two);
+          const uint32_t at = seq + v_pos(t, nt);
           const int s = static_cast<int>(at % kNS);
           ok = warp_wait(full(s), (at / kNS) & 1, abort_flag, p.status);
           if (!ok) break;
           const int row = t_lane, key = key0 + row;
           if (key >= start) {
             bool bad = false;
-            unsigned char* line = gbase + 2 * C::kQ + s * C::kSlot + (row >> 3) * C::kGroup + (row & 7) * 128;
+            unsigned char* line = gbase + C::kQs + s * C::kSlot + (row >> 3) * C::kGroup + (row & 7) * 128;
             constexpr int kChunks = 8 * C::kPanels / 2;  // 16-byte chunks for each of a row's threads
 #pragma unroll 1
             for (int k = 0; k < kChunks; ++k) {
@@ -1185,7 +1169,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           fence_proxy_async();
         }
         tc_fence_after();
-        if (first_row < (tile ? rows1 : rows0)) {
+        if (first_row < sg.rows) {
           const uint32_t t_s = tmem + w * 128 + half * 64 + lane_off;
           uint32_t v0 = 0, v1 = 0;
           if (tail) {
@@ -1193,7 +1177,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             const unsigned long long v =
                 !row_on ? 0ull
                         : (p.words == 1 ? seen64(&mword, 1, off, n)
-                                        : seen64(mask_row(node0 + (tile ? tile_nodes : 0)), p.words, off, n));
+                                        : seen64(mask_row(node), p.words, off, n));
             v0 = static_cast<uint32_t>(v);
             v1 = static_cast<uint32_t>(v >> 32);
           }
@@ -1214,12 +1198,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
             const float a = pow2_down(m_new - m_ref);
             l *= a;
             m_ref = m_new;
-            if (t >= (two ? 2 : 1)) {
-              // of one row tile, PV(t - 1) may still be adding to O: S(t + 1) comes after it
-              if (!two) ok = wait_s(t + 1);
+            if (t > 0) {
+              ok = wait_s(t + 1);  // PV(t - 1) may still be adding to O: S(t + 1) comes after it
               if (!ok) break;
               tc_fence_after();
-              scale_o(tmem + 256 + tile * 128 + half * (D / 2) + lane_off, D / 64, a);
+              scale_o(tmem + 256 + half * (D / 2) + lane_off, D / 64, a);
             }
           }
           l += tail ? softmax_part<T, kN, true>(t_n, t_p, v0, v1, p.scale_log2, m_ref)
@@ -1233,121 +1216,104 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(w));
-        if (two) {  // the next step is the other tile's
-          const float m = m_ref, ll = l;
-          const unsigned long long mw = mword;
-          m_ref = m_b;
-          l = l_b;
-          mword = mword_b;
-          m_b = m;
-          l_b = ll;
-          mword_b = mw;
-        }
       }
       if (!ok) break;
-      ok = wait_s(steps);
+      ok = wait_s(nt);
       if (!ok) break;
-      give_of(steps);
-      ok = wait_s(steps + 1);
+      give_of(nt);
+      ok = wait_s(nt + 1);
       if (!ok) break;
-      give_of(steps + 1);
-      phase[0] += (steps + 3) >> 1;
-      phase[1] += (steps + 2) >> 1;
+      give_of(nt + 1);
+      phase[0] += (nt + 3) >> 1;
+      phase[1] += (nt + 2) >> 1;
       tc_fence_after();
       const bool whole = sg.flags & kSegWhole;
       const int slot = sg.tile0 > 0 ? 0 : 1;
-      for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
-        const int rows = tile ? rows1 : rows0;
-        if (first_row < rows) {  // this thread's half (DUP: quarter) of its row's columns
-          float m = tile ? m_b : m_ref;
-          float lt = tile ? l_b : l;
-          lt += swap(lt);
+      if (first_row < sg.rows) {  // this thread's half (DUP: quarter) of its row's columns
+        float m = m_ref, lt = l + swap(l);
+        if (!ok) break;
+        constexpr int kCols = DUP ? D / 4 : D / 2;  // it stores, kChunk at a time
+        constexpr int kChunk = kCols < 32 ? kCols : 32;
+        const int col0 = half * (D / 2) + side * (D / 4);
+        const uint32_t t_o = tmem + 256 + lane_off;
+        float o[32], f = 1.f;
+        if (DUP) {
+          // Both sides' sums and half of each side's O change hands through the
+          // room behind Q; the next segment's S comes after everyone's o_free.
+          float* x = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + side) * kCols) * 64 + r;
+          tmem_ld32(t_o + half * (D / 2) + (D == 128 ? (side ^ 1) * 32 : 0), o);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) x[i * 64] = D == 128 ? o[i] : (side ? o[i] : o[i + 32 - kCols]);
+          float* at = s_swap + (swaps & 1) * 256 + t_lane;  // (the pair's next buffer)
+          at[half * 128] = half ? lt : m;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(cross(quarter & 1));
+          ok = warp_wait(cross(quarter & 1), crosses++ & 1, abort_flag, p.status);
           if (!ok) break;
-          const bool row_on = r < rows;
-          const int lr = tile * p.tile_rows + r, node = node0 + tile * tile_nodes;
-          constexpr int kCols = DUP ? D / 4 : D / 2;  // it stores, kChunk at a time
-          constexpr int kChunk = kCols < 32 ? kCols : 32;
-          const int col0 = half * (D / 2) + side * (D / 4);
-          const uint32_t t_o = tmem + 256 + tile * 128 + lane_off;
-          float o[32], f = 1.f;
-          if (DUP) {
-            // Both sides' sums and half of each side's O change hands through the
-            // unused second Q tile; the next segment's S comes after everyone's o_free.
-            float* x = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + side) * kCols) * 64 + r;
-            tmem_ld32(t_o + half * (D / 2) + (D == 128 ? (side ^ 1) * 32 : 0), o);
+          const float* other = s_swap + (swaps & 1) * 256 + (t_lane ^ 64);
+          const float m2 = other[0], l2 = other[128];
+          const float m1 = m;
+          m = fmaxf(m1, m2);
+          f = exp2f(m1 - m);  // NaN if a max is
+          const float f2 = exp2f(m2 - m);
+          lt = lt * f + l2 * f2;
+          if (D == 128) tmem_ld32(t_o + col0, o);
+          const float* y = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + (side ^ 1)) * kCols) * 64 + r;
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) x[i * 64] = D == 128 ? o[i] : (side ? o[i] : o[i + 32 - kCols]);
-            float* at = s_swap + (swaps & 1) * 256 + t_lane;  // (the pair's next buffer)
-            at[half * 128] = half ? lt : m;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(cross(quarter & 1));
-            ok = warp_wait(cross(quarter & 1), crosses++ & 1, abort_flag, p.status);
-            if (!ok) break;
-            const float* other = s_swap + (swaps & 1) * 256 + (t_lane ^ 64);
-            const float m2 = other[0], l2 = other[128];
-            const float m1 = m;
-            m = fmaxf(m1, m2);
-            f = exp2f(m1 - m);  // NaN if a max is
-            const float f2 = exp2f(m2 - m);
-            lt = lt * f + l2 * f2;
-            if (D == 128) tmem_ld32(t_o + col0, o);
-            const float* y = reinterpret_cast<float*>(gbase + C::kQ) + ((half * 2 + (side ^ 1)) * kCols) * 64 + r;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i)
-              o[i] = (D == 128 ? o[i] : (side ? o[i + 32 - kCols] : o[i])) * f + y[i * 64] * f2;
-            f = 1.f;
-          }
-          if (whole) f = lt == 0.f ? 0.f : 1.f / lt;
-          T* dst = static_cast<T*>(p.out) +
-                   (static_cast<long long>(sg.q0 + node) * p.Hq + sg.h * p.G + r_head) * D + col0;
+          for (int i = 0; i < kCols; ++i)
+            o[i] = (D == 128 ? o[i] : (side ? o[i + 32 - kCols] : o[i])) * f + y[i * 64] * f2;
+          f = 1.f;
+        }
+        if (whole) f = lt == 0.f ? 0.f : 1.f / lt;
+        T* dst = static_cast<T*>(p.out) +
+                 (static_cast<long long>(sg.q0 + node) * p.Hq + sg.h * p.G + r_head) * D + col0;
 #pragma unroll 1
-          for (int c = 0; c < kCols / kChunk; ++c) {
-            if (!DUP) tmem_ld32(t_o + col0 + c * 32, o);
+        for (int c = 0; c < kCols / kChunk; ++c) {
+          if (!DUP) tmem_ld32(t_o + col0 + c * 32, o);
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) o[i] *= f;
-            if (row_on) {
-              // a store of a warp's 32 rows to out touches a line each: the wider the better
-              if (!whole) {
+          for (int i = 0; i < kChunk; ++i) o[i] *= f;
+          if (row_on) {
+            // a store of a warp's 32 rows to out touches a line each: the wider the better
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < kChunk / 8; ++i)
-                  st_global_32(part_o(p, blockIdx.x, slot, lr, (col0 >> 3) + c * 4 + i, D),
-                               reinterpret_cast<const uint32_t*>(o + 8 * i));
-              } else if (p.out32) {
+              for (int i = 0; i < kChunk / 8; ++i)
+                st_global_32(part_o(p, blockIdx.x, slot, r, (col0 >> 3) + c * 4 + i, D),
+                             reinterpret_cast<const uint32_t*>(o + 8 * i));
+            } else if (p.out32) {
 #pragma unroll
-                for (int i = 0; i < kChunk; i += 16) {
-                  uint32_t v[8];
+              for (int i = 0; i < kChunk; i += 16) {
+                uint32_t v[8];
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
-                  st_global_32(dst + c * 32 + i, v);
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < kChunk; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o + i);
+                for (int e = 0; e < 8; ++e) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
+                st_global_32(dst + c * 32 + i, v);
               }
+            } else {
+#pragma unroll
+              for (int i = 0; i < kChunk; i += 8) *reinterpret_cast<uint4*>(dst + c * 32 + i) = pack8<T>(o + i);
             }
           }
-          if (!whole && row_on && half == 0 && side == 0) *part_ml(p, blockIdx.x, slot, lr) = make_float2(m, lt);
-          if (s_odd[seg % 3] != 0 && row_on) {
-            // the cleared values, added to what this thread has stored for a row that sees them
-            const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
-            const unsigned long long* mrow = mask_row(node);
-            const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
+        }
+        if (!whole && row_on && half == 0 && side == 0) *part_ml(p, blockIdx.x, slot, r) = make_float2(m, lt);
+        if (s_odd[seg % 3] != 0 && row_on) {
+          // the cleared values, added to what this thread has stored for a row that sees them
+          const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
+          const unsigned long long* mrow = mask_row(node);
+          const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
 #pragma unroll 1
-            for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
-              const int jn = key - start;
-              if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
-              const int phys = table[key / p.block_size];
-              if (phys < 0 || phys >= p.num_blocks) continue;
-              const T* vr = static_cast<const T*>(p.v_cache) +
-                            ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
-                            col0;
+          for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
+            const int jn = key - start;
+            if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
+            const int phys = table[key / p.block_size];
+            if (phys < 0 || phys >= p.num_blocks) continue;
+            const T* vr = static_cast<const T*>(p.v_cache) +
+                          ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
+                          col0;
 #pragma unroll 1
-              for (int i = 0; i < kCols; ++i) {
-                const T x = vr[i];
-                if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
-                if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
-                else part_o(p, blockIdx.x, slot, lr, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
-              }
+            for (int i = 0; i < kCols; ++i) {
+              const T x = vr[i];
+              if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
+              if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
+              else part_o(p, blockIdx.x, slot, r, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
             }
           }
         }
@@ -1454,7 +1420,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
 // ------------------------------------------------------------------- host --
 struct Plan {
   bool tc, dup, never_cut;
-  int tile_rows, group_rows, ctas, min_share;
+  int group_rows, ctas, min_share;
   double items;  // bound of the call's work items
   size_t bytes;
 };
@@ -1470,8 +1436,7 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   const int G = Hq / Hkv, keys = tc ? kTcKeys : kKeys;
   pl.tc = tc;
   pl.dup = tc && static_cast<long long>(max_q_len) * G <= kTcRows / 2;
-  pl.tile_rows = tc ? (pl.dup ? kTcRows / 2 : kTcRows) / G * G : kRows;
-  pl.group_rows = tc ? (pl.dup ? 1 : 2) * pl.tile_rows : kRows;
+  pl.group_rows = tc ? (pl.dup ? kTcRows / 2 : kTcRows) / G * G : kRows;
   const int key_tiles = (max_ctx + keys - 1) / keys;
   // a share of fewer key tiles would pay more for its joining than it saves
   pl.min_share = key_tiles < kMinShare ? key_tiles : kMinShare;
@@ -1555,7 +1520,7 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   for (int i = 0; i < 31; ++i)
     if (p.block_size == 1 << i) p.block_shift = i;
   p.out32 = ps_host::aligned(p.out, 32);
-  if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.tile_rows / p.G) ||
+  if (!make_rows_map(&qm, p.q, bf16, p.total_q, p.Hq, D, p.G, p.group_rows / p.G) ||
       !make_cache_map(&km, p.k_cache, bf16, rows, p.Hkv, D, 1 << p.box_shift) ||
       !make_cache_map(&vm, p.v_cache, bf16, rows, p.Hkv, D, 1 << p.box_shift)) {
     ps_host::set_error("tree_attention: cuTensorMapEncodeTiled failed");
@@ -1563,11 +1528,11 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   }
   auto kern = tree_tc_kernel<T, D, DUP>;
   static std::atomic<uint64_t> done{0};
-  if (!ps_host::reserve_smem(reinterpret_cast<const void*>(kern), Tc<D>::kSmem, &done)) {
-    ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D>::kSmem);
+  if (!ps_host::reserve_smem(reinterpret_cast<const void*>(kern), Tc<D, DUP>::kSmem, &done)) {
+    ps_host::set_error("tree_attention: cannot reserve %d bytes of shared memory", Tc<D, DUP>::kSmem);
     return PS_ERR_CUDA;
   }
-  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D>::kSmem, s, qm, km, vm, p);
+  ps_host::launch(kern, p.num_ctas, kTcThreads, Tc<D, DUP>::kSmem, s, qm, km, vm, p);
   ps_host::count_launch();
   const int rc = ps_host::check_launch("tree_attention");
   return rc == PS_OK ? launch_join<T, D>(p, s) : rc;
@@ -1680,10 +1645,9 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.num_ctas = pl.ctas;
   p.min_share = pl.min_share;
   p.never_cut = pl.never_cut;
-  p.tile_rows = pl.tile_rows;
   p.group_rows = pl.group_rows;
   if (pl.tc) {
-    // ceil(n / t), t = group_rows / G <= 256 nodes: exact, since (n + t - 1) * t < 2^20 for n <= 256
+    // ceil(n / t), t = group_rows / G <= 128 nodes: exact, since (n + t - 1) * t < 2^20 for n <= 256
     const uint32_t t = pl.group_rows / p.G;
     p.rg_mul = 1;
     p.rg_add = t - 1;
