@@ -9,7 +9,9 @@
 //   slot(i)  = table[(seq + i) / bs] * bs + (seq + i) % bs
 //   anc(i)   = {i} + anc(parent(i)),  position(i) = seq + |anc(i)| - 1
 //
-// Bound by latency: the bytes are a few kilobytes to a few megabytes. One
+// Bound by latency (captured: 2.9 us for one request, 4.5 for 64 trees of up to 16
+// nodes, 6.2 for 513 requests with tables of 2049 entries, whose 4.2 MB would take
+// 1.0 us): the bytes are a few kilobytes to a few megabytes. One
 // launch, one CTA per request; each CTA sums take and q over the requests
 // before its own, which costs 3 coalesced loads per 256 requests from L2 and
 // needs no second pass, no atomics and no order between CTAs. What does not

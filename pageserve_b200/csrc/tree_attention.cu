@@ -272,8 +272,11 @@ PS_DEVICE bool clear_odd(uint4& x) {
 }
 
 // --------------------------------------------------------- mma.sync kernel --
-// Any block size, head_dim 64 or 128: 64 rows per CTA (16 per warp), 64-key
-// tiles through a 3-stage ring of 16-byte cp.async.
+// Any block size and group: 64 rows per CTA (16 per warp), 64-key tiles through a
+// 3-stage ring of 16-byte cp.async. Bound by its copies' addresses and the MMA
+// chain of four warps: with blocks of 8, which both kernels can read, 64 requests
+// x 8 nodes at 2048 took 85 us (tcgen05: 46, cold L2) and 128 x 16 nodes at 4096
+// with 40 heads 1694 us (370), so it has only what the other cannot take.
 constexpr int kThreads = 128;
 constexpr int kRows = 64;
 constexpr int kKeys = 64;
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
 }
 
 // ----------------------------------------------------------- tcgen05 kernel --
-// Block sizes of whole 16-key groups (the serving layouts). One CTA per SM, 128
+// Block sizes of whole 8-key groups (the serving layouts). One CTA per SM, 128
 // query rows, 128-key tiles:
 //   warps 0, 3 TMA producers of K and of V: tiles go through one ring of equal
 //              slots in the order that the MMAs read them (K0 K1 V0 K2 V1 ...),
@@ -1425,10 +1428,10 @@ struct Plan {
   size_t bytes;
 };
 
-// The tcgen05 kernel takes whole 16-key groups at 32-bit rows and the heads of
-// a group in one tile.
+// The tcgen05 kernel takes blocks of whole 8-key groups (the matrix unit's and its
+// copies' unit) at 32-bit rows and the heads of a group in one tile.
 bool tc_layout(int num_blocks, int block_size, int G) {
-  return block_size % 16 == 0 && (static_cast<long long>(num_blocks) + 1) * block_size < INT32_MAX && G <= kTcRows;
+  return block_size % 8 == 0 && (static_cast<long long>(num_blocks) + 1) * block_size < INT32_MAX && G <= kTcRows;
 }
 
 Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv, int D) {
@@ -1476,8 +1479,7 @@ int launch_mma(TreeParams& p, cudaStream_t s) {
 }
 
 // [rows][heads][D] of 16-bit values in boxes of box_rows x box_heads x 64 dims,
-// 128-byte swizzle: one layer's cache (16 keys of one head) or q (the nodes of
-// a tile, the heads of a group).
+// 128-byte swizzle: q (the nodes of a tile, the heads of a group).
 bool make_rows_map(CUtensorMap* map, const void* base, bool bf16, long long rows, int heads, int D, int box_heads,
                    int box_rows) {
   auto fn = encode_fn();
@@ -1514,7 +1516,7 @@ int launch_tc(TreeParams& p, cudaStream_t s) {
   CUtensorMap qm, km, vm;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const long long rows = static_cast<long long>(p.num_blocks) * p.block_size;
-  p.box_shift = 4;  // the largest power of two of keys that lie together in a block, at most a tile
+  p.box_shift = 3;  // the largest power of two of keys that lie together in a block, at most a tile
   while (p.box_shift < 7 && p.block_size % (2 << p.box_shift) == 0) ++p.box_shift;
   p.block_shift = -1;
   for (int i = 0; i < 31; ++i)
