@@ -592,7 +592,7 @@ struct Tc {
   static constexpr int kQ = kTcRows * D * 2;
   static constexpr int kQs = DUP ? 2 * kQ : kQ;         // (and what DUP's lanes exchange)
   static constexpr int kSlots = (224 * 1024 - kQs) / kSlot;  // 5 or 6 (D = 128), 12 or 13 (D = 64)
-  static constexpr int kSmem = kQs + kSlots * kSlot + 3072 /* barriers, (max, sum), flags */;
+  static constexpr int kSmem = kQs + kSlots * kSlot + 3 * 1024 /* barriers, (max, sum), flags */;
 };
 
 // 128B-swizzled descriptor of a K or V tile: groups of 8 keys sbo bytes apart,
