@@ -639,7 +639,8 @@ class PagedCausalLM:
         (cached tokens), q_lens (rows; 0 waits), held (blocks in its table row)
         int32 (B,); block_tables int32 (B, max_blocks); free_blocks int32: the
         blocks the step may take. max_q_len bounds q_lens (at most 256),
-        max_ctx seq_lens + q_lens (default: what a table row holds). Rows
+        max_ctx seq_lens + q_lens (default: what a table row holds; a closer
+        bound spares short steps the joining of key ranges). Rows
         behind the last request are padding (any token of the vocabulary).
 
         The confirmed tokens of the step are ``accepted.tokens[b,

@@ -17,7 +17,8 @@ the request's cached tokens and its own ancestors.
   agree with and moves its keys and values to the positions they keep.
 
 ``PagedCausalLM.verify_trees`` runs the three around one model pass. All
-lengths stay on the device, so a step can be captured in a CUDA graph.
+lengths stay on the device, so a step can be captured in a CUDA graph (after one
+call outside it).
 """
 
 from __future__ import annotations
