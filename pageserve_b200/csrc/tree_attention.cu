@@ -58,7 +58,6 @@ struct TreeParams {
   int max_ctx;
   int num_seqs;
   int num_ctas;
-  int min_share;   // fewest key tiles worth a CTA
   int never_cut;   // by the call's bounds no row group is cut: there is nothing to join
   int group_rows;  // query rows per work item
   uint32_t rg_mul, rg_add, rg_magic, rg_shift;  // row groups of n nodes: ((n * mul + add) * magic) >> shift
@@ -100,7 +99,10 @@ PS_DEVICE Seq seq_of(const TreeParams& p, int b) {
 // shares cut row groups, which then have to be joined; where whole row groups,
 // an equal number per CTA, take at most kJoinCost key tiles longer, they are not
 // cut (64 sequences x 2 heads at equal contexts: 17 key tiles per CTA against 15
-// and a joining of about 6 us; a key tile takes 1.3 us).
+// and a joining of about 6 us; a key tile takes 1.3 us). A share may be a single
+// key tile: of at least 4, one request of 64 nodes at context 2000 (16 / 2 heads)
+// took 15.3 us instead of 12.9, four of up to 40 nodes at 300 to 2000 20.9 instead
+// of 15.4.
 constexpr int kJoinCost = 4;
 
 struct Cut {  // one segment
@@ -146,7 +148,7 @@ struct Share {
     total = __reduce_add_sync(0xffffffffu, total);
     groups = __reduce_add_sync(0xffffffffu, groups);
     longest = __reduce_max_sync(0xffffffffu, longest);
-    per = max((total + p.num_ctas - 1) / p.num_ctas, p.min_share);
+    per = max((total + p.num_ctas - 1) / p.num_ctas, 1);
     const int whole = (groups + p.num_ctas - 1) / p.num_ctas;
     unit = static_cast<long long>(whole) * longest <= per + kJoinCost;
     const long long lo = static_cast<long long>(unit ? whole : per) * blockIdx.x;
@@ -582,7 +584,6 @@ constexpr int kTcRows = 128;
 constexpr int kTcKeys = 128;
 constexpr int kTcThreads = 384;
 constexpr int kTcCtas = 148;
-constexpr int kMinShare = 4;
 
 template <int D, bool DUP>
 struct Tc {
@@ -1344,7 +1345,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
 // and summed in warp order. 16 row groups of 10 parts (33 nodes at context 32717):
 // the whole call 58.5 us dealt, 57.0 not; 2 of 12 parts and 8 rows: 15.1 and 16.6.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinY = 4;  // blocks per column
+// Blocks of the grid, 4 to 16 per column: with 4 throughout, one request of 64
+// nodes at 2000 (33 CTAs) took 16.5 us instead of 15.5.
+constexpr int kJoinBlocks = 4 * 148;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeParams p) {
@@ -1358,8 +1361,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
   const Part pt = p.parts[c];
   if (pt.c0 < 0) return;
   const int helpers = pt.c1 - pt.c0, parts = helpers + 1;
-  const int units = helpers * kJoinY;  // blocks that share this row group
-  const int unit = (c - pt.c0 - 1) * kJoinY + blockIdx.y;
+  const int units = helpers * gridDim.y;  // blocks that share this row group
+  const int unit = (c - pt.c0 - 1) * gridDim.y + blockIdx.y;
   const int r_begin = pt.rows * unit / units, r_end = pt.rows * (unit + 1) / units;
   // deal a row's parts to the warps
   const bool deal = parts > 2 * kJoinWarps || (parts > kJoinWarps && r_end - r_begin <= 1);
@@ -1426,7 +1429,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
 // ------------------------------------------------------------------- host --
 struct Plan {
   bool tc, dup, never_cut;
-  int group_rows, ctas, min_share;
+  int group_rows, ctas;
   double items;  // bound of the call's work items
   size_t bytes;
 };
@@ -1444,15 +1447,12 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
   pl.dup = tc && static_cast<long long>(max_q_len) * G <= kTcRows / 2;
   pl.group_rows = tc ? (pl.dup ? kTcRows / 2 : kTcRows) / G * G : kRows;
   const int key_tiles = (max_ctx + keys - 1) / keys;
-  // a share of fewer key tiles would pay more for its joining than it saves
-  pl.min_share = key_tiles < kMinShare ? key_tiles : kMinShare;
   const int row_groups = pl.group_rows ? (max_q_len * G + pl.group_rows - 1) / pl.group_rows : 1;
   pl.items = static_cast<double>(num_seqs) * Hkv * row_groups * key_tiles;
-  const double most = pl.items / pl.min_share + 1;
   const int ctas = tc ? kTcCtas : 2 * kTcCtas;
-  pl.ctas = most < ctas ? static_cast<int>(most) : ctas;
+  pl.ctas = pl.items < ctas ? static_cast<int>(pl.items) : ctas;
   // Share::find takes whole row groups if their longest are within kJoinCost of a share
-  pl.never_cut = static_cast<double>(num_seqs) * Hkv * row_groups <= pl.ctas && key_tiles <= pl.min_share + kJoinCost;
+  pl.never_cut = static_cast<double>(num_seqs) * Hkv * row_groups <= pl.ctas && key_tiles <= 1 + kJoinCost;
   const size_t per_cta = 2 * static_cast<size_t>(pl.group_rows) * (D + 2) * sizeof(float) + sizeof(Part);
   pl.bytes = 256 + static_cast<size_t>(pl.ctas) * per_cta;
   return pl;
@@ -1461,7 +1461,9 @@ Plan plan_for(bool tc, int num_seqs, int max_q_len, int max_ctx, int Hq, int Hkv
 template <typename T, int D>
 int launch_join(const TreeParams& p, cudaStream_t s) {
   if (p.num_ctas == 1 || p.never_cut) return PS_OK;
-  ps_host::launch(tree_join_kernel<T, D>, dim3(p.num_ctas - 1, kJoinY), kJoinWarps * 32, 0, s, p);
+  const int y = kJoinBlocks / p.num_ctas;
+  ps_host::launch(tree_join_kernel<T, D>, dim3(p.num_ctas - 1, y < 4 ? 4 : (y > 16 ? 16 : y)), kJoinWarps * 32, 0, s,
+                  p);
   ps_host::count_launch();
   return ps_host::check_launch("tree_attention(join)");
 }
@@ -1648,7 +1650,6 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
   p.max_ctx = max_ctx;
   p.num_seqs = num_seqs;
   p.num_ctas = pl.ctas;
-  p.min_share = pl.min_share;
   p.never_cut = pl.never_cut;
   p.group_rows = pl.group_rows;
   if (pl.tc) {
