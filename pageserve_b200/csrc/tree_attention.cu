@@ -16,7 +16,11 @@
 // What a node does not see does not reach it, NaN and infinities included:
 // masked scores are replaced before the softmax, rows past the context are
 // zero-filled, and a drafted V row with a value that is not finite is cleared
-// from the tile and added back only to the rows that see it.
+// from the tile and given back only to the rows that see it. What a node does
+// see reaches it with a weight above 0, so an infinity is one in the output too:
+// rounded or scaled to 0 a weight would make NaN of it (0 * inf). A row whose
+// output is not finite although its sum is has its V columns looked at again
+// (OddColumns).
 #include <cfloat>
 #include <climits>
 #include <cstdlib>
@@ -273,6 +277,31 @@ PS_DEVICE bool clear_odd(uint4& x) {
   return hit;
 }
 
+// Which of a thread's N columns of V have values that are not finite in the rows
+// that a query row sees, and what their sum is: with weights above 0 and a finite
+// rest the output's value. Only looked for where a tile or an output has shown
+// such a value.
+struct OddColumns {
+  unsigned long long plus = 0, minus = 0, nan = 0;
+  template <typename T>
+  PS_DEVICE void add(int column, T x) {
+    if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) return;
+    const float f = to_f32(x);
+    const unsigned long long bit = 1ull << column;
+    if (f != f) nan |= bit;
+    else if (f > 0.f) plus |= bit;
+    else minus |= bit;
+  }
+  PS_DEVICE bool any(int column) const { return ((plus | minus | nan) >> column) & 1; }
+  PS_DEVICE float value(int column) const {
+    if (((nan | (plus & minus)) >> column) & 1) return NAN;
+    return (plus >> column) & 1 ? INFINITY : -INFINITY;
+  }
+};
+// A finite sum of weights: the row's scores are in order, and a value of its
+// output that is not finite comes from V.
+PS_DEVICE bool finite_sum(float l) { return fabsf(l) <= FLT_MAX; }
+
 // --------------------------------------------------------- mma.sync kernel --
 // Any block size and group: 64 rows per CTA (16 per warp), 64-key tiles through a
 // 3-stage ring of 16-byte cp.async. Bound by its copies' addresses and the MMA
@@ -487,29 +516,35 @@ __global__ void __launch_bounds__(kThreads) tree_mma_kernel(const TreeParams p) 
       l[ri] += __shfl_xor_sync(0xffffffffu, l[ri], 1);
       l[ri] += __shfl_xor_sync(0xffffffffu, l[ri], 2);
     }
-    if (odd_values) {
-      // add the cleared values to the rows that see them
-      const int k0 = max(first_key, sg.start), k1 = min((sg.tile0 + sg.nt) * kKeys, ctx);
-      for (int key = k0; key < k1; ++key) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      float zero = 0.f;  // NaN if a value of this row is not finite
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) zero = fmaf(o[i][2 * hf + e], 0.f, zero);
+      const bool all = zero != 0.f;  // cached values too
+      if (node[hf] < 0 || !finite_sum(l[hf]) || !(odd_values || all)) continue;
+      const unsigned long long* mrow = p.mask + static_cast<long long>(sg.q0 + node[hf]) * p.words;
+      const int k1 = min((sg.tile0 + sg.nt) * kKeys, ctx);
+      OddColumns odd;
+#pragma unroll 1
+      for (int key = all ? first_key : max(first_key, sg.start); key < k1; ++key) {
+        const int jn = key - sg.start;
+        if (jn >= 0 && !((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
         const int phys = table[key / p.block_size];
         if (phys < 0 || phys >= p.num_blocks) continue;
         const T* vr = static_cast<const T*>(p.v_cache) +
                       ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D;
-        const int jn = key - sg.start;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (node[hf] < 0 ||
-              !((p.mask[static_cast<long long>(sg.q0 + node[hf]) * p.words + (jn >> 6)] >> (jn & 63)) & 1))
-            continue;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const T x = vr[i * 8 + 2 * (lane & 3) + e];
-              if (!finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) o[i][2 * hf + e] += to_f32(x);
-            }
-        }
+#pragma unroll 1
+        for (int i = 0; i < D / 8; ++i)
+          for (int e = 0; e < 2; ++e) odd.add(2 * i + e, vr[i * 8 + 2 * (lane & 3) + e]);
       }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (odd.any(2 * i + e)) o[i][2 * hf + e] = odd.value(2 * i + e);
     }
     const int slot = part_slot(sg);
     if (sg.tile0 > 0 && threadIdx.x == 0) p.parts[blockIdx.x] = share.part(sg);
@@ -1269,6 +1304,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           f = 1.f;
         }
         if (whole) f = lt == 0.f ? 0.f : 1.f / lt;
+        float zero = 0.f;  // NaN if one of its values is not finite
         T* dst = static_cast<T*>(p.out) +
                  (static_cast<long long>(sg.q0 + node) * p.Hq + sg.h * p.G + r_head) * D + col0;
 #pragma unroll 1
@@ -1276,6 +1312,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           if (!DUP) tmem_ld32(t_o + col0 + c * 32, o);
 #pragma unroll
           for (int i = 0; i < kChunk; ++i) o[i] *= f;
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) zero = fmaf(o[i], 0.f, zero);
           if (row_on) {
             // a store of a warp's 32 rows to out touches a line each: the wider the better
             if (!whole) {
@@ -1298,27 +1336,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_tc_kernel(const __grid_con
           }
         }
         if (!whole && row_on && half == 0 && side == 0) *part_ml(p, blockIdx.x, slot, r) = make_float2(m, lt);
-        if (s_odd[seg % 3] != 0 && row_on) {
-          // the cleared values, added to what this thread has stored for a row that sees them
+        const bool all = zero != 0.f;  // cached values too
+        if ((all || s_odd[seg % 3] != 0) && row_on && finite_sum(lt)) {
           const int32_t* table = p.tables + static_cast<long long>(sg.b) * p.max_blocks;
           const unsigned long long* mrow = mask_row(node);
-          const int k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
+          const int k0 = sg.tile0 * kTcKeys, k1 = min((sg.tile0 + nt) * kTcKeys, ctx);
+          OddColumns odd;
 #pragma unroll 1
-          for (int key = max(sg.tile0 * kTcKeys, start); key < k1; ++key) {
+          for (int key = all ? k0 : max(k0, start); key < k1; ++key) {
             const int jn = key - start;
-            if (!((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
+            if (jn >= 0 && !((mrow[jn >> 6] >> (jn & 63)) & 1)) continue;
             const int phys = table[key / p.block_size];
             if (phys < 0 || phys >= p.num_blocks) continue;
             const T* vr = static_cast<const T*>(p.v_cache) +
                           ((static_cast<long long>(phys) * p.block_size + key % p.block_size) * p.Hkv + sg.h) * D +
                           col0;
 #pragma unroll 1
-            for (int i = 0; i < kCols; ++i) {
-              const T x = vr[i];
-              if (finite16<T>(*reinterpret_cast<const uint16_t*>(&x))) continue;
-              if (whole) dst[i] = from_f32<T>(to_f32(dst[i]) + to_f32(x));
-              else part_o(p, blockIdx.x, slot, r, (col0 + i) >> 3, D)[(col0 + i) & 7] += to_f32(x);
-            }
+            for (int i = 0; i < kCols; ++i) odd.add(i, vr[i]);
+          }
+#pragma unroll 1
+          for (int i = 0; i < kCols; ++i) {  // over what this thread has stored
+            if (!odd.any(i)) continue;
+            if (whole) dst[i] = from_f32<T>(odd.value(i));
+            else part_o(p, blockIdx.x, slot, r, (col0 + i) >> 3, D)[(col0 + i) & 7] = odd.value(i);
           }
         }
       }
