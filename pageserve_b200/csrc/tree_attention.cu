@@ -1455,6 +1455,26 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreePa
       __syncthreads();
     }
     if (on && (!deal || warp == 0)) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) nan |= acc[i] != acc[i];
+      if (nan && finite_sum(l)) {
+        // An infinity of a part whose weight underflowed became NaN: the value is
+        // the sum of the parts' values that are not finite.
+        float odd[DPL];
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) odd[i] = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < parts; ++k) {
+          const float* src = part_o(p, pt.c0 + k, k == 0, r, lane * DPL / 8, D) + lane * DPL % 8;
+#pragma unroll
+          for (int i = 0; i < DPL; ++i)
+            if (!(fabsf(src[i]) <= FLT_MAX)) odd[i] += src[i];
+        }
+#pragma unroll
+        for (int i = 0; i < DPL; ++i)
+          if (acc[i] != acc[i] && odd[i] != 0.f) acc[i] = odd[i];
+      }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int row = pt.row0 + r;
       T* dst = static_cast<T*>(p.out) +
