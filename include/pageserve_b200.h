@@ -281,7 +281,10 @@ PS_API int ps_sample_topk(int32_t* out_dev, const float* vals_dev, const int32_t
  * slots that got none are -1, held_out counts the blocks that were given, and
  * error 6 is recorded. Lengths below 0, rows past total_tokens, contexts past
  * the table and parents outside [-1, i) are recorded as error 5 and handled as
- * 0, cut off, slot -1 and -1. held_out must not alias held, seq_lens, q_lens. */
+ * 0, cut off, slot -1 and -1. A tree's rows from the first one without a slot on,
+ * and all rows of a request whose context passes the table (ps_tree_attention
+ * leaves it out), get mask 0: ps_accept_trees keeps nothing of them.
+ * held_out must not alias held, seq_lens, q_lens. */
 PS_API int ps_build_step_tables(int32_t* tables_dev, int32_t* held_out_dev, int32_t* cu_q_dev, int32_t* positions_dev,
                                 int32_t* slots_dev, int64_t* tree_mask_dev, int32_t* free_used_dev,
                                 const int32_t* tables_in_dev, const int32_t* held_dev, const int32_t* seq_lens_dev,

@@ -8,6 +8,10 @@
 //   table[j] = old (j < held) | free[first_b + j - held] (j < need) | -1
 //   slot(i)  = table[(seq + i) / bs] * bs + (seq + i) % bs
 //   anc(i)   = {i} + anc(parent(i)),  position(i) = seq + |anc(i)| - 1
+// A tree's rows from the first one on that has no slot get an empty mask, and so
+// do all rows of a request whose context passes the table: the keys of the first
+// are stored nowhere, the second has no attention, and a node whose mask row is
+// empty is never accepted, nor is one behind it.
 //
 // Bound by latency (captured: 2.9 us for one request, 4.5 for 64 trees of up to 16
 // nodes, 6.2 for 513 requests with tables of 2049 entries, whose 4.2 MB would take
@@ -79,6 +83,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
   __shared__ long long s_sum[kThreads / 32][2];
   __shared__ int s_ptr[kMaxNodes];
   __shared__ unsigned long long s_mask[kMaxNodes][kMaxWords];
+  __shared__ int s_seen;  // nodes whose masks are kept
   const int b = blockIdx.x;
   const int tid = threadIdx.x;
   const Span s = span_of(p, b);
@@ -104,6 +109,11 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
     s_sum[tid >> 5][0] = take_before;
     s_sum[tid >> 5][1] = q_before;
   }
+  bool fits = true;  // of thread 0
+  if (tid == 0) {
+    fits = static_cast<long long>(s.seq) + s.q <= static_cast<long long>(p.max_blocks) * p.block_size;
+    s_seen = fits ? kMaxNodes : 0;
+  }
   __syncthreads();
   long long first = 0, cu = 0;
 #pragma unroll
@@ -125,8 +135,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
     p.cu_q[b] = row0;
     int err = kErrNone;
     if (p.seq_lens[b] < 0 || p.q_lens[b] < 0 || p.held_in[b] < 0 || p.held_in[b] > p.max_blocks ||
-        cu_next > T || (p.parents && s.q > p.max_q_len) ||
-        (static_cast<long long>(s.seq) + s.q + p.block_size - 1) / p.block_size > p.max_blocks)
+        cu_next > T || (p.parents && s.q > p.max_q_len) || !fits)
       err = kErrShape;
     else if (given < take)
       err = kErrNoBlocks;
@@ -147,7 +156,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
     else if (j < s.held + given) id = p.free_blocks[first + (j - s.held)];
     int slot = -1;
     if (id >= 0 && id < p.num_blocks) slot = id * p.block_size + static_cast<int>(at % p.block_size);
-    else record_error(p.status, j < s.held + given ? kErrBlockId : (j < s.need ? kErrNoBlocks : kErrShape));
+    else {
+      record_error(p.status, j < s.held + given ? kErrBlockId : (j < s.need ? kErrNoBlocks : kErrShape));
+      if (p.parents) atomicMin(&s_seen, i);
+    }
     p.slots[row0 + i] = slot;
     if (!p.parents) p.positions[row0 + i] = static_cast<int32_t>(at < INT32_MAX ? at : INT32_MAX);
   }
@@ -186,9 +198,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
       for (int w = 0; w < kMaxWords; ++w) depth += __popcll(m[w]);
       const long long at = static_cast<long long>(s.seq) + depth;
       p.positions[row0 + tid] = static_cast<int32_t>(at < INT32_MAX ? at : INT32_MAX);
+      const bool kept = tid < s_seen;  // (complete before the barriers above)
 #pragma unroll
       for (int w = 0; w < kMaxWords; ++w)
-        if (w < p.words) p.mask[static_cast<long long>(row0 + tid) * p.words + w] = m[w];
+        if (w < p.words) p.mask[static_cast<long long>(row0 + tid) * p.words + w] = kept ? m[w] : 0ull;
     }
     // nodes past the limit see nothing and are written nowhere (recorded above)
     for (int i = n + tid; i < row1 - row0; i += kThreads) {

@@ -647,6 +647,8 @@ class PagedCausalLM:
         :accepted.num[b]]``, the same as that many single-token greedy steps
         yield up to the kernels' rounding; the last of them is the next step's
         root. The cache then holds ``accepted.start_pos`` tokens per request.
+        Rows that get no block (a free list that is too short) are not kept, nor
+        rows behind them; a request that cannot store its root yields nothing.
         Nothing is read back to the host, so the call can be captured in a
         CUDA graph after one call outside it. Device errors (a free list that is too
         short, lengths past the bounds) are read by ``_lib.raise_on_device_error``."""

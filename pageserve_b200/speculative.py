@@ -83,7 +83,10 @@ def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables
     256). Without parents the rows are a chunk at seq_len + i. ``out`` takes
     the tables; it may be block_tables itself. A free list that is too short
     leaves -1 entries and slots, free_used above F and device error 6; lengths
-    beyond the given bounds are device error 5 (``_lib.raise_on_device_error``)."""
+    beyond the given bounds are device error 5 (``_lib.raise_on_device_error``).
+    In a tree the rows from the first one without a slot on get mask 0, as do
+    all rows of a request whose context passes its table row, so that
+    :func:`accept_trees` keeps nothing that is not in the cache."""
     _lib.require_cuda(seq_lens)
     if out is None:
         r = _op("build_step_tables")(seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,

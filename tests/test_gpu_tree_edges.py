@@ -6,9 +6,113 @@ import pytest
 import torch
 
 from oracle import tree
-from test_gpu_speculative import _case, _run, _status, dev  # noqa: F401
+from test_gpu_speculative import _case, _i32, _run, _status, dev  # noqa: F401
+from test_gpu_verify_trees import _model, _Requests, near_tie
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------- steps that are not stored whole --
+
+def _greedy(m, prompts, n):
+    """Each prompt's n greedy tokens, one per step."""
+    B, width = len(prompts), 128 // m.block_size
+    tabs = [list(range(b * width, (b + 1) * width)) for b in range(B)]
+    _, nxt = m.forward_batch(np.concatenate(prompts), [len(p) for p in prompts], [0] * B, tabs)
+    out = [[int(x)] for x in nxt.tolist()]
+    for i in range(n - 1):
+        _, nxt = m.forward_batch([t[-1] for t in out], [1] * B, [len(p) + i for p in prompts], tabs)
+        for t, x in zip(out, nxt.tolist()):
+            t.append(x)
+    m.allocate_kv_cache(m.num_blocks, m.block_size)
+    return out
+
+
+def _verify_chains(s, drafts, **kw):
+    """One step of chains: every request's last confirmed token and its draft."""
+    rows, pars, qs = [], [], []
+    for seq, d in zip(s.seqs, drafts):
+        rows += [seq[-1]] + d
+        pars += range(-1, len(d))
+        qs.append(1 + len(d))
+    return s.m.verify_trees(torch.tensor(rows, device=s.dev), torch.tensor(pars, dtype=torch.int32, device=s.dev),
+                            s.cached, torch.tensor(qs, dtype=torch.int32, device=s.dev), s.tables, s.held, s.free,
+                            max(qs), **kw)
+
+
+def _check_sequences(s, prompts):
+    """Every confirmed token is the greedy one of a pass over the sequence."""
+    m, bs = s.m, s.m.block_size
+    m.allocate_kv_cache(m.num_blocks, bs)
+    for seq, p in zip(s.seqs, prompts):
+        lg = m.forward_step(torch.tensor(seq[:-1]), list(range(128 // bs)), 0).float()
+        for i in range(len(p) - 1, len(seq) - 1):
+            assert int(lg[i].argmax()) == seq[i + 1] or near_tie(lg[i], seq[i + 1]), i
+
+
+@pytest.fixture()
+def two_requests(dev):  # noqa: F811
+    """Blocks of 4: request 0 has 8 tokens cached in 2 blocks (its next row
+    needs a third), request 1 has 5 in 2 (room for 3 rows); and what the model
+    goes on with."""
+    m = _model(torch.bfloat16, False, 64, 4)
+    prompts = [np.arange(3, 12), np.arange(40, 46)]
+    likely = _greedy(m, prompts, 12)
+    _status()
+    return _Requests(m, prompts, 8, range(64), dev), prompts, likely
+
+
+def test_verification_with_a_short_free_list(two_requests):
+    """Rows that get no block are stored nowhere: nothing of them is kept, and
+    the next step goes on from what is."""
+    s, prompts, likely = two_requests
+    free, s.free = s.free, s.free[:0]
+    r = _verify_chains(s, [x[:4] for x in likely])
+    assert _status() == 6
+    assert int(r.tables.free_used) == 3  # 13 positions and 10 in blocks of 4: 4 and 3, 2 held each
+    num, start = r.accepted.num.tolist(), r.accepted.start_pos.tolist()
+    assert num[0] == 0 and start[0] == 8 and r.accepted.tokens[0].tolist() == [-1] * 5
+    assert 1 <= num[1] <= 3 and start[1] == 5 + num[1]
+    assert all(p <= h * 4 for p, h in zip(start, r.tables.held.tolist()))
+    s.take(r._replace(tables=r.tables._replace(free_used=torch.zeros(1))))
+    s.free = free
+    for _ in range(2):
+        done = [len(q) - len(p) for q, p in zip(s.seqs, prompts)]
+        r = _verify_chains(s, [x[n:n + 3] for x, n in zip(likely, done)])
+        assert min(r.accepted.num.tolist()) >= 1
+        s.take(r)
+    assert _status() == 0
+    assert s.cached.tolist() == [len(x) - 1 for x in s.seqs]
+    _check_sequences(s, prompts)
+
+
+def test_tables_rows_without_a_slot_see_nothing(dev):  # noqa: F811
+    """Behind the first row without a slot nothing can be kept: masks are 0."""
+    from pageserve_b200 import speculative as sp
+
+    def run(seq, q, tab, held, free, par, mq, **kw):
+        r = sp.build_step_tables(_i32(seq, dev), _i32(q, dev), _i32(tab, dev), _i32(held, dev), _i32(free, dev), 9, 4,
+                                 len(par), parents=_i32(par, dev), max_q_len=mq, **kw)
+        return r.slots.tolist(), [[int(x) & (2 ** 64 - 1) for x in row] for row in r.tree_mask.tolist()], \
+            r.positions.tolist(), _status()
+    # one block for the two that the second request needs
+    slots, mask, pos, e = run([2, 3], [2, 6], [[4, -1, -1], [7, -1, -1]], [1, 1], [5], [-1, 0, -1, 0, 1, 0, 0, 3], 6)
+    assert slots == [18, 19, 31, 20, 21, 22, 23, -1] and e == 6
+    assert [m[0] for m in mask] == [1, 3, 1, 3, 7, 9, 17, 0]
+    assert pos == [2, 3, 3, 4, 5, 4, 4, 5]
+    # a held block outside the pool: rows behind it that have a place count as little
+    slots, mask, pos, e = run([3], [6], [[4, 99, 2]], [3], [], [-1, -1, 0, 1, 0, 2], 6)
+    assert slots == [19, -1, -1, -1, -1, 8] and e == 1
+    assert [m[0] for m in mask] == [1, 0, 0, 0, 0, 0]
+    # past the table: attention leaves the whole request out
+    slots, mask, pos, e = run([6, 1], [3, 2], [[4, 1], [7, -1]], [2, 1], [], [-1, 0, 1, -1, 0], 3)
+    assert slots == [6, 7, -1, 29, 30] and e == 5
+    assert [m[0] for m in mask] == [0, 0, 0, 1, 3]
+    # several words, the rows without a slot in the middle of a warp
+    n = 100
+    slots, mask, pos, e = run([0], [n], [[-1] * 25], [0], range(9), list(range(-1, n - 1)), n)
+    assert e == 6 and slots == list(range(36)) + [-1] * 64
+    assert mask == [[2 ** (i + 1) - 1, 0] for i in range(36)] + [[0, 0]] * 64
 
 
 # ------------------------------------------------- values that are not finite --
