@@ -324,7 +324,10 @@ PS_API int ps_tree_attention(void* out_dev, const void* q_dev, const void* k_cac
  *   [num_seqs][max_q_len] padded with -1, start_out[b] = start_pos[b] + num[b];
  *   in both caches ([num_layers][num_blocks][block_size][num_kv_heads][head_dim],
  *   dtype PS_BF16 / PS_F16 / PS_F32; both NULL: no move) the rows at positions
- *   start + path[k] move to start + k. Rows behind start_out are left over.
+ *   start + path[k] move to start + k. A node whose row or place has no block
+ *   of the pool in the table is recorded (errors 1, 5); with the caches given,
+ *   start_out then counts the nodes before it alone, for the rest is not in the
+ *   cache. Rows behind start_out are left over.
  * num and start_out must not alias start_pos or cu_q, nor the caches each other.
  * max_q_len <= 256. */
 PS_API int ps_accept_trees(int32_t* num_dev, int32_t* nodes_dev, int32_t* out_tokens_dev, int32_t* start_out_dev,

@@ -10,7 +10,8 @@
 // from cache position start + path(k) to start + k. path(k) >= k, so moving
 // in ascending order never overwrites a row that is still to be read, and a
 // thread that owns one 16-byte column of one layer can do it without any
-// other thread.
+// other thread. The cache ends (start_out) before the first node of the path
+// whose row, or whose place, lies in no block of the pool.
 //
 // Bound by latency for few requests (a chain of five dependent loads), by HBM
 // for many: 32 requests moving 6 tokens of 64 layers x 2 x 2 KB rows read and
@@ -59,6 +60,7 @@ __global__ void __launch_bounds__(kThreads) accept_trees_kernel(const AcceptPara
   pdl_trigger();
   __shared__ uint32_t s_ok[kMaxNodes / 32];
   __shared__ int s_best;
+  __shared__ int s_kept;  // path nodes before the first without a block
   __shared__ unsigned long long s_row[kMaxWords];
   __shared__ long long s_src[kMaxNodes], s_dst[kMaxNodes];  // unit offsets in a layer; src < 0: stays
   const int b = blockIdx.y;
@@ -100,7 +102,10 @@ __global__ void __launch_bounds__(kThreads) accept_trees_kernel(const AcceptPara
   if (tid > 0 && tid < n && parent >= 0) ok = p.tokens[q0 + tid] == p.targets[q0 + parent];
   const uint32_t bits = __ballot_sync(0xffffffffu, ok);
   if (lane == 0) s_ok[tid >> 5] = bits;
-  if (tid == 0) s_best = 0;
+  if (tid == 0) {
+    s_best = 0;
+    s_kept = kMaxNodes;
+  }
   __syncthreads();
   bool whole = tid < n && ok;
 #pragma unroll
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) accept_trees_kernel(const AcceptPara
   if (lead) {
     if (tid == 0) {
       p.num[b] = count;
-      p.start_out[b] = start + count;
+      if (!p.k_cache) p.start_out[b] = start + count;
     }
     const long long o = static_cast<long long>(b) * p.max_q_len;
     if (on_path) {
@@ -148,27 +153,30 @@ __global__ void __launch_bounds__(kThreads) accept_trees_kernel(const AcceptPara
   }
   if (!p.k_cache) return;
   if (on_path) {
+    const int32_t* table = p.tables + static_cast<long long>(b) * p.max_blocks;
+    const long long ps = static_cast<long long>(start) + tid, pd = static_cast<long long>(start) + rank;
+    const long long js = ps / p.block_size, jd = pd / p.block_size;
     long long src = -1, dst = -1;
-    if (tid != rank) {
-      const int32_t* table = p.tables + static_cast<long long>(b) * p.max_blocks;
-      const long long ps = static_cast<long long>(start) + tid, pd = static_cast<long long>(start) + rank;
-      const long long js = ps / p.block_size, jd = pd / p.block_size;
-      if (js >= p.max_blocks) {
-        record_error(p.status, kErrShape);
-      } else {
-        const int is = table[js], id = table[jd];
-        if (is < 0 || is >= p.num_blocks || id < 0 || id >= p.num_blocks) {
-          record_error(p.status, kErrBlockId);
-        } else {
-          src = (static_cast<long long>(is) * p.block_size + ps % p.block_size) * p.row_units;
-          dst = (static_cast<long long>(id) * p.block_size + pd % p.block_size) * p.row_units;
-        }
+    bool stored = false;
+    if (js >= p.max_blocks) {
+      record_error(p.status, kErrShape);
+    } else {
+      const int is = table[js], id = table[jd];
+      stored = is >= 0 && is < p.num_blocks && id >= 0 && id < p.num_blocks;
+      if (!stored) {
+        record_error(p.status, kErrBlockId);
+      } else if (tid != rank) {
+        src = (static_cast<long long>(is) * p.block_size + ps % p.block_size) * p.row_units;
+        dst = (static_cast<long long>(id) * p.block_size + pd % p.block_size) * p.row_units;
       }
     }
+    if (!stored) atomicMin(&s_kept, rank);
     s_src[rank] = src;
     s_dst[rank] = dst;
   }
   __syncthreads();
+  count = min(count, s_kept);
+  if (lead && tid == 0) p.start_out[b] = start + count;
   const long long per_tensor = static_cast<long long>(p.num_layers) * p.row_units;
   for (long long u = blockIdx.x * static_cast<long long>(kThreads) + tid; u < 2 * per_tensor;
        u += static_cast<long long>(gridDim.x) * kThreads) {

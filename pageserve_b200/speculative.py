@@ -135,7 +135,9 @@ def accept_trees(tokens: torch.Tensor, targets: torch.Tensor, tree_mask: torch.T
     node (the lowest of them) gives the path; the targets along it are the
     tokens the step yields. With the caches ((L, NB, bs, Hkv, D), or one
     layer's (NB, bs, Hkv, D)) and block_tables, the path's keys and values move
-    in place to the positions start_pos, start_pos + 1, ..."""
+    in place to the positions start_pos, start_pos + 1, ... A node that the
+    table has no block for is a device error (1, 5), and ``start_pos`` of the
+    result ends before it: only what precedes it is in the cache."""
     _lib.require_cuda(tokens)
     return Accepted._make(_op("accept_trees")(tokens, targets, tree_mask, cu_q, start_pos, max_q_len, k_cache, v_cache,
                                               block_tables))

@@ -115,6 +115,35 @@ def test_tables_rows_without_a_slot_see_nothing(dev):  # noqa: F811
     assert mask == [[2 ** (i + 1) - 1, 0] for i in range(36)] + [[0, 0]] * 64
 
 
+def test_acceptance_counts_cached_rows_only(dev):  # noqa: F811
+    """start_pos ends where the table has no block for a row of the path or
+    for its place, whatever the model agrees with."""
+    from pageserve_b200 import speculative as sp
+    sets = tree.ancestors([-1, 0, 0, 2, 3, 4])  # the path 0 2 3 4 5
+    tgt = [1, 9, 2, 3, 4, 5]
+    tok = [0, 8, 1, 2, 3, 4]
+    k = torch.arange(2 * 6 * 2 * 8, dtype=torch.float32, device=dev).view(2, 6, 2, 1, 8)
+
+    def run(start, tab):
+        kc, vc = k.clone(), -k
+        r = sp.accept_trees(torch.tensor(tok, device=dev), _i32(tgt, dev), torch.from_numpy(tree.mask_words(sets, 1)).to(dev),
+                            _i32([0, 6], dev), _i32([start], dev), 6, kc, vc, _i32([tab], dev))
+        assert r.nodes.tolist() == [[0, 2, 3, 4, 5, -1]] and int(r.num) == 5
+        kept = int(r.start_pos) - start
+        want = k.cpu().numpy().copy()
+        tree.move_rows(want, tab, 2, start, [0, 2, 3, 4, 5][:kept])
+        assert np.array_equal(kc.cpu().numpy(), want) and np.array_equal(vc.cpu().numpy(), -want)
+        return kept, _status()
+    assert run(0, [3, 1, 4]) == (5, 0)
+    assert run(2, [5, 3, 1, 4]) == (5, 0)
+    assert run(0, [9, 1, 4]) == (0, 1)      # the root's own block
+    assert run(0, [3, -1, 4]) == (1, 1)     # node 2's
+    assert run(0, [3, 1, 6]) == (3, 1)      # node 4's
+    assert run(1, [3, 1, 0]) == (4, 5)      # node 5 is past the table
+    assert run(5, [9, 9, 2]) == (1, 5)
+    assert run(6, [0, 1, 2]) == (0, 5)
+
+
 # ------------------------------------------------- values that are not finite --
 
 def _with_value(c, dev, places, heads):
