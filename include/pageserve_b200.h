@@ -284,6 +284,8 @@ PS_API int ps_sample_topk(int32_t* out_dev, const float* vals_dev, const int32_t
  * 0, cut off, slot -1 and -1. A tree's rows from the first one without a slot on,
  * and all rows of a request whose context passes the table (ps_tree_attention
  * leaves it out), get mask 0: ps_accept_trees keeps nothing of them.
+ * ps_build_step_tables_bounded treats contexts past max_ctx in the same way, for
+ * a step whose attention is given that bound.
  * held_out must not alias held, seq_lens, q_lens. */
 PS_API int ps_build_step_tables(int32_t* tables_dev, int32_t* held_out_dev, int32_t* cu_q_dev, int32_t* positions_dev,
                                 int32_t* slots_dev, int64_t* tree_mask_dev, int32_t* free_used_dev,
@@ -291,6 +293,13 @@ PS_API int ps_build_step_tables(int32_t* tables_dev, int32_t* held_out_dev, int3
                                 const int32_t* q_lens_dev, const int32_t* free_blocks_dev, const int32_t* parents_dev,
                                 int num_seqs, int total_tokens, int max_q_len, int max_blocks_per_seq, int num_free,
                                 int num_blocks, int block_size, ps_stream_t stream);
+PS_API int ps_build_step_tables_bounded(int32_t* tables_dev, int32_t* held_out_dev, int32_t* cu_q_dev,
+                                        int32_t* positions_dev, int32_t* slots_dev, int64_t* tree_mask_dev,
+                                        int32_t* free_used_dev, const int32_t* tables_in_dev, const int32_t* held_dev,
+                                        const int32_t* seq_lens_dev, const int32_t* q_lens_dev,
+                                        const int32_t* free_blocks_dev, const int32_t* parents_dev, int num_seqs,
+                                        int total_tokens, int max_q_len, int max_blocks_per_seq, int num_free,
+                                        int num_blocks, int block_size, int max_ctx, ps_stream_t stream);
 
 /* Scratch bytes ps_tree_attention needs (any contents; one buffer per stream);
  * 0 for arguments that it rejects. */

@@ -72,6 +72,7 @@ _SIGNATURES = {
     "ps_topk": (c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "ps_sample_topk": (c_int, [_P, _P, _P, _P, _I, _I, c_float, _P]),
     "ps_build_step_tables": (c_int, [_P] * 13 + [_I] * 7 + [_P]),
+    "ps_build_step_tables_bounded": (c_int, [_P] * 13 + [_I] * 8 + [_P]),
     "ps_tree_attention_workspace_size": (c_size_t, [_I, _I, _I, _I, _I, _I]),
     "ps_tree_attention": (c_int, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P,
                                   c_size_t, _P]),

@@ -9,8 +9,8 @@
 //   slot(i)  = table[(seq + i) / bs] * bs + (seq + i) % bs
 //   anc(i)   = {i} + anc(parent(i)),  position(i) = seq + |anc(i)| - 1
 // A tree's rows from the first one on that has no slot get an empty mask, and so
-// do all rows of a request whose context passes the table: the keys of the first
-// are stored nowhere, the second has no attention, and a node whose mask row is
+// do all rows of a request whose context passes the table or the caller's bound:
+// the keys of the first are stored nowhere, the second has no attention, and a node whose mask row is
 // empty is never accepted, nor is one behind it.
 //
 // Bound by latency (captured: 2.9 us for one request, 4.5 for 64 trees of up to 16
@@ -46,6 +46,7 @@ struct TablesParams {
   const int32_t* free_blocks;
   const int32_t* parents;
   int* status;
+  long long max_ctx;  // cached and new tokens of a request
   int num_seqs;
   int total_tokens;
   int max_q_len;
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
   }
   bool fits = true;  // of thread 0
   if (tid == 0) {
-    fits = static_cast<long long>(s.seq) + s.q <= static_cast<long long>(p.max_blocks) * p.block_size;
+    fits = static_cast<long long>(s.seq) + s.q <= p.max_ctx;
     s_seen = fits ? kMaxNodes : 0;
   }
   __syncthreads();
@@ -223,13 +224,26 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesParam
 
 }  // namespace
 
-extern "C" int ps_build_step_tables(int32_t* tables, int32_t* held_out, int32_t* cu_q, int32_t* positions,
-                                    int32_t* slots, int64_t* tree_mask, int32_t* free_used, const int32_t* tables_in,
-                                    const int32_t* held, const int32_t* seq_lens, const int32_t* q_lens,
-                                    const int32_t* free_blocks, const int32_t* parents, int num_seqs,
-                                    int total_tokens, int max_q_len, int max_blocks, int num_free, int num_blocks,
-                                    int block_size, ps_stream_t stream) {
-  if (num_seqs <= 0 || total_tokens < 0 || max_blocks <= 0 || num_free < 0 || num_blocks <= 0 || block_size <= 0) {
+extern "C" {
+
+int ps_build_step_tables(int32_t* tables, int32_t* held_out, int32_t* cu_q, int32_t* positions, int32_t* slots,
+                         int64_t* tree_mask, int32_t* free_used, const int32_t* tables_in, const int32_t* held,
+                         const int32_t* seq_lens, const int32_t* q_lens, const int32_t* free_blocks,
+                         const int32_t* parents, int num_seqs, int total_tokens, int max_q_len, int max_blocks,
+                         int num_free, int num_blocks, int block_size, ps_stream_t stream) {
+  return ps_build_step_tables_bounded(tables, held_out, cu_q, positions, slots, tree_mask, free_used, tables_in, held,
+                                      seq_lens, q_lens, free_blocks, parents, num_seqs, total_tokens, max_q_len,
+                                      max_blocks, num_free, num_blocks, block_size, INT32_MAX, stream);
+}
+
+int ps_build_step_tables_bounded(int32_t* tables, int32_t* held_out, int32_t* cu_q, int32_t* positions,
+                                 int32_t* slots, int64_t* tree_mask, int32_t* free_used, const int32_t* tables_in,
+                                 const int32_t* held, const int32_t* seq_lens, const int32_t* q_lens,
+                                 const int32_t* free_blocks, const int32_t* parents, int num_seqs, int total_tokens,
+                                 int max_q_len, int max_blocks, int num_free, int num_blocks, int block_size,
+                                 int max_ctx, ps_stream_t stream) {
+  if (num_seqs <= 0 || total_tokens < 0 || max_blocks <= 0 || num_free < 0 || num_blocks <= 0 || block_size <= 0 ||
+      max_ctx < 0) {
     ps_host::set_error("build_step_tables: invalid sizes (seqs %d, tokens %d, table width %d, free %d, pool %d x %d)",
                        num_seqs, total_tokens, max_blocks, num_free, num_blocks, block_size);
     return PS_ERR_INVALID;
@@ -267,6 +281,8 @@ extern "C" int ps_build_step_tables(int32_t* tables, int32_t* held_out, int32_t*
   p.free_blocks = free_blocks;
   p.parents = parents;
   p.status = ps_host::status_word(PS_TU_TREE);
+  const long long capacity = static_cast<long long>(max_blocks) * block_size;
+  p.max_ctx = max_ctx < capacity ? max_ctx : capacity;
   p.num_seqs = num_seqs;
   p.total_tokens = total_tokens;
   p.max_q_len = max_q_len;
@@ -279,3 +295,5 @@ extern "C" int ps_build_step_tables(int32_t* tables, int32_t* held_out, int32_t*
   ps_host::count_launch();
   return ps_host::check_launch("build_step_tables");
 }
+
+}  // extern "C"

@@ -648,7 +648,8 @@ class PagedCausalLM:
         yield up to the kernels' rounding; the last of them is the next step's
         root. The cache then holds ``accepted.start_pos`` tokens per request.
         Rows that get no block (a free list that is too short) are not kept, nor
-        rows behind them; a request that cannot store its root yields nothing.
+        rows behind them; a request that cannot store its root, or whose tokens
+        pass max_ctx or its table row, yields nothing.
         Nothing is read back to the host, so the call can be captured in a
         CUDA graph after one call outside it. Device errors (a free list that is too
         short, lengths past the bounds) are read by ``_lib.raise_on_device_error``."""
@@ -662,10 +663,10 @@ class PagedCausalLM:
             raise ValueError(f"verify_trees: tokens on {tokens.device}, the model on {self.device}")
         if T == 0:
             raise ValueError("verify_trees: no rows")
-        tabs = build_step_tables(seq_lens, q_lens, block_tables, held, free_blocks, self.num_blocks, self.block_size,
-                                 T, parents=parents, max_q_len=max_q_len)
         if max_ctx is None:
             max_ctx = block_tables.shape[1] * self.block_size
+        tabs = build_step_tables(seq_lens, q_lens, block_tables, held, free_blocks, self.num_blocks, self.block_size,
+                                 T, parents=parents, max_q_len=max_q_len, max_ctx=max_ctx)
         logits = self._forward(tokens, TreeMeta(tabs, seq_lens, max_q_len, max_ctx), None)
         targets = self.next_tokens(logits)
         acc = accept_trees(tokens, targets, tabs.tree_mask, tabs.cu_q, seq_lens, max_q_len, self.k_cache, self.v_cache,

@@ -70,7 +70,7 @@ def _op(name: str):
 def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables: torch.Tensor, held: torch.Tensor,
                       free_blocks: torch.Tensor, num_blocks: int, block_size: int, total_tokens: int,
                       parents: torch.Tensor | None = None, max_q_len: int | None = None,
-                      out: torch.Tensor | None = None) -> StepTables:
+                      out: torch.Tensor | None = None, max_ctx: int | None = None) -> StepTables:
     """Block tables, positions, slots and ancestor masks of one step.
 
     seq_lens, q_lens, held int32 (B,): each request's cached tokens, new tokens
@@ -85,15 +85,17 @@ def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables
     leaves -1 entries and slots, free_used above F and device error 6; lengths
     beyond the given bounds are device error 5 (``_lib.raise_on_device_error``).
     In a tree the rows from the first one without a slot on get mask 0, as do
-    all rows of a request whose context passes its table row, so that
-    :func:`accept_trees` keeps nothing that is not in the cache."""
+    all rows of a request whose context passes its table row or ``max_ctx``
+    (give the bound that :func:`tree_attention` gets), so that
+    :func:`accept_trees` keeps nothing that is not in the cache or that the
+    attention leaves out."""
     _lib.require_cuda(seq_lens)
     if out is None:
         r = _op("build_step_tables")(seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
-                                     total_tokens, parents, max_q_len)
+                                     total_tokens, parents, max_q_len, max_ctx)
     else:
         r = (out, *_op("build_step_tables_out")(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks,
-                                                block_size, total_tokens, parents, max_q_len))
+                                                block_size, total_tokens, parents, max_q_len, max_ctx))
     if parents is None:
         r = (*r[:5], None, r[6])
     return StepTables._make(r)

@@ -294,7 +294,8 @@ using StepOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::T
 StepOut step_tables_call(at::Tensor& out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
                               const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
                               int64_t num_blocks, int64_t block_size, int64_t total_tokens,
-                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len,
+                              c10::optional<int64_t> max_ctx) {
   constexpr const char* what = "build_step_tables";
   const at::Device dev = seq_lens.device();
   metadata(seq_lens, dev, what);
@@ -325,16 +326,16 @@ StepOut step_tables_call(at::Tensor& out, const at::Tensor& seq_lens, const at::
   at::Tensor positions = o.take({T}, at::kInt), slots = o.take({T}, at::kInt), held_out = o.take({B}, at::kInt);
   at::Tensor cu_q = o.take({B + 1}, at::kInt), used = o.take({1}, at::kInt);
   if (!out.defined()) out = o.take(block_tables.sizes(), at::kInt);
-  check_v(ps_build_step_tables(out.data_ptr<int32_t>(), held_out.data_ptr<int32_t>(), cu_q.data_ptr<int32_t>(),
-                               positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
-                               parents.has_value() ? mask.data_ptr<int64_t>() : nullptr, used.data_ptr<int32_t>(),
-                               block_tables.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
-                               seq_lens.data_ptr<int32_t>(), q_lens.data_ptr<int32_t>(),
-                               free_blocks.data_ptr<int32_t>(),
-                               parents.has_value() ? parents->data_ptr<int32_t>() : nullptr, int_arg(B, what),
-                               int_arg(T, what), int_arg(max_q_len.value_or(0), what),
-                               int_arg(block_tables.size(1), what), int_arg(free_blocks.numel(), what),
-                               int_arg(num_blocks, what), int_arg(block_size, what), stream_of(seq_lens)),
+  check_v(ps_build_step_tables_bounded(
+              out.data_ptr<int32_t>(), held_out.data_ptr<int32_t>(), cu_q.data_ptr<int32_t>(),
+              positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
+              parents.has_value() ? mask.data_ptr<int64_t>() : nullptr, used.data_ptr<int32_t>(),
+              block_tables.data_ptr<int32_t>(), held.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+              q_lens.data_ptr<int32_t>(), free_blocks.data_ptr<int32_t>(),
+              parents.has_value() ? parents->data_ptr<int32_t>() : nullptr, int_arg(B, what), int_arg(T, what),
+              int_arg(max_q_len.value_or(0), what), int_arg(block_tables.size(1), what),
+              int_arg(free_blocks.numel(), what), int_arg(num_blocks, what), int_arg(block_size, what),
+              int_arg(max_ctx.value_or(INT32_MAX), what), stream_of(seq_lens)),
           what);
   return {held_out, cu_q, positions, slots, mask, used};
 }
@@ -342,18 +343,19 @@ StepOut step_tables_call(at::Tensor& out, const at::Tensor& seq_lens, const at::
 StepOut build_step_tables_out(at::Tensor out, const at::Tensor& seq_lens, const at::Tensor& q_lens,
                               const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
                               int64_t num_blocks, int64_t block_size, int64_t total_tokens,
-                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+                              const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len,
+                              c10::optional<int64_t> max_ctx) {
   return step_tables_call(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size, total_tokens,
-                          parents, max_q_len);
+                          parents, max_q_len, max_ctx);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_step_tables(
     const at::Tensor& seq_lens, const at::Tensor& q_lens, const at::Tensor& block_tables, const at::Tensor& held,
     const at::Tensor& free_blocks, int64_t num_blocks, int64_t block_size, int64_t total_tokens,
-    const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len) {
+    const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len, c10::optional<int64_t> max_ctx) {
   at::Tensor out;
   auto r = step_tables_call(out, seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size,
-                                 total_tokens, parents, max_q_len);
+                                 total_tokens, parents, max_q_len, max_ctx);
   return {out, std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r), std::get<5>(r)};
 }
 
@@ -502,7 +504,7 @@ std::tuple<at::Tensor, at::Tensor> topk_meta(const at::Tensor& l, int64_t k) {
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_tables_meta(
     const at::Tensor& seq_lens, const at::Tensor&, const at::Tensor& block_tables, const at::Tensor&,
     const at::Tensor&, int64_t, int64_t, int64_t T, const c10::optional<at::Tensor>& parents,
-    c10::optional<int64_t> max_q_len) {
+    c10::optional<int64_t> max_q_len, c10::optional<int64_t>) {
   const auto i32 = seq_lens.options();
   const int64_t B = seq_lens.numel();
   auto mask = parents.has_value() ? at::empty({T, (max_q_len.value_or(0) + 63) / 64}, i32.dtype(at::kLong))
@@ -545,11 +547,12 @@ TORCH_LIBRARY(pageserve_b200, m) {
   m.def("topk(Tensor logits, int k) -> (Tensor, Tensor)");
   m.def("copy_kv_blocks(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor pairs) -> ()");
   m.def("build_step_tables(Tensor seq_lens, Tensor q_lens, Tensor block_tables, Tensor held, Tensor free_blocks, "
-        "int num_blocks, int block_size, int total_tokens, Tensor? parents=None, int? max_q_len=None) "
+        "int num_blocks, int block_size, int total_tokens, Tensor? parents=None, int? max_q_len=None, "
+        "int? max_ctx=None) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("build_step_tables_out(Tensor(a!) out, Tensor seq_lens, Tensor q_lens, Tensor block_tables, Tensor held, "
         "Tensor free_blocks, int num_blocks, int block_size, int total_tokens, Tensor? parents=None, "
-        "int? max_q_len=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "int? max_q_len=None, int? max_ctx=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_q, Tensor start_pos, "
         "Tensor tree_mask, int max_q_len, int max_ctx, Tensor? workspace=None) -> Tensor");
   m.def("tree_attention_out(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "

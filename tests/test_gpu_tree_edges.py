@@ -144,6 +144,30 @@ def test_acceptance_counts_cached_rows_only(dev):  # noqa: F811
     assert run(6, [0, 1, 2]) == (0, 5)
 
 
+def test_verification_past_the_bounds_keeps_nothing(two_requests):
+    """A request whose context passes max_ctx, or its row of the table, is
+    left out by the attention: nothing of it is kept, the others are right."""
+    s, prompts, likely = two_requests
+    r = _verify_chains(s, [x[:4] for x in likely], max_ctx=12)  # contexts 13 and 10
+    assert _status() == 5
+    assert r.accepted.num[0] == 0 and r.accepted.start_pos[0] == 8
+    assert r.accepted.nodes[0].tolist() == [-1] * 5 and r.accepted.tokens[0].tolist() == [-1] * 5
+    assert r.accepted.num[1] >= 1
+    s.take(r)
+    wide, s.tables = s.tables, s.tables[:, :3].contiguous()  # 12 positions
+    done = len(s.seqs[1]) - len(prompts[1])
+    r = _verify_chains(s, [likely[0][:4], likely[1][done:done + 1]])
+    assert _status() == 5
+    assert r.accepted.num[0] == 0 and r.accepted.start_pos[0] == 8 and r.accepted.num[1] >= 1
+    s.take(r)
+    s.tables = torch.cat([s.tables, wide[:, 3:]], 1)
+    for _ in range(2):
+        done = [len(q) - len(p) for q, p in zip(s.seqs, prompts)]
+        s.take(_verify_chains(s, [x[n:n + 2] for x, n in zip(likely, done)], max_ctx=20))
+    assert _status() == 0
+    _check_sequences(s, prompts)
+
+
 # ------------------------------------------------- values that are not finite --
 
 def _with_value(c, dev, places, heads):
