@@ -286,7 +286,7 @@ PS_API int ps_sample_topk(int32_t* out_dev, const float* vals_dev, const int32_t
  * leaves it out), get mask 0: ps_accept_trees keeps nothing of them.
  * ps_build_step_tables_bounded treats contexts past max_ctx in the same way, for
  * a step whose attention is given that bound.
- * held_out must not alias held, seq_lens, q_lens. */
+ * No output may overlap an input, but for tables == tables_in. */
 PS_API int ps_build_step_tables(int32_t* tables_dev, int32_t* held_out_dev, int32_t* cu_q_dev, int32_t* positions_dev,
                                 int32_t* slots_dev, int64_t* tree_mask_dev, int32_t* free_used_dev,
                                 const int32_t* tables_in_dev, const int32_t* held_dev, const int32_t* seq_lens_dev,

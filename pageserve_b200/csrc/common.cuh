@@ -187,6 +187,15 @@ int* status_word(int tu);  // device status word of translation unit `tu`
 bool reserve_smem(const void* kern, int bytes, std::atomic<uint64_t>* done);
 // true for NULL or a pointer aligned to `bytes` (vector loads need it)
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+// a buffer of a call, and whether two of them share a byte (never for NULL)
+struct Range {
+  const void* at;
+  uintptr_t bytes;
+};
+inline bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && x < y + b.bytes && y < x + a.bytes;
+}
 }  // namespace ps_host
 
 // Translation-unit ids for the device status words.

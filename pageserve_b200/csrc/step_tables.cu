@@ -258,14 +258,25 @@ int ps_build_step_tables_bounded(int32_t* tables, int32_t* held_out, int32_t* cu
     ps_host::set_error("build_step_tables: null pointer");
     return PS_ERR_INVALID;
   }
-  if (held_out == held || held_out == seq_lens || held_out == q_lens) {
-    ps_host::set_error("build_step_tables: held_out must not be one of the inputs (every request reads them all)");
-    return PS_ERR_INVALID;
-  }
   if (parents && (max_q_len <= 0 || max_q_len > kMaxNodes)) {
     ps_host::set_error("build_step_tables: trees of 1 to %d nodes per request (max_q_len %d)", kMaxNodes, max_q_len);
     return max_q_len <= 0 ? PS_ERR_INVALID : PS_ERR_UNSUPPORTED;
   }
+  // A request's outputs are written while others still read their inputs; tables
+  // in place are the exception, for a request reads its own row alone.
+  const uintptr_t b4 = 4ull * num_seqs, t4 = 4ull * total_tokens, w4 = b4 * max_blocks;
+  const uintptr_t mask_bytes = parents ? 2 * t4 * ((max_q_len + 63) / 64) : 0;
+  const ps_host::Range ins[] = {{tables_in, w4}, {held, b4}, {seq_lens, b4}, {q_lens, b4},
+                                {free_blocks, 4ull * num_free}, {parents, t4}};
+  const ps_host::Range outs[] = {{tables, w4}, {held_out, b4}, {cu_q, b4 + 4}, {positions, t4}, {slots, t4},
+                                 {parents ? tree_mask : nullptr, mask_bytes}, {free_used, 4}};
+  for (const auto& out : outs)
+    for (const auto& in : ins)
+      if (ps_host::overlap(out, in) && !(out.at == tables && in.at == tables_in && tables == tables_in)) {
+        ps_host::set_error("build_step_tables: an output overlaps an input that other requests still read "
+                           "(tables may be tables_in itself, nothing else)");
+        return PS_ERR_INVALID;
+      }
   TablesParams p{};
   p.tables = tables;
   p.held_out = held_out;

@@ -81,7 +81,8 @@ def build_step_tables(seq_lens: torch.Tensor, q_lens: torch.Tensor, block_tables
     among its request's rows, -1 for none; a row's position is then its depth
     past seq_len, and tree_mask is made (max_q_len bounds q_lens, at most
     256). Without parents the rows are a chunk at seq_len + i. ``out`` takes
-    the tables; it may be block_tables itself. A free list that is too short
+    the tables; it may be block_tables itself, but must not overlap it or another
+    input in any other way. A free list that is too short
     leaves -1 entries and slots, free_used above F and device error 6; lengths
     beyond the given bounds are device error 5 (``_lib.raise_on_device_error``).
     In a tree the rows from the first one without a slot on get mask 0, as do
