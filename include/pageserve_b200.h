@@ -337,7 +337,7 @@ PS_API int ps_tree_attention(void* out_dev, const void* q_dev, const void* k_cac
  *   of the pool in the table is recorded (errors 1, 5); with the caches given,
  *   start_out then counts the nodes before it alone, for the rest is not in the
  *   cache. Rows behind start_out are left over.
- * num and start_out must not alias start_pos or cu_q, nor the caches each other.
+ * No output may overlap an input, nor the caches each other.
  * max_q_len <= 256. */
 PS_API int ps_accept_trees(int32_t* num_dev, int32_t* nodes_dev, int32_t* out_tokens_dev, int32_t* start_out_dev,
                            const int64_t* tokens_dev, const int32_t* targets_dev, const int64_t* tree_mask_dev,

@@ -221,10 +221,6 @@ extern "C" int ps_accept_trees(int32_t* num, int32_t* nodes, int32_t* out_tokens
     ps_host::set_error("accept_trees: null pointer");
     return PS_ERR_INVALID;
   }
-  if (start_out == start_pos || num == start_pos || start_out == cu_q || num == cu_q) {
-    ps_host::set_error("accept_trees: the outputs must not be the inputs (every block of a request reads them)");
-    return PS_ERR_INVALID;
-  }
   AcceptParams p{};
   int slices = 1;
   if (k_cache || v_cache) {
@@ -259,6 +255,17 @@ extern "C" int ps_accept_trees(int32_t* num, int32_t* nodes, int32_t* out_tokens
     const long long most = (kCtas + num_seqs - 1) / num_seqs;
     slices = static_cast<int>(want < most ? want : most);
   }
+  // a request's first block writes its outputs while the others read all inputs
+  const uintptr_t b4 = 4ull * num_seqs, t4 = 4ull * total_tokens;
+  const ps_host::Range ins[] = {{tokens, 2 * t4}, {targets, t4}, {tree_mask, 2 * t4 * ((max_q_len + 63) / 64)},
+                                {cu_q, b4 + 4}, {start_pos, b4}, {k_cache ? tables : nullptr, b4 * max_blocks}};
+  const ps_host::Range outs[] = {{num, b4}, {nodes, b4 * max_q_len}, {out_tokens, b4 * max_q_len}, {start_out, b4}};
+  for (const auto& out : outs)
+    for (const auto& in : ins)
+      if (ps_host::overlap(out, in)) {
+        ps_host::set_error("accept_trees: an output overlaps an input that other blocks still read");
+        return PS_ERR_INVALID;
+      }
   p.num = num;
   p.nodes = nodes;
   p.out_tokens = out_tokens;

@@ -44,3 +44,27 @@ def test_build_step_tables_refuses_shifted_tables():
     for shift in (-56, -28, 28, 56, 4):
         assert _tables(lib, tables=IN["tin"] + shift) == _lib.PS_ERR_INVALID
         assert "overlap" in _lib.last_error()
+
+
+ACC_IN = dict(tok=P + 0x1000, tgt=P + 0x2000, mask=P + 0x3000, cu=P + 0x4000, sp=P + 0x5000, tab=P + 0x6000)
+ACC_SIZE = dict(num=12, nodes=3 * 70 * 4, out=3 * 70 * 4, start_out=12, tok=320, tgt=160, mask=40 * 16, cu=16, sp=12,
+                tab=3 * 8 * 4)
+
+
+def _accept(lib, **kw):
+    a = dict(num=P + 0x10000, nodes=P + 0x11000, out=P + 0x12000, start_out=P + 0x13000, tok=0, tgt=0, mask=0, cu=0,
+             sp=0, B=3, T=40, max_q=70, k=P + 0x100000, v=P + 0x200000, tab=0, width=8, L=2, nb=16, bs=16, hkv=2, d=64,
+             dt=_lib.PS_BF16)
+    a.update(ACC_IN)
+    a.update(kw)
+    return lib.ps_accept_trees(*a.values(), None)
+
+
+@pytest.mark.parametrize("out", ["num", "nodes", "out", "start_out"])
+@pytest.mark.parametrize("src", list(ACC_IN))
+def test_accept_trees_refuses_outputs_over_inputs(out, src):
+    """One block of a request writes what the others still read."""
+    lib = _lib_or_skip()
+    for at in (ACC_IN[src] + ACC_SIZE[src] - 4, ACC_IN[src] - ACC_SIZE[out] + 4):
+        assert _accept(lib, **{out: at}) == _lib.PS_ERR_INVALID
+        assert "overlap" in _lib.last_error()
