@@ -313,7 +313,8 @@ PS_API size_t ps_tree_attention_workspace_size(int num_seqs, int max_q_len, int 
  * the cache already. Rows behind cu_q[num_seqs] are left as they were.
  * max_q_len <= 256 and max_ctx are host bounds; a request beyond them is
  * skipped and recorded (error 5). head_dim 64 or 128, PS_BF16 or PS_F16, any
- * block size; q, out and the caches 16-byte aligned; out must not overlap q. */
+ * block size; q, out and the caches 16-byte aligned; out and the workspace must
+ * not overlap an input or each other. */
 PS_API int ps_tree_attention(void* out_dev, const void* q_dev, const void* k_cache_dev, const void* v_cache_dev,
                              const int32_t* block_tables_dev, int max_blocks_per_seq, const int32_t* cu_q_dev,
                              const int32_t* start_pos_dev, const int64_t* tree_mask_dev, int num_seqs, int total_q,

@@ -1677,10 +1677,18 @@ int ps_tree_attention(void* out, const void* q, const void* k_cache, const void*
     ps_host::set_error("tree_attention: workspace of %zu bytes needed, %zu given", pl.bytes, workspace_bytes);
     return PS_ERR_INVALID;
   }
-  const uintptr_t q_at = reinterpret_cast<uintptr_t>(q), out_at = reinterpret_cast<uintptr_t>(out);
-  const uintptr_t span = static_cast<uintptr_t>(total_q) * Hq * D * 2;
-  if (q_at < out_at + span && out_at < q_at + span) {
-    ps_host::set_error("tree_attention: out overlaps q, which other blocks may still read");
+  const uintptr_t rows = static_cast<uintptr_t>(total_q) * Hq * D * 2, b4 = 4ull * num_seqs;
+  const uintptr_t cache = static_cast<uintptr_t>(num_blocks) * block_size * Hkv * D * 2;
+  const ps_host::Range ins[] = {{q, rows}, {k_cache, cache}, {v_cache, cache}, {tables, b4 * max_blocks},
+                                {cu_q, b4 + 4}, {start_pos, b4},
+                                {tree_mask, 8ull * total_q * ((max_q_len + 63) / 64)}};
+  const ps_host::Range outs[] = {{out, rows}, {workspace, pl.bytes}};
+  bool shared = ps_host::overlap(outs[0], outs[1]);
+  for (const auto& o : outs)
+    for (const auto& in : ins) shared |= ps_host::overlap(o, in);
+  if (shared) {
+    ps_host::set_error("tree_attention: out or the workspace overlaps q, another input that blocks may still read, "
+                       "or the other");
     return PS_ERR_INVALID;
   }
   TreeParams p{};

@@ -110,8 +110,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     int64 (total_q, ceil(max_q_len / 64)) from :func:`build_step_tables`.
     Node i of request b sees the cached keys [0, start_pos[b]) and the nodes
     of its mask row (stored at start_pos[b] + node); 0 when it sees nothing.
-    Rows of ``out`` (which must not overlap q) behind cu_q[-1] are left as
-    they were. A workspace serves calls on one stream at a time; without one
+    Rows of ``out`` (which must not overlap an input) behind cu_q[-1] are left
+    as they were. A workspace serves calls on one stream at a time; without one
     the scratch is allocated per call."""
     _lib.require_cuda(q)
     buf = None

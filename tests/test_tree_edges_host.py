@@ -68,3 +68,31 @@ def test_accept_trees_refuses_outputs_over_inputs(out, src):
     for at in (ACC_IN[src] + ACC_SIZE[src] - 4, ACC_IN[src] - ACC_SIZE[out] + 4):
         assert _accept(lib, **{out: at}) == _lib.PS_ERR_INVALID
         assert "overlap" in _lib.last_error()
+
+
+ATT_IN = dict(q=P + 0x10000, k=P + 0x40000, v=P + 0x80000, tab=P + 0x1000, cu=P + 0x2000, sp=P + 0x3000, mask=P + 0x4000)
+ATT_SIZE = dict(q=8 * 4 * 128 * 2, k=16 * 16 * 2 * 128 * 2, v=16 * 16 * 2 * 128 * 2, tab=2 * 8 * 4, cu=12, sp=8,
+                mask=64, out=8 * 4 * 128 * 2)
+
+
+def _attn(lib, **kw):
+    a = dict(out=P + 0x20000, **ATT_IN, B=2, T=8, max_q=4, max_ctx=100, nb=16, bs=16, hq=4, hkv=2, d=128,
+             dt=_lib.PS_BF16, ws=P + 0x1000000, wsb=1 << 24)
+    a = {k: a[k] for k in ("out", "q", "k", "v", "tab")} | {"width": 8} | {k: a[k] for k in list(a) if k not in (
+        "out", "q", "k", "v", "tab")}
+    a.update(kw)
+    return lib.ps_tree_attention(*a.values(), None)
+
+
+@pytest.mark.parametrize("src", list(ATT_IN))
+def test_tree_attention_refuses_outputs_over_inputs(src):
+    """Blocks finish at any time: what one writes another may still have to read."""
+    lib = _lib_or_skip()
+    last = (ATT_IN[src] + ATT_SIZE[src] - 1) // 16 * 16
+    for at in (last, last - ATT_SIZE["out"] + 16):
+        assert _attn(lib, out=at) == _lib.PS_ERR_INVALID
+        assert "overlap" in _lib.last_error()
+    for at in (last, last - 4096):
+        assert _attn(lib, ws=at) == _lib.PS_ERR_INVALID
+        assert "overlap" in _lib.last_error()
+    assert _attn(lib, ws=P + 0x20000 + 16) == _lib.PS_ERR_INVALID and "overlap" in _lib.last_error()
