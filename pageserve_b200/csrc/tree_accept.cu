@@ -66,11 +66,13 @@ __global__ void __launch_bounds__(kThreads) accept_trees_kernel(const AcceptPara
   const int b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31;
   const int q0 = p.cu_q[b];
-  const int n = p.cu_q[b + 1] - q0;
+  const long long rows = static_cast<long long>(p.cu_q[b + 1]) - q0;  // of any 32-bit numbers
   const int start = p.start_pos[b];
   const bool lead = blockIdx.x == 0;
-  const bool bad = n < 0 || n > p.max_q_len || q0 < 0 || start < 0 || q0 + n > p.total_tokens;
-  if (n <= 0 || bad) {
+  const bool bad = rows < 0 || rows > p.max_q_len || q0 < 0 || start < 0 || q0 + rows > p.total_tokens ||
+                   start + rows > INT32_MAX;
+  const int n = bad ? 0 : static_cast<int>(rows);
+  if (n == 0) {
     if (lead) {
       if (tid == 0) {
         p.num[b] = 0;

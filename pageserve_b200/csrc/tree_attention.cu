@@ -84,11 +84,11 @@ template <int KEYS>
 PS_DEVICE Seq make_seq(const TreeParams& p, int q0, int q1, int start, bool* bad) {
   Seq s;
   s.q0 = q0;
-  s.n = q1 - q0;
   s.start = start;
-  const long long ctx = static_cast<long long>(start) + s.n;
-  *bad = s.n != 0 && (s.n < 0 || s.n > p.max_q_len || q0 < 0 || q1 > p.total_q || start < 0 || ctx > p.max_ctx);
-  if (*bad) s.n = 0;
+  const long long n = static_cast<long long>(q1) - q0;  // of any 32-bit numbers
+  const long long ctx = start + n;
+  *bad = n != 0 && (n < 0 || n > p.max_q_len || q0 < 0 || q1 > p.total_q || start < 0 || ctx > p.max_ctx);
+  s.n = *bad ? 0 : static_cast<int>(n);
   s.row_groups = ((s.n * p.rg_mul + p.rg_add) * p.rg_magic) >> p.rg_shift;
   s.key_tiles = s.n ? (static_cast<int>(ctx) + KEYS - 1) / KEYS : 0;
   return s;

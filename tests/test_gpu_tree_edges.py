@@ -168,6 +168,49 @@ def test_verification_past_the_bounds_keeps_nothing(two_requests):
     _check_sequences(s, prompts)
 
 
+LO, HI = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("cu", [[HI - 2, LO + 2], [LO, LO + 3], [HI - 2, HI], [-1, 2], [4, 9], [3, 1], [LO, HI], [HI, LO]])
+def test_row_offsets_of_any_value(dev, cu):  # noqa: F811
+    """Row offsets that are out of range, or whose difference wraps to a small
+    number, are recorded and skipped."""
+    from pageserve_b200 import speculative as sp
+    c = _case(44, [30], [7], 16, 2, 128, 16, torch.bfloat16)
+    c["max_q"], c["cu"] = 7, np.asarray(cu)
+    for bs in (16, 4):
+        c["bs"] = bs
+        out = torch.full((7, 16, 128), 7.0, dtype=torch.bfloat16, device=dev)
+        _run(c, dev, out=out)
+        assert (out == 7).all() and _status() == 5
+        c["k"], c["v"] = (x.reshape(-1, 4, 2, 128) for x in (c["k"], c["v"]))
+        c["tab"] = np.zeros((1, 12), int)
+    k = torch.randn(1, 4, 4, 1, 8, device=dev)
+    v, k0 = -k, k.clone()
+    mask = torch.tensor([[(2 << i) - 1] for i in range(7)], device=dev)
+    tok = torch.zeros(7, dtype=torch.int64, device=dev)
+    r = sp.accept_trees(tok, tok.int(), mask, _i32(cu, dev), _i32([3], dev), 7, k, v, _i32([[0, 1, 2]], dev))
+    assert _status() == 5
+    assert r.num.tolist() == [0] and r.start_pos.tolist() == [3]
+    assert r.nodes.tolist() == [[-1] * 7] and r.tokens.tolist() == [[-1] * 7]
+    assert torch.equal(k, k0) and torch.equal(v, -k0)
+
+
+def test_start_positions_of_any_value(dev):  # noqa: F811
+    """A start whose sum with the rows passes 32 bits, and one below 0."""
+    from pageserve_b200 import speculative as sp
+    mask = torch.tensor([[(2 << i) - 1] for i in range(3)], device=dev)
+    tok = torch.zeros(3, dtype=torch.int64, device=dev)
+    for start in (HI, HI - 2, -1, LO):
+        for caches in ((), (torch.zeros(1, 4, 4, 1, 8, device=dev), torch.zeros(1, 4, 4, 1, 8, device=dev),
+                            _i32([[0, 1]], dev))):
+            r = sp.accept_trees(tok, tok.int(), mask, _i32([0, 3], dev), _i32([start], dev), 3, *caches)
+            assert _status() == 5
+            assert r.num.tolist() == [0] and r.start_pos.tolist() == [start] and r.tokens.tolist() == [[-1] * 3]
+    r = sp.accept_trees(tok, tok.int(), mask, _i32([0, 3], dev), _i32([HI - 3], dev), 3)
+    assert _status() == 0 and r.num.tolist() == [3] and r.start_pos.tolist() == [HI]
+
+
 # ------------------------------------------------- values that are not finite --
 
 def _with_value(c, dev, places, heads):
