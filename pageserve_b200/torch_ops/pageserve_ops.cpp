@@ -512,6 +512,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   return {at::empty(block_tables.sizes(), i32), at::empty({B}, i32), at::empty({B + 1}, i32), at::empty({T}, i32),
           at::empty({T}, i32), mask, at::empty({1}, i32)};
 }
+StepOut step_tables_out_meta(at::Tensor, const at::Tensor& seq_lens, const at::Tensor& q_lens,
+                             const at::Tensor& block_tables, const at::Tensor& held, const at::Tensor& free_blocks,
+                             int64_t num_blocks, int64_t block_size, int64_t T,
+                             const c10::optional<at::Tensor>& parents, c10::optional<int64_t> max_q_len,
+                             c10::optional<int64_t> max_ctx) {
+  auto r = step_tables_meta(seq_lens, q_lens, block_tables, held, free_blocks, num_blocks, block_size, T, parents,
+                            max_q_len, max_ctx);
+  return {std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r), std::get<5>(r), std::get<6>(r)};
+}
+void tree_attention_out_meta(at::Tensor, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t,
+                             const c10::optional<at::Tensor>&) {}
 at::Tensor tree_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                                const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t,
                                const c10::optional<at::Tensor>&) {
@@ -596,6 +608,8 @@ TORCH_LIBRARY_IMPL(pageserve_b200, Meta, m) {
   m.impl("argmax", &argmax_meta);
   m.impl("topk", &topk_meta);
   m.impl("build_step_tables", &step_tables_meta);
+  m.impl("build_step_tables_out", &step_tables_out_meta);
   m.impl("tree_attention", &tree_attention_meta);
+  m.impl("tree_attention_out", &tree_attention_out_meta);
   m.impl("accept_trees", &accept_meta);
 }

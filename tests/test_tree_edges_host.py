@@ -2,6 +2,7 @@
 shapes for tracing, scratch that captured calls go on using."""
 
 import pytest
+import torch
 
 from pageserve_b200 import _lib
 
@@ -96,3 +97,31 @@ def test_tree_attention_refuses_outputs_over_inputs(src):
         assert _attn(lib, ws=at) == _lib.PS_ERR_INVALID
         assert "overlap" in _lib.last_error()
     assert _attn(lib, ws=P + 0x20000 + 16) == _lib.PS_ERR_INVALID and "overlap" in _lib.last_error()
+
+
+def test_out_forms_have_meta_functions():
+    """Fake-tensor tracing of the forms that write into a given tensor (the
+    model's step calls one)."""
+    from pageserve_b200 import ops as torch_ops
+    if not torch_ops.LIB_PATH.exists():
+        pytest.skip("libpageserve_torch_ops.so is not built")
+    ns = torch_ops.load()
+    i = lambda *s: torch.empty(s, dtype=torch.int32, device="meta")  # noqa: E731
+    r = ns.build_step_tables_out(i(3, 7), i(3), i(3), i(3, 7), i(3), i(9), 9, 16, 20, i(20), 70)
+    assert [tuple(x.shape) for x in r] == [(3,), (4,), (20,), (20,), (20, 2), (1,)]
+    assert [x.dtype for x in r] == [torch.int32] * 4 + [torch.int64, torch.int32]
+    r = ns.build_step_tables_out(i(3, 7), i(3), i(3), i(3, 7), i(3), i(9), 9, 16, 20)
+    assert r[4].shape == (0,)
+    q = torch.empty(20, 4, 64, dtype=torch.bfloat16, device="meta")
+    kv = torch.empty(9, 16, 2, 64, dtype=torch.bfloat16, device="meta")
+    mask = torch.empty(20, 2, dtype=torch.int64, device="meta")
+    assert ns.tree_attention_out(torch.empty_like(q), q, kv, kv, i(3, 7), i(4), i(3), mask, 70, 112) is None
+
+
+def test_every_operator_has_a_meta_function():
+    from pageserve_b200 import ops as torch_ops
+    if not torch_ops.LIB_PATH.exists():
+        pytest.skip("libpageserve_torch_ops.so is not built")
+    torch_ops.load()
+    for name in ("build_step_tables", "build_step_tables_out", "tree_attention", "tree_attention_out", "accept_trees"):
+        assert torch._C._dispatch_has_kernel_for_dispatch_key(f"pageserve_b200::{name}", "Meta"), name
