@@ -8,6 +8,7 @@
 // (engine/paged_attention.py, engine/quantization.py, engine/model.py); the
 // batched forms take device-resident int32 metadata (graph-capturable).
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -265,28 +266,11 @@ int int_arg(int64_t v, const char* what) {
   return static_cast<int>(v);
 }
 
-// The outputs of one call, cut from one allocation: an allocation costs about
-// a microsecond of the host's time, as much as a small step's kernel takes, and
-// build_step_tables has seven outputs. They share a storage, not an element.
-class Outputs {
- public:
-  Outputs(int64_t bytes, const at::TensorOptions& opt)
-      : base_(at::empty({bytes}, opt.dtype(at::kByte))) {}
-  static int64_t size(int64_t n, int64_t item) { return (n * item + 15) / 16 * 16; }
-  at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
-    const int64_t item = static_cast<int64_t>(c10::elementSize(type));
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(),
-                                                            c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_storage_offset(off_ / item);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    off_ += size(t.numel(), item);
-    return t;
-  }
-
- private:
-  at::Tensor base_;
-  int64_t off_ = 0;
-};
+// An output of its own storage (operators' outputs must not alias, and a caller
+// keeps some of them), without at::empty's dispatch: build_step_tables has seven.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, dev, c10::nullopt));
+}
 
 using StepOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
@@ -318,14 +302,11 @@ StepOut step_tables_call(at::Tensor& out, const at::Tensor& seq_lens, const at::
     words = (std::max<int64_t>(*max_q_len, 0) + 63) / 64;
   }
   c10::cuda::CUDAGuard g(dev);
-  const int64_t mask_rows = parents.has_value() ? T : 0;
-  Outputs o(Outputs::size(mask_rows * words, 8) + 2 * Outputs::size(T, 4) + Outputs::size(B, 4) +
-                Outputs::size(B + 1, 4) + Outputs::size(1, 4) + (out.defined() ? 0 : Outputs::size(block_tables.numel(), 4)),
-            seq_lens.options());
-  at::Tensor mask = parents.has_value() ? o.take({T, words}, at::kLong) : o.take({0}, at::kLong);
-  at::Tensor positions = o.take({T}, at::kInt), slots = o.take({T}, at::kInt), held_out = o.take({B}, at::kInt);
-  at::Tensor cu_q = o.take({B + 1}, at::kInt), used = o.take({1}, at::kInt);
-  if (!out.defined()) out = o.take(block_tables.sizes(), at::kInt);
+  at::Tensor mask = parents.has_value() ? fresh({T, words}, at::kLong, dev) : fresh({0}, at::kLong, dev);
+  at::Tensor positions = fresh({T}, at::kInt, dev), slots = fresh({T}, at::kInt, dev);
+  at::Tensor held_out = fresh({B}, at::kInt, dev), cu_q = fresh({B + 1}, at::kInt, dev);
+  at::Tensor used = fresh({1}, at::kInt, dev);
+  if (!out.defined()) out = fresh(block_tables.sizes(), at::kInt, dev);
   check_v(ps_build_step_tables_bounded(
               out.data_ptr<int32_t>(), held_out.data_ptr<int32_t>(), cu_q.data_ptr<int32_t>(),
               positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
@@ -448,9 +429,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> accept_trees(
   }
   c10::cuda::CUDAGuard g(dev);
   const int64_t wide = std::max<int64_t>(max_q_len, 0);  // the C call refuses 0 and below
-  Outputs o(2 * Outputs::size(B, 4) + 2 * Outputs::size(B * wide, 4), start_pos.options());
-  at::Tensor num = o.take({B}, at::kInt), start = o.take({B}, at::kInt);
-  at::Tensor nodes = o.take({B, wide}, at::kInt), out = o.take({B, wide}, at::kInt);
+  at::Tensor num = fresh({B}, at::kInt, dev), start = fresh({B}, at::kInt, dev);
+  at::Tensor nodes = fresh({B, wide}, at::kInt, dev), out = fresh({B, wide}, at::kInt, dev);
   check_v(ps_accept_trees(num.data_ptr<int32_t>(), nodes.data_ptr<int32_t>(), out.data_ptr<int32_t>(),
                           start.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), targets.data_ptr<int32_t>(),
                           tree_mask.data_ptr<int64_t>(), cu_q.data_ptr<int32_t>(), start_pos.data_ptr<int32_t>(),

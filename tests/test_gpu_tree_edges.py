@@ -273,3 +273,19 @@ def test_attention_infinity_of_small_weight(dev, D, bs, nodes, ctx, dtype):  # n
         col = _with_value(c, dev, [(key, float("inf"))], 4)
         assert (col == float("inf")).all(), key
     assert _status() == 0
+
+
+# ------------------------------------------------------------- the operators --
+
+def test_outputs_are_tensors_of_their_own(dev):  # noqa: F811
+    """No two outputs share a storage: what a caller keeps for the next step
+    holds no other output, and tracing may free each by itself."""
+    from pageserve_b200 import speculative as sp
+    i, tab = _i32([3, 5], dev), _i32([[0, -1], [1, -1]], dev)
+    t = sp.build_step_tables(i, _i32([2, 1], dev), tab, _i32([1, 1], dev), _i32([2, 3], dev), 4, 16, 3,
+                             parents=_i32([-1, 0, -1], dev), max_q_len=2)
+    a = sp.accept_trees(torch.tensor([1, 2, 3], device=dev), _i32([2, 3, 4], dev), t.tree_mask, t.cu_q, i, 2)
+    for outs in (t, a, sp.build_step_tables(i, _i32([2, 1], dev), tab, _i32([1, 1], dev), _i32([2, 3], dev), 4, 16, 3)):
+        outs = [x for x in outs if x is not None]
+        assert len({x.untyped_storage().data_ptr() for x in outs}) == len(outs)
+        assert all(x.untyped_storage().nbytes() == x.numel() * x.element_size() for x in outs)
