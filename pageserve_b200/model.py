@@ -468,7 +468,9 @@ class PagedCausalLM:
                                                  stream), "build_slot_mapping")
             runs = attention_runs(meta.q_lens, hq // hkv)
         q = torch.empty((T, hq, d), dtype=self.dtype, device=self.device)
-        attn = torch.empty((T, hq, d), dtype=self.dtype, device=self.device)
+        # tree attention leaves padding rows, and requests past its bounds, as they are: zeros
+        attn = (torch.zeros if isinstance(meta, TreeMeta) else torch.empty)((T, hq, d), dtype=self.dtype,
+                                                                            device=self.device)
         num_slots = self.num_blocks * self.block_size
         comm = self.comm  # fused TP reduction: o_proj -> set 0, down_proj -> set 1, consumed by the next norm
         if comm is not None and T > comm.max_tokens:
@@ -641,7 +643,8 @@ class PagedCausalLM:
         blocks the step may take. max_q_len bounds q_lens (at most 256),
         max_ctx seq_lens + q_lens (default: what a table row holds; a closer
         bound spares short steps the joining of key ranges). Rows
-        behind the last request are padding (any token of the vocabulary).
+        behind the last request are padding (any token of the vocabulary): their
+        logits and targets mean nothing, but are the same every time.
 
         The confirmed tokens of the step are ``accepted.tokens[b,
         :accepted.num[b]]``, the same as that many single-token greedy steps

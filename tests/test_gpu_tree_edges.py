@@ -168,6 +168,27 @@ def test_verification_past_the_bounds_keeps_nothing(two_requests):
     _check_sequences(s, prompts)
 
 
+def test_padding_rows_are_the_same_every_time(dev):  # noqa: F811
+    """Rows behind the last request have defined results, whatever the memory
+    held before."""
+    m = _model(torch.bfloat16, True, 16, 16)
+    s = _Requests(m, [np.arange(20), np.arange(5)], 4, range(16), dev)
+    tok = torch.arange(9, device=dev)
+    par = torch.full((9,), -1, dtype=torch.int32, device=dev)
+    q = torch.ones(2, dtype=torch.int32, device=dev)
+    got = []
+    for fill in (float("nan"), 3.0):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        junk = [torch.full((2 ** k,), fill, dtype=torch.bfloat16, device=dev) for k in range(8, 22) for _ in range(4)]
+        del junk
+        got.append(m.verify_trees(tok, par, s.cached, q, s.tables, s.held, s.free, 1, return_logits=True))
+    for r in got:
+        assert torch.isfinite(r.logits).all()
+    assert torch.equal(got[0].logits, got[1].logits) and torch.equal(got[0].targets, got[1].targets)
+    assert _status() == 0
+
+
 LO, HI = -2 ** 31, 2 ** 31 - 1
 
 
