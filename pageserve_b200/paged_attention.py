@@ -72,19 +72,37 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, block_s
     return flat_k.index_select(0, slots), flat_v.index_select(0, slots)
 
 
-class AttentionWorkspace:
-    """Grow-only scratch buffer for split-context partials (reused across
-    calls; allocate it before capturing a CUDA graph)."""
+class Workspace:
+    """Grow-only scratch buffer, reused across calls. A buffer that a later
+    call outgrows is kept as long as the workspace: a captured CUDA graph holds
+    its address. Each is at least twice the last, so that what is kept is less
+    than what is in use."""
 
     def __init__(self):
         self.buf: torch.Tensor | None = None
+        self._outgrown: list[torch.Tensor] = []
+
+    def _new(self, nbytes: int, device) -> torch.Tensor:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
     def get(self, nbytes: int, device) -> torch.Tensor | None:
         if nbytes == 0:
             return None
         if self.buf is None or self.buf.numel() < nbytes or self.buf.device != torch.device(device):
-            self.buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            if self.buf is not None:
+                self._outgrown.append(self.buf)
+                nbytes = max(nbytes, 2 * self.buf.numel())
+            self.buf = self._new(nbytes, device)
         return self.buf
+
+    def nbytes(self) -> int:
+        """Bytes held, outgrown buffers among them."""
+        return sum(b.numel() for b in self._outgrown) + (0 if self.buf is None else self.buf.numel())
+
+
+class AttentionWorkspace(Workspace):
+    """Scratch for split-context partials (allocate it before capturing a CUDA
+    graph)."""
 
 
 _default_ws: dict[torch.device, AttentionWorkspace] = {}

@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .paged_attention import Workspace
 
 
 def _cuda_device(t: torch.Tensor) -> torch.device:
@@ -49,22 +50,15 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torc
     return (q.to(torch.float32) * scale).to(dtype)
 
 
-class LinearWorkspace:
-    """Grow-only scratch buffer of the tensor-core linear: the float32
+class LinearWorkspace(Workspace):
+    """Scratch of the tensor-core linear: the float32
     partial tiles that the split-K CTAs of an output tile exchange through L2
     (each call writes every slot it reads, so no clearing is needed). One
     buffer serves all the linears of a step (calls on one stream only);
     without it the splits reduce through shared memory, more slowly."""
 
-    def __init__(self):
-        self.buf: torch.Tensor | None = None
-
-    def get(self, nbytes: int, device) -> torch.Tensor | None:
-        if nbytes == 0:
-            return None
-        if self.buf is None or self.buf.numel() < nbytes or self.buf.device != torch.device(device):
-            self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-        return self.buf
+    def _new(self, nbytes: int, device) -> torch.Tensor:
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
 
 
 _default_ws: dict[torch.device, LinearWorkspace] = {}

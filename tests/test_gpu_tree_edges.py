@@ -310,3 +310,34 @@ def test_outputs_are_tensors_of_their_own(dev):  # noqa: F811
         outs = [x for x in outs if x is not None]
         assert len({x.untyped_storage().data_ptr() for x in outs}) == len(outs)
         assert all(x.untyped_storage().nbytes() == x.numel() * x.element_size() for x in outs)
+
+
+def test_captured_call_keeps_its_scratch(dev):  # noqa: F811
+    """A graph that was captured with a workspace goes on being right when a
+    larger call has outgrown it, and writes nowhere else."""
+    from pageserve_b200 import speculative as sp
+    from pageserve_b200.paged_attention import AttentionWorkspace
+    c = _case(45, [700, 300], [8, 30], 16, 2, 128, 16, torch.bfloat16)
+    want = _run(c, dev)
+    q, k, v = (c[x].to(dev) for x in "qkv")
+    a = (_i32(c["tab"], dev), _i32(c["cu"], dev), _i32(c["sp"], dev),
+         torch.from_numpy(tree.mask_words(c["sets"], 1)).to(dev), 30, 708)
+    out, ws = torch.zeros_like(q), AttentionWorkspace()
+    sp.tree_attention(q, k, v, *a, out=out, workspace=ws)
+    size = ws.buf.numel()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        sp.tree_attention(q, k, v, *a, out=out, workspace=ws)
+    big = _case(46, [5000] * 8, [40] * 8, 40, 8, 128, 16, torch.bfloat16)
+    for _ in range(2):
+        _run(big, dev, workspace=ws)
+    assert ws.buf.numel() > size
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    other = [torch.full((size,), 77, dtype=torch.uint8, device=dev) for _ in range(4)]
+    out.zero_()
+    g.replay()
+    assert torch.equal(out, want)
+    assert all((x == 77).all() for x in other)
+    assert _status() == 0

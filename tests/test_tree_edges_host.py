@@ -1,10 +1,14 @@
 """Drafted-tree operators without a GPU: refusals of buffers that overlap,
 shapes for tracing, scratch that captured calls go on using."""
 
+import weakref
+
 import pytest
 import torch
 
 from pageserve_b200 import _lib
+from pageserve_b200.paged_attention import AttentionWorkspace
+from pageserve_b200.quantization import LinearWorkspace
 
 P = 1 << 20  # an aligned address that no check reads
 
@@ -97,6 +101,23 @@ def test_tree_attention_refuses_outputs_over_inputs(src):
         assert _attn(lib, ws=at) == _lib.PS_ERR_INVALID
         assert "overlap" in _lib.last_error()
     assert _attn(lib, ws=P + 0x20000 + 16) == _lib.PS_ERR_INVALID and "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kind", [AttentionWorkspace, LinearWorkspace])
+def test_workspace_keeps_what_it_outgrew(kind):
+    """A captured graph holds the scratch's address, not the tensor: a later,
+    larger call must not free it."""
+    ws = kind()
+    first = weakref.ref(ws.get(1000, "cpu"))
+    assert ws.get(500, "cpu") is first() and ws.get(0, "cpu") is None
+    second = weakref.ref(ws.get(1001, "cpu"))
+    assert second() is not first() and second().numel() >= 1001
+    assert first() is not None
+    # whatever the steps in which it grows, what is kept is bounded by the last one
+    for n in range(1100, 200000, 700):
+        assert ws.get(n, "cpu").numel() >= n
+    assert first() is not None and second() is not None
+    assert ws.nbytes() <= 4 * 200000
 
 
 def test_out_forms_have_meta_functions():
