@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import tree
-from test_gpu_speculative import _case, _i32, _run, _status, dev  # noqa: F401
+from test_gpu_speculative import _case, _gpu_reference, _i32, _run, _status, dev  # noqa: F401
 from test_gpu_verify_trees import _model, _Requests, near_tie
 
 pytestmark = pytest.mark.gpu
@@ -294,6 +294,62 @@ def test_attention_infinity_of_small_weight(dev, D, bs, nodes, ctx, dtype):  # n
         col = _with_value(c, dev, [(key, float("inf"))], 4)
         assert (col == float("inf")).all(), key
     assert _status() == 0
+
+
+# ------------------------------------------------------- errors on average --
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ctxs,nodes,Hq,Hkv,D,bs", [
+    ([300, 5, 511], [33, 64, 1], 16, 2, 128, 16), ([700, 130, 64], [7, 8, 2], 16, 2, 128, 16),
+    ([5000, 1, 2048, 700], [3, 1, 8, 11], 14, 2, 64, 16), ([900, 77], [12, 50], 40, 8, 128, 4),
+    ([6000], [40], 40, 8, 128, 16)])
+def test_attention_error_on_average(dev, ctxs, nodes, Hq, Hkv, D, bs, dtype):  # noqa: F811
+    """Roundings are independent, so their mean square adds up. With u half a
+    step of the type: rounding a weight w is off by at most u w and, spread
+    evenly, by u w / sqrt(3) in the mean, and so is the output o. The mean of
+    err^2 / (u^2 / 3 (sum w^2 v^2 + o^2)) is then at most 1 and, as a value lies
+    anywhere between two powers of two, about 1/2 (half steps are between u/2 and
+    u of a value). f16 weights of 2^-14 of the reference power or less are off
+    by up to 2^-25 of it, the sum being at least 1/2 of it: 2^-24 v each. Scores
+    are off by a few 2^-22, below 1% of u. So the root is below 1; a second
+    rounding of P, or f16 weights taken through bf16, would give 1.2 or 8."""
+    c = _case(43, ctxs, nodes, Hq, Hkv, D, bs, dtype)
+    got = _run(c, dev).double()
+    ref, _ = _gpu_reference(c, dev)
+    sq, count = _gpu_squares(c, dev)
+    u = torch.finfo(dtype).eps / 2
+    var = u * u / 3 * (sq + ref * ref)
+    if dtype == torch.float16:
+        var = var + count * (2.0 ** -24) ** 2 / 3
+    z = float(((got - ref) ** 2 / var).mean().sqrt())
+    assert z < 1.0, z
+    assert _status() == 0
+
+
+def _gpu_squares(c, dev):  # noqa: F811
+    """Of every output: the sum of w^2 v^2, and the sum of v^2 of the weights
+    that 16 bits hold with a fixed step, in 64 bits."""
+    q, k, v = (c[x].to(dev) for x in "qkv")
+    hq, d = q.shape[1:]
+    hkv, bs = k.shape[2], c["bs"]
+    sqs, counts = [], []
+    for b, n0 in enumerate(c["sp"]):
+        a, e = int(c["cu"][b]), int(c["cu"][b + 1])
+        n = e - a
+        pos = torch.arange(n0 + n, device=dev)
+        row = torch.as_tensor(c["tab"][b], device=dev)
+        kb, vb = (x[row[pos // bs], pos % bs].double().permute(1, 0, 2) for x in (k, v))
+        qb = q[a:e].double().reshape(n, hkv, hq // hkv, d).permute(1, 2, 0, 3)
+        s = torch.einsum("hgnd,hkd->hgnk", qb, kb) / np.sqrt(d)
+        sees = torch.zeros(n, n, dtype=torch.bool)
+        for i, x in enumerate(c["sets"][a:e]):
+            sees[i, list(x)] = True
+        s[..., n0:].masked_fill_(~sees.to(dev), -float("inf"))
+        w = torch.softmax(s, -1)
+        small = ((w < 2.0 ** -13) & (w > 0)).double()
+        sqs.append(torch.einsum("hgnk,hkd->hgnd", w * w, vb * vb).permute(2, 0, 1, 3).reshape(n, hq, d))
+        counts.append(torch.einsum("hgnk,hkd->hgnd", small, vb * vb).permute(2, 0, 1, 3).reshape(n, hq, d))
+    return torch.cat(sqs), torch.cat(counts)
 
 
 # ------------------------------------------------------------- the operators --
