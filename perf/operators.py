@@ -211,7 +211,7 @@ def prepare(case, seed):
             tab[b, :h] = perm[at:at + h]
             at += h
         s.update(q_lens=_i32(q), tables=_i32(tab), held=_i32(held), free=_i32(perm[at:]), num_blocks=num_blocks,
-                 total=T + _pad_rows(case), parents=None)
+                 total=T + _pad_rows(case), parents=None, no_mask=torch.zeros(0, dtype=torch.long, device=DEV))
         if case["tree"]:
             par = np.full(s["total"], -1, np.int32)
             cu = _cu(q)
@@ -385,7 +385,7 @@ def run(s):
         r = speculative.build_step_tables(s["seq_lens"], s["q_lens"], s["tables"], s["held"], s["free"],
                                           s["num_blocks"], s["bs"], s["total"], parents=s["parents"],
                                           max_q_len=s["max_q"])
-        mask = r.tree_mask if r.tree_mask is not None else s["seq_lens"].new_zeros(0, dtype=torch.long)
+        mask = r.tree_mask if r.tree_mask is not None else s["no_mask"]
         return r.block_tables, r.held, r.cu_q, r.positions, r.slots, mask, r.free_used
     if s["op"] == "attn":
         return speculative.tree_attention(s["q"], s["k"], s["v"], s["tables"], s["cu_q"], s["seq_lens"], s["mask"],
