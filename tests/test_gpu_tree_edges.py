@@ -271,6 +271,29 @@ def test_attention_cached_infinities_of_both_signs(dev, D, bs, nodes):  # noqa: 
     assert torch.isnan(col).all()
 
 
+@pytest.mark.parametrize("D,bs,nodes", [(128, 16, 6), (64, 16, 20), (128, 4, 6)])
+def test_attention_infinities_in_the_cache_and_in_a_node(dev, D, bs, nodes):  # noqa: F811
+    """Rows that see the node get NaN of both signs, the others keep the cache's."""
+    for ctx in (50, 900):
+        c = _case(47, [ctx, 40], [nodes, 5], 8, 2, D, bs, torch.bfloat16)
+        sees = torch.tensor([2 in x for x in c["sets"][:nodes]])
+        col = _with_value(c, dev, [(ctx // 3, float("-inf")), (ctx + 2, float("inf"))], 4)
+        assert torch.isnan(col[sees]).all() and (col[~sees] == float("-inf")).all()
+        assert sees.any() and not sees.all()
+
+
+@pytest.mark.parametrize("D,bs,n", [(128, 16, 8), (64, 16, 40), (128, 4, 8)])
+def test_attention_many_infinities(dev, D, bs, n):  # noqa: F811
+    """Every row of many segments of a CTA is looked at again."""
+    rng = np.random.default_rng(48)
+    c = _case(48, rng.integers(1, 900, 60).tolist(), [n] * 60, 40, 8, D, bs, torch.bfloat16)
+    for b in range(60):
+        c["v"][c["tab"][b, 0], 0] = float("inf")
+    for _ in range(3):
+        assert torch.isposinf(_run(c, dev)).all()
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D,bs,nodes,ctx", [(128, 16, 6, 700), (64, 16, 20, 700), (128, 4, 6, 700), (128, 16, 6, 6000),
                                             (128, 4, 20, 6000)])
