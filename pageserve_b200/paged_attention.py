@@ -73,14 +73,14 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, block_s
 
 
 class Workspace:
-    """Grow-only scratch buffer, reused across calls. A buffer that a later
-    call outgrows is kept as long as the workspace: a captured CUDA graph holds
-    its address. Each is at least twice the last, so that what is kept is less
-    than what is in use."""
+    """Grow-only scratch buffer, reused across calls (one per device). A buffer
+    that a later call outgrows is kept as long as the workspace: a captured CUDA
+    graph holds its address. Each is at least twice the last, so that what is
+    kept is less than what is in use."""
 
     def __init__(self):
-        self.buf: torch.Tensor | None = None
-        self._outgrown: list[torch.Tensor] = []
+        self.buf: torch.Tensor | None = None  # the last one handed out
+        self._bufs: dict[torch.device, list[torch.Tensor]] = {}
 
     def _new(self, nbytes: int, device) -> torch.Tensor:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -88,16 +88,20 @@ class Workspace:
     def get(self, nbytes: int, device) -> torch.Tensor | None:
         if nbytes == 0:
             return None
-        if self.buf is None or self.buf.numel() < nbytes or self.buf.device != torch.device(device):
-            if self.buf is not None:
-                self._outgrown.append(self.buf)
-                nbytes = max(nbytes, 2 * self.buf.numel())
-            self.buf = self._new(nbytes, device)
+        if self.buf is not None and self.buf.numel() >= nbytes and self.buf.device == device:
+            return self.buf
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        bufs = self._bufs.setdefault(device, [])
+        if not bufs or bufs[-1].numel() < nbytes:
+            bufs.append(self._new(max(nbytes, 2 * bufs[-1].numel()) if bufs else nbytes, device))
+        self.buf = bufs[-1]
         return self.buf
 
     def nbytes(self) -> int:
         """Bytes held, outgrown buffers among them."""
-        return sum(b.numel() for b in self._outgrown) + (0 if self.buf is None else self.buf.numel())
+        return sum(b.numel() for bufs in self._bufs.values() for b in bufs)
 
 
 class AttentionWorkspace(Workspace):

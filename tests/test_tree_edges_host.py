@@ -120,6 +120,15 @@ def test_workspace_keeps_what_it_outgrew(kind):
     assert ws.nbytes() <= 4 * 200000
 
 
+def test_workspace_of_several_devices():
+    """A call on another device neither frees nor grows what the first one has."""
+    ws = AttentionWorkspace()
+    a, b = ws.get(1000, "cpu"), ws.get(600, "meta")
+    for _ in range(50):
+        assert ws.get(1000, torch.device("cpu")) is a and ws.get(600, torch.device("meta")) is b
+    assert ws.nbytes() == 1600
+
+
 def test_out_forms_have_meta_functions():
     """Fake-tensor tracing of the forms that write into a given tensor (the
     model's step calls one)."""
