@@ -13,8 +13,8 @@
 // the keys of the first are stored nowhere, the second has no attention, and a node whose mask row is
 // empty is never accepted, nor is one behind it.
 //
-// Bound by latency (captured: 2.9 us for one request, 4.5 for 64 trees of up to 16
-// nodes, 6.2 for 513 requests with tables of 2049 entries, whose 4.2 MB would take
+// Bound by latency (captured: 2.9 us for one request, 4.3 for 64 trees of up to 16
+// nodes, 6.1 for 513 requests with tables of 2049 entries, whose 4.2 MB would take
 // 1.0 us): the bytes are a few kilobytes to a few megabytes. One
 // launch, one CTA per request; each CTA sums take and q over the requests
 // before its own, which costs 3 coalesced loads per 256 requests from L2 and

@@ -13,11 +13,11 @@
 // other thread. The cache ends (start_out) before the first node of the path
 // whose row, or whose place, lies in no block of the pool.
 //
-// Bound by latency for few requests (a chain of five dependent loads), by HBM
-// for many: 32 requests moving 6 tokens of 64 layers x 2 x 2 KB rows read and
-// write 101 MB in 18.0 us back to back (5.6 TB/s). Every CTA of a request finds
-// the path again (at most 256 nodes, three barriers), which is cheaper than a
-// second launch.
+// Bound by latency for few requests (a chain of five dependent loads), by the
+// move for many: 32 requests moving 6 tokens of 64 layers x 2 x 2 KB rows read
+// and write 101 MB in 18.2 us back to back, most of it in L2, and in 26.6 from
+// HBM (3.8 TB/s, the chain included). Every CTA of a request finds the path
+// again (at most 256 nodes, four barriers), which is cheaper than a second launch.
 #include "common.cuh"
 
 namespace {
@@ -252,7 +252,7 @@ extern "C" int ps_accept_trees(int32_t* num, int32_t* nodes, int32_t* out_tokens
     // One unit per thread, unless that is more than kCtas CTAs, whose finding of
     // the path would then cost more than their loads overlap: 32 trees of 61 nodes
     // over 64 layers x 2 x 2 KB rows took 22.0 us as 2048 CTAs, 18.0 as 1184 and
-    // 20.2 as 296 (back to back; 31.6, 28.7 and 28.7 from a cold L2).
+    // 20.2 as 296 (back to back, in L2; 31.6, 28.7 and 28.7 from HBM).
     const long long want = (2LL * num_layers * p.row_units + kThreads - 1) / kThreads;
     const long long most = (kCtas + num_seqs - 1) / num_seqs;
     slices = static_cast<int>(want < most ? want : most);

@@ -103,7 +103,8 @@ PS_DEVICE Seq seq_of(const TreeParams& p, int b) {
 // shares cut row groups, which then have to be joined; where whole row groups,
 // an equal number per CTA, take at most kJoinCost key tiles longer, they are not
 // cut (64 sequences x 2 heads at equal contexts: 17 key tiles per CTA against 15
-// and a joining of about 6 us; a key tile takes 1.3 us). A share may be a single
+// and a joining of about 6 us; a key tile takes 1.3 us; that case has doubled rows,
+// and the bound serves the other forms too, unmeasured there). A share may be a single
 // key tile: of at least 4, one request of 64 nodes at context 2000 (16 / 2 heads)
 // took 15.3 us instead of 12.9, four of up to 40 nodes at 300 to 2000 20.9 instead
 // of 15.4.
