@@ -74,34 +74,36 @@ def gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, block_s
 
 class Workspace:
     """Grow-only scratch buffer, reused across calls (one per device). A buffer
-    that a later call outgrows is kept as long as the workspace: a captured CUDA
-    graph holds its address. Each is at least twice the last, so that what is
-    kept is less than what is in use."""
+    that was handed out while a CUDA graph was captured is kept as long as the
+    workspace, though a later call outgrows it: the graph holds its address."""
 
     def __init__(self):
         self.buf: torch.Tensor | None = None  # the last one handed out
-        self._bufs: dict[torch.device, list[torch.Tensor]] = {}
+        self._bufs: dict[torch.device, torch.Tensor] = {}
+        self._captured: list[torch.Tensor] = []
 
     def _new(self, nbytes: int, device) -> torch.Tensor:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
+    @staticmethod
+    def _capturing(buf: torch.Tensor) -> bool:
+        return buf.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def get(self, nbytes: int, device) -> torch.Tensor | None:
         if nbytes == 0:
             return None
-        if self.buf is not None and self.buf.numel() >= nbytes and self.buf.device == device:
-            return self.buf
-        device = torch.device(device)
-        if device.type == "cuda" and device.index is None:
-            device = torch.device("cuda", torch.cuda.current_device())
-        bufs = self._bufs.setdefault(device, [])
-        if not bufs or bufs[-1].numel() < nbytes:
-            bufs.append(self._new(max(nbytes, 2 * bufs[-1].numel()) if bufs else nbytes, device))
-        self.buf = bufs[-1]
-        return self.buf
-
-    def nbytes(self) -> int:
-        """Bytes held, outgrown buffers among them."""
-        return sum(b.numel() for bufs in self._bufs.values() for b in bufs)
+        buf = self.buf
+        if buf is None or buf.numel() < nbytes or buf.device != device:
+            device = torch.device(device)
+            if device.type == "cuda" and device.index is None:
+                device = torch.device("cuda", torch.cuda.current_device())
+            buf = self._bufs.get(device)
+            if buf is None or buf.numel() < nbytes:
+                buf = self._bufs[device] = self._new(nbytes, device)
+            self.buf = buf
+        if self._capturing(buf) and not any(b is buf for b in self._captured):
+            self._captured.append(buf)
+        return buf
 
 
 class AttentionWorkspace(Workspace):
